@@ -546,6 +546,99 @@ int32_t ucmx_kvstar_scores(const void* reps_f16, int32_t n_slots, int32_t M, int
                            const int64_t* pruned_index, void* workspace, size_t workspace_bytes,
                            float* out_scores, ucmx_stream_t stream);
 
+/* ---------------------------------------------------------------- quantised paged KV cache
+ * (No counterpart in the reference, which keeps and moves blocks in the cache's own type.)
+ * A paged cache of 4- or 8-bit codes, one uint8 array of blocks; K and V of a block lie together, so a block is one
+ * contiguous slice for ucmx_gather_blocks, ucmx_move_blocks and the stores.
+ *
+ * Values: a row is one token's K (or V) of one KV head.  With L = 2^bits - 1:
+ *   zero = smallest value of the row;  scale = bf16((largest - smallest) / L);  code = (x - zero) / scale rounded to the
+ *   nearest integer (ties to even), at most L; all 0 where scale is 0.  A code stands for code*scale + zero.
+ *   A row that holds an infinity or a NaN gets scale = zero = NaN: it reads back as NaN.
+ * Layout: [block][kv head][group of 16 tokens]; a group is
+ *   K codes, V codes (16 * head_dim * bits/8 bytes each), then bf16 pairs (scale, zero) of 16 K rows and of 16 V rows.
+ *   A row's codes lie in order of the dimension, 4-bit codes two to a byte with the lower dimension in the low bits, and are cut
+ *   into panels of P = min(64, row bytes) bytes.  A K panel is [token][P bytes].  A V panel is
+ *   [token / 8][P/8-byte chunk 0..7][token % 8 / 2][2-byte unit of the chunk][token % 2][2 bytes]: what one lane of a matrix
+ *   instruction needs of V lies together.
+ * Limits: block_tokens a multiple of 16, head_dim 64, 128 or 256, bits 4 or 8. */
+typedef struct ucmx_quant_geometry {
+    int64_t n_blocks;
+    int64_t block_stride; /* bytes from block to block: a multiple of 16, at least ucmx_quant_block_bytes() */
+    int32_t block_tokens;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+    int32_t bits;
+} ucmx_quant_geometry;
+/* Bytes of one block (K and V of all heads); 0 for a geometry outside the limits.  Looks at the last four fields only. Host. */
+size_t ucmx_quant_block_bytes(const ucmx_quant_geometry* geom /* host */);
+/* K/V rows of n tokens (bf16 [n, n_kv_heads, head_dim], k_stride / v_stride elements between tokens, multiples of 8) are
+ * quantised into slots[i] = block * block_tokens + token (int64, device).  A negative slot skips its token; one at or beyond the
+ * cache is dropped and reported (ucmx_device_error code 3).  The slots of a call must differ: a slot that is named twice ends up
+ * with a mixture of both rows. */
+int32_t ucmx_quant_write_tokens(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int64_t n,
+                                const int64_t* slots, void* cache, const ucmx_quant_geometry* geom /* host */,
+                                ucmx_stream_t stream);
+/* Whole blocks of a bf16 paged cache -> quantised blocks: block block_ids[i] of the bf16 cache goes to block out_slots[i] (or i)
+ * of the quantised one.  Negative ids skip, ids beyond either cache are dropped and reported (code 3); out_slots must differ.
+ * Block tokens, heads and head_dim of the three geometries must agree. */
+int32_t ucmx_quant_write_blocks(const void* k_cache, const ucmx_kv_geometry* k_geom /* host */, const void* v_cache,
+                                const ucmx_kv_geometry* v_geom /* host */, const int32_t* block_ids, const int32_t* out_slots,
+                                int32_t n, void* cache, const ucmx_quant_geometry* geom /* host */, ucmx_stream_t stream);
+/* The way back: quantised block block_ids[i] -> block out_slots[i] (or i) of the bf16 caches, each value rounded to bf16 once. */
+int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_geometry* geom /* host */, const int32_t* block_ids,
+                               const int32_t* out_slots, int32_t n, void* k_cache, const ucmx_kv_geometry* k_geom /* host */,
+                               void* v_cache, const ucmx_kv_geometry* v_geom /* host */, ucmx_stream_t stream);
+
+/* ---------------------------------------------------------------- attention over listed blocks
+ * What the selection of stages 1-3 is for.  (The reference hands its selection to the serving engine's attention as a shorter
+ * block table, ucm/sparse/esa/esa.py:313-339; its sequences' positions are lost there, here they may be given.)
+ *
+ * Every request r lists KV blocks; each of its query tokens attends to the tokens of those blocks, for every query head of a KV
+ * head over that head's K and V:  out = sum_t softmax_t(scale * q . k_t) v_t.  fp32 inside, out is bf16 [n_q_tokens, n_q_heads,
+ * head_dim], out_lse (NULL, or fp32 [n_q_tokens, n_q_heads]) the natural logarithm of the softmax's sum, for joining with
+ * attention over other tokens.  A query that sees nothing gets zeros and -infinity.
+ * Lists (all device pointers but the struct itself): entries [offsets[r], offsets[r+1]), offsets[0] = 0, ascending; `total` is
+ *   the capacity of the entry arrays (what lies behind offsets[n_req] is not read, so a captured launch may be replayed with
+ *   fewer entries); counts (or NULL) cuts a request's list short.
+ *   block_ids[e] is the physical block, negative = skip the entry; with block_ids NULL the physical block is
+ *   table[table_offsets[r] + positions[e]] (the request's row of a block table; table_offsets has n_req+1 entries).
+ *   positions[e] is the block's place in its sequence, negative = skip; with positions NULL the i-th entry stands at i.
+ *   ctx_lens[r] (or NULL: every token of every listed block is seen) is the length of the sequence, the query tokens included:
+ *   query token j of the request's n sees the tokens at places below ctx_lens[r] - (n-1-j).  Tokens nobody may see are not
+ *   read, and may hold anything.
+ * An id beyond its cache or table is dropped and reported (ucmx_device_error code 3).
+ * q is bf16 [n_q_tokens, n_q_heads, head_dim], q_stride elements between tokens (a multiple of 8).  q_offsets (n_req+1 entries)
+ *   gives each request's query tokens, at most max_q_tokens; NULL: one each.  Rows of out behind q_offsets[n_req] stay as they are.
+ *   More than one query token per request needs ctx_lens.
+ * n_q_heads a multiple of the cache's heads; head_dim 64, 128 or 256; any block_tokens (bf16 cache).  An infinity in a V row that
+ *   is seen makes that dimension infinite or NaN.
+ * workspace: ucmx_attention_workspace_bytes(...) bytes (bits: 16 for the bf16 cache), 16-byte aligned, any contents; it depends
+ *   on neither the lists nor the batch.  Launches that may overlap need workspaces of their own.  Two kernels per call. */
+typedef struct ucmx_block_lists {
+    const int32_t* offsets;
+    const int32_t* counts;
+    const int32_t* block_ids;
+    const int32_t* positions;
+    const int32_t* table;
+    const int32_t* table_offsets;
+    const int32_t* ctx_lens;
+    int32_t n_req;
+    int32_t total;
+} ucmx_block_lists;
+size_t ucmx_attention_workspace_bytes(int32_t bits, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_q_tokens);
+int32_t ucmx_block_attention(const void* q, int64_t q_stride, int32_t n_q_heads, const int32_t* q_offsets, int32_t n_q_tokens,
+                             int32_t max_q_tokens, const void* k_cache, const ucmx_kv_geometry* k_geom /* host */,
+                             const void* v_cache, const ucmx_kv_geometry* v_geom /* host */,
+                             const ucmx_block_lists* lists /* host */, float scale, void* out, float* out_lse, void* workspace,
+                             size_t workspace_bytes, ucmx_stream_t stream);
+/* The same over the quantised cache: K and V are what the codes stand for, without another rounding. */
+int32_t ucmx_quant_block_attention(const void* q, int64_t q_stride, int32_t n_q_heads, const int32_t* q_offsets,
+                                   int32_t n_q_tokens, int32_t max_q_tokens, const void* cache,
+                                   const ucmx_quant_geometry* geom /* host */, const ucmx_block_lists* lists /* host */,
+                                   float scale, void* out, float* out_lse, void* workspace, size_t workspace_bytes,
+                                   ucmx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

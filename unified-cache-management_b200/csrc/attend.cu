@@ -1,0 +1,140 @@
+// Attention over listed blocks: the C entries, their checks, and the bf16 cache's instances (kernel: attend.cuh).
+#include "attend.cuh"
+
+namespace ucmx {
+namespace attend {
+
+int32_t run_bf16(const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st)
+{
+    return run_format<16>(p, head_dim, cols, launch, plan, st);
+}
+
+namespace {
+
+int32_t refuse(const char* why, int32_t code = UCMX_EPARAM)
+{
+    set_last_text(why);
+    return code;
+}
+
+int32_t run_any(int bits, const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st)
+{
+    return bits == 16 ? run_bf16(p, head_dim, cols, launch, plan, st)
+         : bits == 8  ? run_q8(p, head_dim, cols, launch, plan, st)
+                      : run_q4(p, head_dim, cols, launch, plan, st);
+}
+
+// what both entries check and fill in; the cache's part of `p` is set by the caller
+int32_t attend_common(Params& p, int bits, int32_t head_dim, const void* q, int64_t q_stride, int32_t n_q_heads, int32_t n_kv_heads,
+                      const int32_t* q_offsets, int32_t n_q_tokens, int32_t max_q_tokens, const ucmx_block_lists* l, float scale,
+                      void* out, float* out_lse, void* workspace, size_t workspace_bytes, ucmx_stream_t stream)
+{
+    if (!l || l->n_req < 0 || l->total < 0 || n_q_tokens < 0) return refuse("attention: negative sizes or no lists");
+    if (l->n_req == 0 || n_q_tokens == 0) return UCMX_OK;
+    if (!q || !out || !l->offsets || !workspace) return refuse("attention: a pointer is missing");
+    if (l->total > 0 && !l->block_ids && !(l->positions && l->table && l->table_offsets))
+        return refuse("attention: block_ids, or positions with table and table_offsets");
+    if (n_kv_heads < 1 || n_q_heads < n_kv_heads || n_q_heads % n_kv_heads) return refuse("attention: n_q_heads must be a multiple of n_kv_heads");
+    if (max_q_tokens < 1 || (!q_offsets && max_q_tokens != 1)) return refuse("attention: more than one query token per request needs q_offsets");
+    if (max_q_tokens > 1 && !l->ctx_lens) return refuse("attention: several query tokens per request need ctx_lens");
+    if (q_stride % 8 || q_stride < (int64_t)n_q_heads * head_dim || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 15))
+        return refuse("attention: query rows, out and workspace must start on 16 bytes");
+    if (p.k_block % 16 || ((uintptr_t)p.k & 15) || ((uintptr_t)p.v & 15)) return refuse("attention: the cache must start on 16 bytes");
+    if ((int64_t)max_q_tokens * (n_q_heads / n_kv_heads) > (1 << 20)) return refuse("attention: too many query rows per request", UCMX_EUNSUPPORTED);
+    p.q = (const uint16_t*)q;
+    p.q_stride = q_stride;
+    p.q_offsets = q_offsets;
+    p.n_q_tokens = n_q_tokens;
+    p.max_q = max_q_tokens;
+    p.Hq = n_q_heads;
+    p.H = n_kv_heads;
+    p.G = n_q_heads / n_kv_heads;
+    p.spe = (p.T + kRows - 1) / kRows;
+    p.offsets = l->offsets;
+    p.counts = l->counts;
+    p.block_ids = l->block_ids;
+    p.positions = l->positions;
+    p.table = l->table;
+    p.table_offsets = l->table_offsets;
+    p.ctx = l->ctx_lens;
+    p.n_req = l->n_req;
+    p.total = l->total;
+    p.scale_log2 = scale * kLog2e;
+    p.out = (uint16_t*)out;
+    p.lse = out_lse;
+    p.ws = (float*)workspace;
+    p.err = error_word();
+    const int cols = max_q_tokens * p.G;
+    Plan plan;
+    const int32_t rc = run_any(bits, p, head_dim, cols, false, &plan, nullptr);
+    if (rc != UCMX_OK) return refuse("attention: head_dim must be 64, 128 or 256", rc);
+    if (workspace_bytes < (size_t)plan.ctas * 2 * plan.part * sizeof(float)) return refuse("attention: workspace too small");
+    p.cols_per_tile = plan.cols;
+    p.col_tiles = (cols + plan.cols - 1) / plan.cols;
+    // a request's slices of all heads and tiles are counted in 32 bits inside the kernel
+    if ((int64_t)p.total * p.spe > INT32_MAX) return refuse("attention: more than 2^31 slices in the lists", UCMX_EUNSUPPORTED);
+    return run_any(bits, p, head_dim, cols, true, &plan, (cudaStream_t)stream);
+}
+
+}  // namespace
+}  // namespace attend
+}  // namespace ucmx
+
+using namespace ucmx;
+using namespace ucmx::attend;
+
+extern "C" size_t ucmx_attention_workspace_bytes(int32_t bits, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_q_tokens)
+{
+    if ((bits != 16 && bits != 8 && bits != 4) || n_kv_heads < 1 || n_q_heads < n_kv_heads || max_q_tokens < 1) return 0;
+    Plan plan;
+    Params p = {};
+    const int64_t cols = (int64_t)max_q_tokens * (n_q_heads / n_kv_heads);
+    if (run_any(bits, p, head_dim, cols > 64 ? 64 : (int)cols, false, &plan, nullptr) != UCMX_OK) return 0;
+    return (size_t)plan.ctas * 2 * plan.part * sizeof(float);
+}
+
+extern "C" int32_t ucmx_block_attention(const void* q, int64_t q_stride, int32_t n_q_heads, const int32_t* q_offsets, int32_t n_q_tokens,
+                                        int32_t max_q_tokens, const void* k_cache, const ucmx_kv_geometry* kg, const void* v_cache,
+                                        const ucmx_kv_geometry* vg, const ucmx_block_lists* lists, float scale, void* out, float* out_lse,
+                                        void* workspace, size_t workspace_bytes, ucmx_stream_t stream)
+{
+    if (!kg || !vg || !lists) return refuse("block_attention: geometry or lists missing");
+    if (kg->block_tokens < 1 || kg->n_kv_heads < 1 || kg->reserved < 1) return refuse("block_attention: the geometry must carry tokens, heads and blocks");
+    if (vg->block_tokens != kg->block_tokens || vg->n_kv_heads != kg->n_kv_heads || vg->head_dim != kg->head_dim)
+        return refuse("block_attention: K and V blocks differ in shape");
+    const int64_t E = (int64_t)kg->n_kv_heads * kg->head_dim;
+    if (kg->token_stride < E || vg->token_stride < E || kg->token_stride % 8 || vg->token_stride % 8 || kg->block_stride % 8 || vg->block_stride % 8 ||
+        kg->block_stride < 0 || vg->block_stride < 0)
+        return refuse("block_attention: strides must be multiples of 8 elements and hold a token's heads");
+    if (lists->n_req > 0 && lists->total > 0 && n_q_tokens > 0 && (!k_cache || !v_cache)) return refuse("block_attention: no cache");
+    Params p = {};
+    p.k = (const uint8_t*)k_cache;
+    p.v = (const uint8_t*)v_cache;
+    p.k_block = kg->block_stride * 2;
+    p.v_block = vg->block_stride * 2;
+    p.k_token = kg->token_stride * 2;
+    p.v_token = vg->token_stride * 2;
+    p.T = kg->block_tokens;
+    p.n_blocks = kg->reserved < vg->reserved ? kg->reserved : vg->reserved;
+    return attend_common(p, 16, kg->head_dim, q, q_stride, n_q_heads, kg->n_kv_heads, q_offsets, n_q_tokens, max_q_tokens, lists, scale, out,
+                         out_lse, workspace, workspace_bytes, stream);
+}
+
+extern "C" int32_t ucmx_quant_block_attention(const void* q, int64_t q_stride, int32_t n_q_heads, const int32_t* q_offsets, int32_t n_q_tokens,
+                                              int32_t max_q_tokens, const void* cache, const ucmx_quant_geometry* g,
+                                              const ucmx_block_lists* lists, float scale, void* out, float* out_lse, void* workspace,
+                                              size_t workspace_bytes, ucmx_stream_t stream)
+{
+    if (!lists) return refuse("quant_block_attention: no lists");
+    if (ucmx_quant_block_bytes(g) == 0) return refuse("quant_block_attention: a cache geometry that the library does not hold", UCMX_EUNSUPPORTED);
+    if (g->n_blocks < 1 || g->block_stride < (int64_t)ucmx_quant_block_bytes(g) || g->block_stride % 16)
+        return refuse("quant_block_attention: block_stride must be a multiple of 16 and hold a block");
+    if (lists->n_req > 0 && lists->total > 0 && n_q_tokens > 0 && !cache) return refuse("quant_block_attention: no cache");
+    Params p = {};
+    p.k = (const uint8_t*)cache;
+    p.k_block = g->block_stride;
+    p.T = g->block_tokens;
+    p.n_blocks = g->n_blocks;
+    return attend_common(p, g->bits, g->head_dim, q, q_stride, n_q_heads, g->n_kv_heads, q_offsets, n_q_tokens, max_q_tokens, lists, scale, out,
+                         out_lse, workspace, workspace_bytes, stream);
+}

@@ -1,0 +1,435 @@
+// The quantised paged KV cache: rows of new tokens or whole bf16 blocks in, whole blocks back out.
+//
+// Per row x (one token, one KV head, K or V): zero = min x, scale = bf16((max x - min x) / L), code = nearest((x - zero) /
+// scale), L = 15 or 255; the layout is described at ucmx_quant_geometry.  All three kernels are streams: a row of 128 values is
+// 256 bytes on the bf16 side and 68 (132) on the other, with one reduction over the lanes that hold it in between.
+//
+// Eight or sixteen values per lane, so that a row is 8 or 16 lanes and a warp holds two or four neighbouring tokens of one head.
+// V's layout puts the codes of tokens 2i and 2i+1 side by side in pairs of bytes: neighbouring rows of the warp exchange words, so
+// that V moves in 32-bit words like K (a token whose partner is not in the call stores 16-bit pieces).
+//
+// Arithmetic.  The differences are taken of halves (exact, and no overflow for any finite row).  A reciprocal and one residual
+// give the quotient's nearest integer: the residual x - code*scale is exact in fp32, so a step in the wrong direction shows and
+// is taken back; a tie, where the rounding of x - zero might have decided, is settled in fp64.  (A division per value was the
+// bound of this kernel.)
+#include "common.cuh"
+
+namespace ucmx {
+namespace {
+
+constexpr int kRows = 16;
+
+template <int BITS, int D>
+struct Q {
+    static constexpr int kRowBytes = D * BITS / 8;
+    static constexpr int kPanel = kRowBytes < 64 ? kRowBytes : 64;
+    static constexpr int kDims = D == 256 ? 16 : 8;      // values a lane holds
+    static constexpr int kLanes = D / kDims;             // lanes of a row
+    static constexpr int kTokens = 32 / kLanes;          // rows of a warp: neighbouring tokens of one head
+    static constexpr int kWords = kDims * BITS / 32;     // code words of a lane
+    static constexpr int kGroup = 2 * kRows * kRowBytes + 2 * kRows * 4;
+    static constexpr int kTop = (1 << BITS) - 1;
+};
+
+struct QuantParams {
+    const uint16_t* k;                 // bf16 side: rows of tokens, or a paged cache
+    const uint16_t* v;
+    int64_t k_block, v_block;          // elements
+    int64_t k_token, v_token;
+    uint8_t* cache;
+    int64_t block_stride;              // bytes
+    int64_t n_blocks;                  // of the quantised cache
+    int64_t n_src;                     // blocks of the bf16 cache
+    const int64_t* slots;              // token form
+    const int32_t* ids;                // block forms
+    const int32_t* out_slots;
+    int32_t T, H;
+    int64_t n;                         // tokens or blocks
+    int64_t units;                     // warp-sized pieces of work
+    int32_t* err;
+};
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// nearest integer to (x - zero) / scale, ties to even; inv = 1 / (scale / 2)
+__device__ __forceinline__ int code_of(float x, float half_zero, float half_scale, float inv, float zero, float scale)
+{
+    const float hx = fmaf(x, 0.5f, -half_zero);
+    float c = rintf(hx * inv);
+    const float e = fmaf(-c, half_scale, hx);
+    const float off = fabsf(e), half = 0.5f * half_scale;
+    if (off > half) c += e > 0.f ? 1.f : -1.f;
+    if (off == half) c = (float)rint(((double)x - (double)zero) / (double)scale);
+    return (int)c;
+}
+
+// byte offset of a lane's codes inside K's part of a group / of unit u (2 bytes of a row) inside V's part
+template <int BITS, int D>
+__device__ __forceinline__ int k_at(int t, int lr)
+{
+    using X = Q<BITS, D>;
+    const int b = lr * X::kWords * 4;
+    return (b / X::kPanel) * (kRows * X::kPanel) + t * X::kPanel + b % X::kPanel;
+}
+template <int BITS, int D>
+__device__ __forceinline__ int v_at(int t, int u)
+{
+    using X = Q<BITS, D>;
+    const int b = (u * 2) % X::kPanel;
+    constexpr int kChunk = X::kPanel / 8;
+    return (u * 2 / X::kPanel) * (kRows * X::kPanel) + (t >> 3) * (8 * X::kPanel) + (b / kChunk) * X::kPanel + ((t & 7) >> 1) * (2 * kChunk) +
+           (b % kChunk) / 2 * 4 + (t & 1) * 2;
+}
+
+// Unit -> (token group, K or V, head); heads are innermost, neighbouring warps read neighbouring rows of the same tokens.
+struct Unit {
+    int64_t tg;
+    int32_t kv, h;
+};
+__device__ __forceinline__ Unit unit_of(int64_t u, int H)
+{
+    Unit x;
+    const int64_t a = u / H;
+    x.h = (int32_t)(u - a * H);
+    x.kv = (int32_t)(a & 1);
+    x.tg = a >> 1;
+    return x;
+}
+
+template <int BITS, int D, bool BLOCKS>
+__global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
+{
+    using X = Q<BITS, D>;
+    const int lane = threadIdx.x & 31, lr = lane % X::kLanes, row = lane / X::kLanes;
+    const int64_t step = (int64_t)gridDim.x * 8;
+    const int per_block = (p.T + X::kTokens - 1) / X::kTokens;
+    for (int64_t un = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); un < p.units; un += step) {
+        const Unit x = unit_of(un, p.H);
+        // ---- where the row comes from and where it goes
+        const uint16_t* src = x.kv ? p.v : p.k;
+        int64_t block = -1;
+        int t = 0;
+        if (BLOCKS) {
+            const int64_t i = x.tg / per_block;
+            t = (int)(x.tg - i * per_block) * X::kTokens + row;
+            const int id = checked_block_id(p.ids, i, p.n_src, lr == 0 && row == 0 ? p.err : nullptr);
+            const int64_t out = checked_out_row(p.out_slots, i, p.n_blocks, lr == 0 && row == 0 ? p.err : nullptr);
+            if (id >= 0 && out >= 0) block = out;
+            src += (int64_t)(id < 0 ? 0 : id) * (x.kv ? p.v_block : p.k_block) + (int64_t)t * (x.kv ? p.v_token : p.k_token);
+        } else {
+            const int64_t i = x.tg * X::kTokens + row;
+            int64_t slot = i < p.n ? __ldg(p.slots + i) : -1;
+            if (slot >= p.n_blocks * p.T) {
+                if (p.err && lr == 0) atomicExch(p.err, 3);
+                slot = -1;
+            }
+            if (slot >= 0) {
+                block = slot / p.T;
+                t = (int)(slot - block * p.T);
+            }
+            src += i * (x.kv ? p.v_token : p.k_token);
+        }
+        src += (int64_t)x.h * D + lr * X::kDims;
+        const bool live = block >= 0;
+        uint4 raw[X::kDims / 8];
+#pragma unroll
+        for (int i = 0; i < X::kDims / 8; ++i) raw[i] = live ? ld_stream16(src + i * 8) : make_uint4(0, 0, 0, 0);
+        float f[X::kDims];
+#pragma unroll
+        for (int i = 0; i < X::kDims / 8; ++i) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f[i * 8 + 2 * j] = bf16lo(w[j]);
+                f[i * 8 + 2 * j + 1] = bf16hi(w[j]);
+            }
+        }
+        // ---- the row's range; x - x is 0 for a number and NaN for anything else
+        float lo = f[0], hi = f[0], odd = 0.f;
+#pragma unroll
+        for (int i = 0; i < X::kDims; ++i) {
+            lo = fminf(lo, f[i]);
+            hi = fmaxf(hi, f[i]);
+            odd += f[i] - f[i];
+        }
+#pragma unroll
+        for (int o = 1; o < X::kLanes; o <<= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            odd += __shfl_xor_sync(0xffffffffu, odd, o);
+        }
+        const bool bad = !(odd == 0.f);
+        const float half_lo = 0.5f * lo;
+        const uint32_t sb = bad ? 0x7fc0u : f32_to_bf16_bits(fmaf(0.5f, hi, -half_lo) / (0.5f * (float)X::kTop));
+        const uint32_t zb = bad ? 0x7fc0u : __float_as_uint(lo) >> 16;
+        const float scale = __uint_as_float(sb << 16), half_scale = 0.5f * scale;
+        // ---- codes
+        uint32_t w[X::kWords];
+#pragma unroll
+        for (int i = 0; i < X::kWords; ++i) w[i] = 0u;
+        if (!bad && scale > 0.f) {
+            const bool tiny = scale < 1e-30f;            // the reciprocal would leave the range: everything in fp64
+            const float inv = tiny ? 0.f : 1.f / half_scale;
+#pragma unroll
+            for (int i = 0; i < X::kDims; ++i) {
+                int c;
+                if (tiny)
+                    c = (int)fmin(rint(((double)f[i] - (double)lo) / (double)scale), (double)X::kTop);
+                else
+                    c = code_of(f[i], half_lo, half_scale, inv, lo, scale);
+                c = min(max(c, 0), X::kTop);
+                w[i * BITS / 32] |= (uint32_t)c << (i * BITS % 32);
+            }
+        }
+        uint8_t* const group = p.cache + block * p.block_stride + ((int64_t)x.h * (p.T / kRows) + t / kRows) * X::kGroup;
+        const int tt = t % kRows;
+        if (x.kv == 0) {
+            if (live) {
+                uint8_t* const d = group + k_at<BITS, D>(tt, lr);
+                if (X::kWords == 1) *reinterpret_cast<uint32_t*>(d) = w[0];
+                if (X::kWords == 2) *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[X::kWords - 1]);
+                if (X::kWords == 4) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1 % X::kWords], w[2 % X::kWords], w[3 % X::kWords]);
+            }
+        } else {
+            uint8_t* const part = group + kRows * X::kRowBytes;
+            // is the neighbouring row the other token of the pair?
+            const int64_t place = live ? block * p.T + t : -2 - row;
+            const int64_t other = __shfl_xor_sync(0xffffffffu, place, X::kLanes);
+            const bool paired = live && other == (place ^ 1) && (place & 1) == (row & 1);
+#pragma unroll
+            for (int i = 0; i < X::kWords; ++i) {
+                const uint32_t y = __shfl_xor_sync(0xffffffffu, w[i], X::kLanes);
+                const int u = (lr * X::kWords + i) * 2;
+                if (paired) {
+                    const uint32_t z = (row & 1) ? __byte_perm(y, w[i], 0x7632) : __byte_perm(w[i], y, 0x5410);
+                    *reinterpret_cast<uint32_t*>(part + v_at<BITS, D>(tt & ~1, u + (row & 1))) = z;
+                } else if (live) {
+                    *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u)) = (uint16_t)w[i];
+                    *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u + 1)) = (uint16_t)(w[i] >> 16);
+                }
+            }
+        }
+        if (live && lr == 0)
+            *reinterpret_cast<uint32_t*>(group + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4) = sb | (zb << 16);
+    }
+}
+
+template <int BITS, int D>
+__global__ void __launch_bounds__(256) quant_read_kernel(const QuantParams p)
+{
+    using X = Q<BITS, D>;
+    const int lane = threadIdx.x & 31, lr = lane % X::kLanes, row = lane / X::kLanes;
+    const int64_t step = (int64_t)gridDim.x * 8;
+    const int per_block = p.T / X::kTokens;
+    for (int64_t un = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); un < p.units; un += step) {
+        const Unit x = unit_of(un, p.H);
+        const int64_t i = x.tg / per_block;
+        const int t = (int)(x.tg - i * per_block) * X::kTokens + row;
+        const int id = checked_block_id(p.ids, i, p.n_blocks, lane == 0 ? p.err : nullptr);
+        const int64_t out = checked_out_row(p.out_slots, i, p.n_src, lane == 0 ? p.err : nullptr);
+        if (id < 0 || out < 0) continue;                 // (the same for the whole warp)
+        const uint8_t* const group = p.cache + (int64_t)id * p.block_stride + ((int64_t)x.h * (p.T / kRows) + t / kRows) * X::kGroup;
+        const int tt = t % kRows;
+        uint32_t w[X::kWords];
+        if (x.kv == 0) {
+            const uint8_t* const s = group + k_at<BITS, D>(tt, lr);
+            if (X::kWords == 1) w[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+            if (X::kWords == 2) {
+                const uint2 y = __ldg(reinterpret_cast<const uint2*>(s));
+                w[0] = y.x;
+                w[X::kWords - 1] = y.y;
+            }
+            if (X::kWords == 4) {
+                const uint4 y = __ldg(reinterpret_cast<const uint4*>(s));
+                w[0] = y.x;
+                w[1 % X::kWords] = y.y;
+                w[2 % X::kWords] = y.z;
+                w[3 % X::kWords] = y.w;
+            }
+        } else {
+            const uint8_t* const part = group + kRows * X::kRowBytes;
+#pragma unroll
+            for (int j = 0; j < X::kWords; ++j) {
+                const int u = (lr * X::kWords + j) * 2;
+                const uint32_t mine = __ldg(reinterpret_cast<const uint32_t*>(part + v_at<BITS, D>(tt & ~1, u + (row & 1))));
+                const uint32_t y = __shfl_xor_sync(0xffffffffu, mine, X::kLanes);
+                w[j] = (row & 1) ? __byte_perm(y, mine, 0x7632) : __byte_perm(mine, y, 0x5410);
+            }
+        }
+        const uint32_t sz = __ldg(reinterpret_cast<const uint32_t*>(group + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4));
+        const float scale = bf16lo(sz), zero = bf16hi(sz);
+        uint16_t* const dst = const_cast<uint16_t*>(x.kv ? p.v : p.k) + out * (x.kv ? p.v_block : p.k_block) +
+                              (int64_t)t * (x.kv ? p.v_token : p.k_token) + (int64_t)x.h * D + lr * X::kDims;
+#pragma unroll
+        for (int j = 0; j < X::kDims / 8; ++j) {
+            uint32_t o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int a = j * 8 + 2 * k;
+                const uint32_t c0 = (w[a * BITS / 32] >> (a * BITS % 32)) & X::kTop;
+                const uint32_t c1 = (w[(a + 1) * BITS / 32] >> ((a + 1) * BITS % 32)) & X::kTop;
+                o[k] = pack2(fmaf((float)c0, scale, zero), fmaf((float)c1, scale, zero));
+            }
+            st_stream16(dst + j * 8, make_uint4(o[0], o[1], o[2], o[3]));
+        }
+    }
+}
+
+enum Form { kTokensForm, kBlocksForm, kReadForm };
+
+template <int BITS, int D>
+int32_t launch(QuantParams& p, Form form, cudaStream_t st)
+{
+    using X = Q<BITS, D>;
+    const int64_t groups = form == kTokensForm ? (p.n + X::kTokens - 1) / X::kTokens : p.n * (p.T / X::kTokens);
+    p.units = groups * 2 * p.H;
+    int64_t grid = (p.units + 7) / 8;
+    const int64_t most = (int64_t)sm_count() * 8;
+    if (grid > most) grid = most;
+    if (form == kTokensForm)
+        quant_write_kernel<BITS, D, false><<<(unsigned)grid, 256, 0, st>>>(p);
+    else if (form == kBlocksForm)
+        quant_write_kernel<BITS, D, true><<<(unsigned)grid, 256, 0, st>>>(p);
+    else
+        quant_read_kernel<BITS, D><<<(unsigned)grid, 256, 0, st>>>(p);
+    UCMX_LAUNCH_CHECK("quant_cache_kernel");
+    return UCMX_OK;
+}
+
+int32_t dispatch(QuantParams& p, const ucmx_quant_geometry* g, Form form, cudaStream_t st)
+{
+    p.err = error_word();
+    const int which = (g->bits == 4 ? 0 : 1) * 1000 + g->head_dim;
+    switch (which) {
+        case 64: return launch<4, 64>(p, form, st);
+        case 128: return launch<4, 128>(p, form, st);
+        case 256: return launch<4, 256>(p, form, st);
+        case 1064: return launch<8, 64>(p, form, st);
+        case 1128: return launch<8, 128>(p, form, st);
+        default: return launch<8, 256>(p, form, st);
+    }
+}
+
+int32_t refuse(const char* why, int32_t code = UCMX_EPARAM)
+{
+    set_last_text(why);
+    return code;
+}
+
+int32_t check_cache(const void* cache, const ucmx_quant_geometry* g)
+{
+    const size_t bytes = ucmx_quant_block_bytes(g);
+    if (bytes == 0) return refuse("quantised cache: a geometry that the library does not hold", UCMX_EUNSUPPORTED);
+    if (!cache || ((uintptr_t)cache & 15)) return refuse("quantised cache: must start on 16 bytes");
+    if (g->n_blocks < 1 || g->block_stride < (int64_t)bytes || g->block_stride % 16)
+        return refuse("quantised cache: block_stride must be a multiple of 16 and hold a block");
+    return UCMX_OK;
+}
+
+// the bf16 side of the block forms
+int32_t check_pair(QuantParams& p, const void* k, const ucmx_kv_geometry* kg, const void* v, const ucmx_kv_geometry* vg,
+                   const ucmx_quant_geometry* g)
+{
+    if (!k || !v || ((uintptr_t)k & 15) || ((uintptr_t)v & 15)) return refuse("quantised cache: bf16 caches must start on 16 bytes");
+    if (!kg || !vg || kg->reserved < 1 || vg->reserved < 1) return refuse("quantised cache: the geometries must carry the number of blocks");
+    const ucmx_kv_geometry* both[2] = {kg, vg};
+    for (const ucmx_kv_geometry* x : both) {
+        if (x->block_tokens != g->block_tokens || x->n_kv_heads != g->n_kv_heads || x->head_dim != g->head_dim)
+            return refuse("quantised cache: the bf16 blocks have another shape");
+        if (x->token_stride < (int64_t)x->n_kv_heads * x->head_dim || x->token_stride % 8 || x->block_stride % 8 || x->block_stride < 0)
+            return refuse("quantised cache: strides must be multiples of 8 elements and hold a token's heads");
+    }
+    p.k = (const uint16_t*)k;
+    p.v = (const uint16_t*)v;
+    p.k_block = kg->block_stride;
+    p.v_block = vg->block_stride;
+    p.k_token = kg->token_stride;
+    p.v_token = vg->token_stride;
+    p.n_src = kg->reserved < vg->reserved ? kg->reserved : vg->reserved;
+    return UCMX_OK;
+}
+
+void set_cache(QuantParams& p, const void* cache, const ucmx_quant_geometry* g)
+{
+    p.cache = (uint8_t*)const_cast<void*>(cache);
+    p.block_stride = g->block_stride;
+    p.n_blocks = g->n_blocks;
+    p.T = g->block_tokens;
+    p.H = g->n_kv_heads;
+}
+
+}  // namespace
+}  // namespace ucmx
+
+using namespace ucmx;
+
+extern "C" size_t ucmx_quant_block_bytes(const ucmx_quant_geometry* g)
+{
+    if (!g || (g->bits != 4 && g->bits != 8) || (g->head_dim != 64 && g->head_dim != 128 && g->head_dim != 256)) return 0;
+    if (g->block_tokens < 16 || g->block_tokens % 16 || g->n_kv_heads < 1 || g->block_tokens > (1 << 20) || g->n_kv_heads > (1 << 16)) return 0;
+    const size_t group = (size_t)(2 * 16) * (g->head_dim * g->bits / 8) + 2 * 16 * 4;
+    return group * (size_t)(g->block_tokens / 16) * (size_t)g->n_kv_heads;
+}
+
+extern "C" int32_t ucmx_quant_write_tokens(const void* k, const void* v, int64_t k_stride, int64_t v_stride, int64_t n, const int64_t* slots,
+                                           void* cache, const ucmx_quant_geometry* g, ucmx_stream_t stream)
+{
+    if (n < 0) return refuse("quant_write_tokens: a negative count");
+    if (n == 0) return UCMX_OK;
+    const int32_t rc = check_cache(cache, g);
+    if (rc != UCMX_OK) return rc;
+    if (!k || !v || !slots || ((uintptr_t)k & 15) || ((uintptr_t)v & 15)) return refuse("quant_write_tokens: rows must start on 16 bytes");
+    const int64_t E = (int64_t)g->n_kv_heads * g->head_dim;
+    if (k_stride < E || v_stride < E || k_stride % 8 || v_stride % 8)
+        return refuse("quant_write_tokens: strides must be multiples of 8 elements and hold a token's heads");
+    QuantParams p = {};
+    p.k = (const uint16_t*)k;
+    p.v = (const uint16_t*)v;
+    p.k_token = k_stride;
+    p.v_token = v_stride;
+    p.slots = slots;
+    p.n = n;
+    set_cache(p, cache, g);
+    return dispatch(p, g, kTokensForm, (cudaStream_t)stream);
+}
+
+extern "C" int32_t ucmx_quant_write_blocks(const void* k_cache, const ucmx_kv_geometry* kg, const void* v_cache, const ucmx_kv_geometry* vg,
+                                           const int32_t* block_ids, const int32_t* out_slots, int32_t n, void* cache,
+                                           const ucmx_quant_geometry* g, ucmx_stream_t stream)
+{
+    if (n < 0) return refuse("quant_write_blocks: a negative count");
+    if (n == 0) return UCMX_OK;
+    int32_t rc = check_cache(cache, g);
+    QuantParams p = {};
+    if (rc == UCMX_OK) rc = check_pair(p, k_cache, kg, v_cache, vg, g);
+    if (rc != UCMX_OK) return rc;
+    if (!block_ids) return refuse("quant_write_blocks: no block ids");
+    p.ids = block_ids;
+    p.out_slots = out_slots;
+    p.n = n;
+    set_cache(p, cache, g);
+    return dispatch(p, g, kBlocksForm, (cudaStream_t)stream);
+}
+
+extern "C" int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_geometry* g, const int32_t* block_ids, const int32_t* out_slots,
+                                          int32_t n, void* k_cache, const ucmx_kv_geometry* kg, void* v_cache, const ucmx_kv_geometry* vg,
+                                          ucmx_stream_t stream)
+{
+    if (n < 0) return refuse("quant_read_blocks: a negative count");
+    if (n == 0) return UCMX_OK;
+    int32_t rc = check_cache(cache, g);
+    QuantParams p = {};
+    if (rc == UCMX_OK) rc = check_pair(p, k_cache, kg, v_cache, vg, g);
+    if (rc != UCMX_OK) return rc;
+    if (!block_ids) return refuse("quant_read_blocks: no block ids");
+    p.ids = block_ids;
+    p.out_slots = out_slots;
+    p.n = n;
+    set_cache(p, cache, g);
+    return dispatch(p, g, kReadForm, (cudaStream_t)stream);
+}

@@ -49,6 +49,19 @@ class KvGeometry(C.Structure):
     ]
 
 
+class QuantGeometry(C.Structure):
+    """ucmx_quant_geometry: a paged cache of 4- or 8-bit codes."""
+    _fields_ = [("n_blocks", C.c_int64), ("block_stride", C.c_int64), ("block_tokens", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("bits", C.c_int32)]
+
+
+class BlockLists(C.Structure):
+    """ucmx_block_lists: which blocks each request's queries attend to."""
+    _fields_ = [("offsets", C.c_void_p), ("counts", C.c_void_p), ("block_ids", C.c_void_p), ("positions", C.c_void_p),
+                ("table", C.c_void_p), ("table_offsets", C.c_void_p), ("ctx_lens", C.c_void_p), ("n_req", C.c_int32),
+                ("total", C.c_int32)]
+
+
 _vp, _i32, _i64, _f32, _sz = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t
 _pvp = C.POINTER(C.c_void_p)
 _pi32 = C.POINTER(C.c_int32)
@@ -117,9 +130,21 @@ SIGNATURES = {
     "ucmx_kvstar_workspace_bytes": [_i32, _i32, _i32, _i32, _i32],
     "ucmx_kvstar_scores": [_vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _sz,
                            _vp, _vp],
+    "ucmx_quant_block_bytes": [C.POINTER(QuantGeometry)],
+    "ucmx_quant_write_tokens": [_vp, _vp, _i64, _i64, _i64, _vp, _vp, C.POINTER(QuantGeometry), _vp],
+    "ucmx_quant_write_blocks": [_vp, C.POINTER(KvGeometry), _vp, C.POINTER(KvGeometry), _vp, _vp, _i32, _vp,
+                                C.POINTER(QuantGeometry), _vp],
+    "ucmx_quant_read_blocks": [_vp, C.POINTER(QuantGeometry), _vp, _vp, _i32, _vp, C.POINTER(KvGeometry), _vp,
+                               C.POINTER(KvGeometry), _vp],
+    "ucmx_attention_workspace_bytes": [_i32, _i32, _i32, _i32, _i32],
+    "ucmx_block_attention": [_vp, _i64, _i32, _vp, _i32, _i32, _vp, C.POINTER(KvGeometry), _vp, C.POINTER(KvGeometry),
+                             C.POINTER(BlockLists), _f32, _vp, _vp, _vp, _sz, _vp],
+    "ucmx_quant_block_attention": [_vp, _i64, _i32, _vp, _i32, _i32, _vp, C.POINTER(QuantGeometry), C.POINTER(BlockLists), _f32,
+                                   _vp, _vp, _vp, _sz, _vp],
 }
 _RESTYPES = {"ucmx_last_error": C.c_char_p, "ucmx_kvstar_workspace_bytes": C.c_size_t,
-             "ucmx_peer_exchange_bytes": C.c_size_t}
+             "ucmx_peer_exchange_bytes": C.c_size_t, "ucmx_quant_block_bytes": C.c_size_t,
+             "ucmx_attention_workspace_bytes": C.c_size_t}
 
 
 class RemapMoves(C.Structure):

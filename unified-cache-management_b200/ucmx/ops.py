@@ -506,3 +506,193 @@ def kvstar_scores(reps: torch.Tensor, req_offsets: torch.Tensor, q: torch.Tensor
                                   workspace.numel() * workspace.element_size(), _ptr(out), _stream(reps))
     N.check("ucmx_kvstar_scores", st, 3 if total and n_req else 0)
     return out
+
+
+# ------------------------------------------------------------------------------------ quantised cache, attention over blocks
+
+class QuantKvCache:
+    """A paged cache of 4- or 8-bit codes (layout: ucmx_quant_geometry in include/ucmx.h): `data` is uint8
+    [n_blocks, n_kv_heads, block_tokens/16, group bytes], each block contiguous, K and V together - so [data] is one plane for
+    gather_blocks, move_blocks and the stores."""
+
+    def __init__(self, data: torch.Tensor, *, head_dim: int, bits: int):
+        if data.dtype != torch.uint8 or data.dim() != 4:
+            raise ValueError("data must be uint8 [n_blocks, n_kv_heads, block_tokens/16, group bytes]")
+        nb, H, groups, gb = data.shape
+        if data.stride()[1:] != (groups * gb, gb, 1):
+            raise ValueError("each block of the quantised cache must be contiguous")
+        self.geometry = N.QuantGeometry(nb, data.stride(0) if nb > 1 else H * groups * gb, groups * 16, H, head_dim, bits)
+        if N.lib.ucmx_quant_block_bytes(C.byref(self.geometry)) != H * groups * gb:
+            raise ValueError("bits must be 4 or 8, head_dim 64, 128 or 256, and the last dimension the bytes of a 16-token group")
+        self.data = data
+
+    @classmethod
+    def alloc(cls, n_blocks: int, block_tokens: int, n_kv_heads: int, head_dim: int, bits: int, device) -> "QuantKvCache":
+        """A zeroed cache."""
+        bytes_ = N.lib.ucmx_quant_block_bytes(C.byref(N.QuantGeometry(n_blocks, 0, block_tokens, n_kv_heads, head_dim, bits)))
+        if bytes_ == 0:
+            raise ValueError("bits must be 4 or 8, head_dim 64, 128 or 256, block_tokens a multiple of 16")
+        groups = block_tokens // 16
+        shape = (n_blocks, n_kv_heads, groups, bytes_ // (n_kv_heads * groups))
+        return cls(torch.zeros(shape, dtype=torch.uint8, device=device), head_dim=head_dim, bits=bits)
+
+    @property
+    def block_bytes(self) -> int:
+        return int(N.lib.ucmx_quant_block_bytes(C.byref(self.geometry)))
+
+
+def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]):
+    """All tensors on the device of `first`, made current for the launch where it is not."""
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError("all tensors of a call must be on the same device")
+    return torch.cuda.device(first.device)
+
+
+def quant_write_tokens(cache: QuantKvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Quantise the K and V rows of new tokens into the cache: k, v bf16 [n, n_kv_heads, head_dim] (rows of a wider tensor are
+    fine), slots int64 [n] = block * block_tokens + token, all different; a negative slot skips its token."""
+    _need_cuda(cache.data, k, v, slots)
+    g = cache.geometry
+    n = slots.numel()
+    for x in (k, v):
+        if x.dtype != torch.bfloat16 or tuple(x.shape) != (n, g.n_kv_heads, g.head_dim) or x.stride()[1:] != (g.head_dim, 1):
+            raise ValueError("k and v must be bf16 [n, n_kv_heads, head_dim] with contiguous heads")
+    if slots.dtype != torch.int64 or not slots.is_contiguous():
+        raise ValueError("slots must be contiguous int64")
+    with _same_device(cache.data, k, v, slots):
+        strides = [x.stride(0) if n > 1 else g.n_kv_heads * g.head_dim for x in (k, v)]
+        st = N.lib.ucmx_quant_write_tokens(_ptr(k), _ptr(v), strides[0], strides[1], n, _ptr(slots), _ptr(cache.data), C.byref(g),
+                                           _stream(cache.data))
+    N.check("ucmx_quant_write_tokens", st, 1 if n else 0)
+
+
+def quant_write_blocks(cache: QuantKvCache, k_cache: torch.Tensor, v_cache: torch.Tensor, block_ids: torch.Tensor, *,
+                       out_slots: Optional[torch.Tensor] = None) -> None:
+    """Quantise blocks block_ids[i] of a bf16 paged cache into block out_slots[i] (or i) of the quantised one."""
+    _need_cuda(cache.data, k_cache, v_cache, block_ids, out_slots)
+    ids = _i32(block_ids, "block_ids")
+    n = ids.numel()
+    if out_slots is not None and out_slots.numel() != n:
+        raise ValueError("one out_slots entry per block id")
+    with _same_device(cache.data, k_cache, v_cache, block_ids, out_slots):
+        st = N.lib.ucmx_quant_write_blocks(_ptr(k_cache), C.byref(kv_geometry(k_cache)), _ptr(v_cache), C.byref(kv_geometry(v_cache)),
+                                           _ptr(ids), _ptr(_i32(out_slots, "out_slots")), n, _ptr(cache.data), C.byref(cache.geometry),
+                                           _stream(cache.data))
+    N.check("ucmx_quant_write_blocks", st, 1 if n else 0)
+
+
+def quant_read_blocks(cache: QuantKvCache, block_ids: torch.Tensor, *, k_out: Optional[torch.Tensor] = None,
+                      v_out: Optional[torch.Tensor] = None, out_slots: Optional[torch.Tensor] = None):
+    """Blocks block_ids[i] of the quantised cache -> block out_slots[i] (or i) of bf16 paged caches, which are allocated
+    ([n, block_tokens, n_kv_heads, head_dim]) where none are given.  Returns (k_out, v_out)."""
+    _need_cuda(cache.data, block_ids, k_out, v_out, out_slots)
+    g = cache.geometry
+    ids = _i32(block_ids, "block_ids")
+    n = ids.numel()
+    if (k_out is None) != (v_out is None) or (k_out is None and out_slots is not None):
+        raise ValueError("give both outputs, or neither and no out_slots")
+    if out_slots is not None and out_slots.numel() != n:
+        raise ValueError("one out_slots entry per block id")
+    if k_out is None:
+        k_out, v_out = (torch.zeros((n, g.block_tokens, g.n_kv_heads, g.head_dim), dtype=torch.bfloat16, device=cache.data.device)
+                        for _ in range(2))
+    with _same_device(cache.data, block_ids, k_out, v_out, out_slots):
+        st = N.lib.ucmx_quant_read_blocks(_ptr(cache.data), C.byref(g), _ptr(ids), _ptr(_i32(out_slots, "out_slots")), n, _ptr(k_out),
+                                          C.byref(kv_geometry(k_out)), _ptr(v_out), C.byref(kv_geometry(v_out)), _stream(cache.data))
+    N.check("ucmx_quant_read_blocks", st, 1 if n else 0)
+    return k_out, v_out
+
+
+def attention_workspace(query: torch.Tensor, n_kv_heads: int, *, max_q_tokens: int = 1, bits: int = 16) -> torch.Tensor:
+    """Scratch for block_attention (bits 16) or quant_block_attention (bits of the cache) with queries of this shape, whatever the
+    lists; to be kept where the calls must not allocate.  Calls that may overlap need one each."""
+    with torch.cuda.device(query.device):
+        need = int(N.lib.ucmx_attention_workspace_bytes(bits, query.shape[1], n_kv_heads, query.shape[2], max_q_tokens))
+    if need == 0:
+        raise ValueError("unsupported attention shape: head_dim 64, 128 or 256, query heads a multiple of the KV heads")
+    return torch.empty((need,), dtype=torch.uint8, device=query.device)
+
+
+def _attend(name: str, bits: int, n_kv_heads: int, head_dim: int, cache_args, caches, query, req_offsets, block_ids, positions,
+            block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out, lse, workspace):
+    _need_cuda(query, req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, out, lse,
+               workspace, *caches)
+    if query.dim() != 3 or query.dtype != torch.bfloat16 or query.shape[2] != head_dim:
+        raise ValueError(f"query must be bf16 [n_query_tokens, n_q_heads, {head_dim}]")
+    n_tok, Hq, D = query.shape
+    if query.stride()[1:] != (D, 1) or (n_tok > 1 and query.stride(0) % 8):
+        query = query.contiguous()
+    n_req = req_offsets.numel() - 1
+    if n_req < 0:
+        raise ValueError("req_offsets must hold n_req + 1 entries")
+    if block_ids is None and (positions is None or block_table is None or table_offsets is None):
+        raise ValueError("give block_ids, or positions with block_table and table_offsets")
+    if block_ids is not None and block_table is not None:
+        raise ValueError("give block_ids or block_table, not both")
+    entries = block_ids if block_ids is not None else positions
+    for t, n, what in ((block_ids, entries.numel(), "block_ids"), (positions, entries.numel(), "positions"), (req_counts, n_req, "req_counts"),
+                       (ctx_lens, n_req, "ctx_lens"), (q_offsets, n_req + 1, "q_offsets"), (table_offsets, n_req + 1, "table_offsets")):
+        if t is not None and t.numel() != n:
+            raise ValueError(f"{what} must hold {n} entries")
+    if q_offsets is None and (n_tok != n_req or max_q_tokens != 1):
+        raise ValueError("without q_offsets there is one query token per request")
+    if out is None:
+        out = torch.empty((n_tok, Hq, D), dtype=torch.bfloat16, device=query.device)
+    elif out.dtype != torch.bfloat16 or not out.is_contiguous() or tuple(out.shape) != (n_tok, Hq, D):
+        raise ValueError("out must be contiguous bf16 of the query's shape")
+    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (n_tok, Hq)):
+        raise ValueError("lse must be contiguous fp32 [n_query_tokens, n_q_heads]")
+    if n_req == 0 or n_tok == 0:
+        return out
+    with _same_device(query, req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, out, lse,
+                      workspace, *caches):
+        if workspace is None:
+            workspace = attention_workspace(query, n_kv_heads, max_q_tokens=max_q_tokens, bits=bits)
+        adr = lambda t, what: 0 if t is None else _i32(t, what).data_ptr()  # noqa: E731
+        lists = N.BlockLists(adr(req_offsets, "req_offsets"), adr(req_counts, "req_counts"), adr(block_ids, "block_ids"),
+                             adr(positions, "positions"), adr(block_table, "block_table"), adr(table_offsets, "table_offsets"),
+                             adr(ctx_lens, "ctx_lens"), n_req, entries.numel())
+        st = getattr(N.lib, name)(_ptr(query), query.stride(0) if n_tok > 1 else Hq * D, Hq, _ptr(_i32(q_offsets, "q_offsets")), n_tok,
+                                  max_q_tokens, *cache_args, C.byref(lists), float(D ** -0.5 if scale is None else scale), _ptr(out),
+                                  _ptr(lse), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(query))
+    N.check(name, st, 2)
+    return out
+
+
+def block_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, req_offsets: torch.Tensor, *,
+                    block_ids: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                    block_table: Optional[torch.Tensor] = None, table_offsets: Optional[torch.Tensor] = None,
+                    ctx_lens: Optional[torch.Tensor] = None, req_counts: Optional[torch.Tensor] = None,
+                    q_offsets: Optional[torch.Tensor] = None, max_q_tokens: int = 1, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of every request's query tokens over the KV blocks listed for it; returns bf16 [n_query_tokens, n_q_heads, head_dim].
+
+    query bf16 [n_query_tokens, n_q_heads, head_dim]; k_cache, v_cache bf16 [num_blocks, block_tokens, n_kv_heads, head_dim].
+    The lists are int32, request r's entries [req_offsets[r], req_offsets[r+1]), cut to req_counts[r] where given:
+    block_ids are physical blocks (what topk_ragged returns with id_map, or remap_resident's table); or positions are places in
+    the sequence (topk_ragged without id_map) and block_table / table_offsets the requests' block tables.  Negative = skip.
+    With both block_ids and positions the latter only say where the blocks stand; without positions the i-th stands at i.
+    ctx_lens: lengths of the sequences; tokens at or beyond are not seen (nor read), and of a request's n query tokens the j-th
+    sees n-1-j fewer.  Without it every token of every listed block is seen.
+    q_offsets, max_q_tokens: each request's query tokens (one each without).  A query that sees nothing gives zeros.
+    lse: fp32 [n_query_tokens, n_q_heads], receives the logarithm of the softmax's sum.  scale defaults to head_dim ** -0.5."""
+    kg, vg = kv_geometry(k_cache), kv_geometry(v_cache)
+    args = (_ptr(k_cache), C.byref(kg), _ptr(v_cache), C.byref(vg))
+    return _attend("ucmx_block_attention", 16, kg.n_kv_heads, kg.head_dim, args, (k_cache, v_cache), query, req_offsets, block_ids, positions,
+                   block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out, lse, workspace)
+
+
+def quant_block_attention(query: torch.Tensor, cache: QuantKvCache, req_offsets: torch.Tensor, *,
+                          block_ids: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                          block_table: Optional[torch.Tensor] = None, table_offsets: Optional[torch.Tensor] = None,
+                          ctx_lens: Optional[torch.Tensor] = None, req_counts: Optional[torch.Tensor] = None,
+                          q_offsets: Optional[torch.Tensor] = None, max_q_tokens: int = 1, scale: Optional[float] = None,
+                          out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                          workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """block_attention over a quantised cache: the codes are read in place and never written out as bf16."""
+    g = cache.geometry
+    return _attend("ucmx_quant_block_attention", g.bits, g.n_kv_heads, g.head_dim, (_ptr(cache.data), C.byref(g)), (cache.data,), query,
+                   req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out,
+                   lse, workspace)
