@@ -605,8 +605,8 @@ int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_geometry* geo
  *   table[table_offsets[r] + positions[e]] (the request's row of a block table; table_offsets has n_req+1 entries).
  *   positions[e] is the block's place in its sequence, negative = skip; with positions NULL the i-th entry stands at i.
  *   ctx_lens[r] (or NULL: every token of every listed block is seen) is the length of the sequence, the query tokens included:
- *   query token j of the request's n sees the tokens at places below ctx_lens[r] - (n-1-j).  Tokens nobody may see are not
- *   read, and may hold anything.
+ *   query token j of the request's n sees the tokens at places below ctx_lens[r] - (n-1-j).  What stands in tokens that a
+ *   query does not see, NaN and infinities among it, does not reach its result.
  * An id beyond its cache or table is dropped and reported (ucmx_device_error code 3).
  * q is bf16 [n_q_tokens, n_q_heads, head_dim], q_stride elements between tokens (a multiple of 8).  q_offsets (n_req+1 entries)
  *   gives each request's query tokens, at most max_q_tokens; NULL: one each.  Rows of out behind q_offsets[n_req] stay as they are.

@@ -1,12 +1,14 @@
 // Attention over listed blocks: the C entries, their checks, and the bf16 cache's instances (kernel: attend.cuh).
+#include <mutex>
+
 #include "attend.cuh"
 
 namespace ucmx {
 namespace attend {
 
-int32_t run_bf16(const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st)
+int32_t run_bf16(const Params& p, int head_dim, int cols, const Maps* maps, Plan* plan, cudaStream_t st)
 {
-    return run_format<16>(p, head_dim, cols, launch, plan, st);
+    return run_format<16>(p, head_dim, cols, maps, plan, st);
 }
 
 namespace {
@@ -17,11 +19,43 @@ int32_t refuse(const char* why, int32_t code = UCMX_EPARAM)
     return code;
 }
 
-int32_t run_any(int bits, const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st)
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn()
 {
-    return bits == 16 ? run_bf16(p, head_dim, cols, launch, plan, st)
-         : bits == 8  ? run_q8(p, head_dim, cols, launch, plan, st)
-                      : run_q4(p, head_dim, cols, launch, plan, st);
+    static std::mutex mu;
+    static EncodeTiledFn fn = nullptr;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiledFn)p;
+    }
+    return fn;
+}
+
+// one side of the bf16 cache as a tensor [block][token][head][value], loaded 64 values x `box` tokens at a time
+bool make_map(CUtensorMap* map, const uint8_t* base, const Params& p, int head_dim, int64_t token_bytes, int64_t block_bytes)
+{
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)p.H, (cuuint64_t)p.T, (cuuint64_t)p.n_blocks};
+    const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)token_bytes,
+                                   (cuuint64_t)(block_bytes > 0 ? block_bytes : token_bytes)};   // (one block: any stride will do)
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)p.box, 1}, one[4] = {1, 1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint8_t*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int32_t run_any(int bits, const Params& p, int head_dim, int cols, const Maps* maps, Plan* plan, cudaStream_t st)
+{
+    return bits == 16 ? run_bf16(p, head_dim, cols, maps, plan, st)
+         : bits == 8  ? run_q8(p, head_dim, cols, maps, plan, st)
+                      : run_q4(p, head_dim, cols, maps, plan, st);
 }
 
 // what both entries check and fill in; the cache's part of `p` is set by the caller
@@ -66,14 +100,22 @@ int32_t attend_common(Params& p, int bits, int32_t head_dim, const void* q, int6
     p.err = error_word();
     const int cols = max_q_tokens * p.G;
     Plan plan;
-    const int32_t rc = run_any(bits, p, head_dim, cols, false, &plan, nullptr);
+    const int32_t rc = run_any(bits, p, head_dim, cols, nullptr, &plan, nullptr);
     if (rc != UCMX_OK) return refuse("attention: head_dim must be 64, 128 or 256", rc);
     if (workspace_bytes < (size_t)plan.ctas * 2 * plan.part * sizeof(float)) return refuse("attention: workspace too small");
     p.cols_per_tile = plan.cols;
     p.col_tiles = (cols + plan.cols - 1) / plan.cols;
-    // a request's slices of all heads and tiles are counted in 32 bits inside the kernel
-    if ((int64_t)p.total * p.spe > INT32_MAX) return refuse("attention: more than 2^31 slices in the lists", UCMX_EUNSUPPORTED);
-    return run_any(bits, p, head_dim, cols, true, &plan, (cudaStream_t)stream);
+    // the slices of all requests, heads and tiles are numbered in 32 bits
+    if ((int64_t)p.total * p.spe > INT32_MAX / 2 || (int64_t)p.total * p.spe * p.H > INT32_MAX / 2 ||
+        (int64_t)p.total * p.spe * p.H * p.col_tiles > INT32_MAX - (1 << 20))
+        return refuse("attention: more than 2^31 pieces of 16 tokens in the lists of all heads", UCMX_EUNSUPPORTED);
+    Maps maps = {};
+    if (bits == 16 && p.total > 0) {
+        p.box = p.T < kRows ? p.T : kRows;
+        if (!make_map(&maps.k, p.k, p, head_dim, p.k_token, p.k_block) || !make_map(&maps.v, p.v, p, head_dim, p.v_token, p.v_block))
+            return refuse("attention: no tensor map for a cache with these strides", UCMX_EUNSUPPORTED);
+    }
+    return run_any(bits, p, head_dim, cols, &maps, &plan, (cudaStream_t)stream);
 }
 
 }  // namespace
@@ -89,7 +131,7 @@ extern "C" size_t ucmx_attention_workspace_bytes(int32_t bits, int32_t n_q_heads
     Plan plan;
     Params p = {};
     const int64_t cols = (int64_t)max_q_tokens * (n_q_heads / n_kv_heads);
-    if (run_any(bits, p, head_dim, cols > 64 ? 64 : (int)cols, false, &plan, nullptr) != UCMX_OK) return 0;
+    if (run_any(bits, p, head_dim, cols > 64 ? 64 : (int)cols, nullptr, &plan, nullptr) != UCMX_OK) return 0;
     return (size_t)plan.ctas * 2 * plan.part * sizeof(float);
 }
 

@@ -24,6 +24,8 @@
 // share one instruction (columns 4..7 repeat 0..3), otherwise they are two.
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace ucmx {
@@ -49,6 +51,7 @@ struct Params {
     int64_t k_block, v_block;          // bytes between blocks
     int64_t k_token, v_token;          // bytes between tokens (bf16)
     int32_t T, spe;                    // tokens per block, slices per block
+    int32_t box;                       // bf16: rows that one load brings, min(16, T)
     int64_t n_blocks;
     const int32_t* offsets;            // [n_req+1] into the lists
     const int32_t* counts;             // [n_req] or NULL
@@ -66,24 +69,29 @@ struct Params {
     int32_t* err;
 };
 
+// K and V of the bf16 cache as tensors [block][token][head][value]; unused for the quantised cache.
+struct Maps {
+    CUtensorMap k, v;
+};
+
 // One item's part inside a thread block's range.
 struct Seg {
-    int64_t begin, end;                // of the whole item, in the order of all slices
-    int64_t lo, hi;                    // the part of it
+    int32_t begin, end;                // of the whole item, in the order of all slices
+    int32_t lo, hi;                    // the part of it
     int32_t r, h, ct;
     int32_t first;                     // offsets[r]
     int32_t n;                         // entries of the request's list
 };
 
 // The last r with offsets[r] <= e (a warp probes 32 places at a time).  All lanes get it.
-__device__ __forceinline__ int request_of(const int32_t* __restrict__ offsets, int n_req, int64_t e)
+__device__ __forceinline__ int request_of(const int32_t* __restrict__ offsets, int n_req, int32_t e)
 {
     const int lane = threadIdx.x & 31;
     int lo = 0, n = n_req;
     while (n > 1) {
         const int step = (n + 31) >> 5;
         const int at = lo + lane * step;
-        const bool below = lane * step < n && (int64_t)__ldg(offsets + at) <= e;
+        const bool below = lane * step < n && __ldg(offsets + at) <= e;
         const int c = __popc(__ballot_sync(0xffffffffu, below));
         const int adv = (c > 0 ? c - 1 : 0) * step;
         lo += adv;
@@ -92,29 +100,29 @@ __device__ __forceinline__ int request_of(const int32_t* __restrict__ offsets, i
     return lo;
 }
 
-__device__ __forceinline__ int64_t entries_total(const Params& p)
+__device__ __forceinline__ int32_t entries_total(const Params& p)
 {
     const int32_t n = __ldg(p.offsets + p.n_req);      // a captured batch may use less than its capacity
     return n < 0 ? 0 : n < p.total ? n : p.total;
 }
-__device__ __forceinline__ int64_t slices_per_entry(const Params& p) { return (int64_t)p.spe * p.H * p.col_tiles; }
+__device__ __forceinline__ int32_t slices_per_entry(const Params& p) { return p.spe * p.H * p.col_tiles; }
 
-__device__ __forceinline__ int64_t cut(int64_t all, int c, int n) { return all / n * c + all % n * c / n; }
+// Part c of n equal parts begins at min(all, c * ceil(all / n)).  (The host keeps all + n below 2^31.)
+__device__ __forceinline__ int32_t part_size(int32_t all, int32_t n) { return (int32_t)(((uint32_t)all + (uint32_t)n - 1u) / (uint32_t)n); }
 
 // The item that holds position `at` (< hi); called by whole warps.
-__device__ __forceinline__ Seg segment_at(const Params& p, int64_t at, int64_t hi)
+__device__ __forceinline__ Seg segment_at(const Params& p, int32_t at, int32_t hi)
 {
     Seg s;
-    const int64_t spe = slices_per_entry(p);
+    const int32_t spe = slices_per_entry(p);
     s.r = request_of(p.offsets, p.n_req, at / spe);
     s.first = __ldg(p.offsets + s.r);
     s.n = min(__ldg(p.offsets + s.r + 1), p.total) - s.first;
-    const int64_t item = (int64_t)s.n * p.spe;         // slices of one (KV head, column tile)
-    const int64_t rel = at - (int64_t)s.first * spe;
-    const int32_t i = (int32_t)(rel / item);
+    const int32_t item = s.n * p.spe;                  // slices of one (KV head, column tile)
+    const int32_t i = (at - s.first * spe) / item;
     s.h = i / p.col_tiles;
     s.ct = i - s.h * p.col_tiles;
-    s.begin = (int64_t)s.first * spe + (int64_t)i * item;
+    s.begin = s.first * spe + i * item;
     s.end = s.begin + item;
     s.lo = at;
     s.hi = s.end < hi ? s.end : hi;
@@ -137,7 +145,26 @@ __device__ __forceinline__ void queries_of(const Params& p, int r, int& q0, int&
     }
 }
 
-__device__ __forceinline__ float exp2_fast(float x) { return exp2f(x); }
+// 2^x for a weight: x is at most kMaxSlack, and what is below 2^-126 of the largest weight is nothing
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 64 values of `box` tokens of one head -> rows of 128 bytes, their 16-byte pieces XORed with the row (mod 8)
+__device__ __forceinline__ void load_panel(unsigned char* dst, const CUtensorMap* map, int x, int h, int token, int block, uint64_t* bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(h), "r"(token), "r"(block), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
 {
@@ -160,6 +187,26 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float f16lo(uint32_t x) { return __half2float(__ushort_as_half((unsigned short)x)); }
+__device__ __forceinline__ float f16hi(uint32_t x) { return __half2float(__ushort_as_half((unsigned short)(x >> 16))); }
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
 {
@@ -192,19 +239,49 @@ __device__ __forceinline__ uint32_t lds4(uint32_t a)
     return v;
 }
 
-// Codes to centred integers in bf16 (exact): 4 bits: c - 8, two per register from bits [4i, 4i+4) of both halves.
+template <int BYTES>
+__device__ __forceinline__ void lds_words(uint32_t (&w)[4], uint32_t a)
+{
+    if (BYTES == 16) {
+        const uint4 u = lds16(a);
+        w[0] = u.x;
+        w[1] = u.y;
+        w[2] = u.z;
+        w[3] = u.w;
+    } else {
+        const uint2 u = lds8(a);
+        w[0] = u.x;
+        w[1] = u.y;
+    }
+}
+
+// V's codes as centred integers in bf16 (exact): 4 bits: c - 8, two per register from bits [4i, 4i+4) of both halves.
 // 0x4300 is 128.0 and a bf16 of that size counts in ones, so or-ing the code in adds it.
-__device__ __forceinline__ uint32_t nibbles(uint32_t w, int i)
+__device__ __forceinline__ uint32_t v_nibbles(uint32_t w, int i)
 {
     return sub_bf16x2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, 0x43084308u);
 }
 // 8 bits: c - 128 from bytes i and i+2.  The low seven bits are or-ed into 128.0; the top bit chooses what is taken off:
 // 256.0 (0x4380) where it is clear, 128.0 (0x4300) where it is set.
-__device__ __forceinline__ uint32_t bytes(uint32_t w, int i)
+__device__ __forceinline__ uint32_t v_bytes(uint32_t w, int i)
 {
     const uint32_t x = w >> (8 * i);
     return sub_bf16x2((x & 0x007f007fu) | 0x43004300u, (~x & 0x00800080u) | 0x43004300u);
 }
+// K's codes become fp16, whose eleven bits hold two nibble positions: half the shifts, and half or none of the subtractions.
+// (The queries can follow: a column scaled by a power of two fits fp16 to 2^-25 of its largest value.  The weights cannot:
+// their range is not bounded.)  0x6400 is 1024.0, counting in ones.  4 bits: registers i = 0, 2 hold c - 8, registers i = 1, 3
+// hold 1024 + 16 c, whose 1024 + 128 the accumulator starts below (kOddOffset times those queries' sum) and whose 16 is in the
+// queries.  With that offset in all four the sums would lose four bits more.
+__device__ __forceinline__ uint32_t k_nibbles(uint32_t w, int i)
+{
+    const uint32_t x = i < 2 ? w : w >> 8;
+    if (i & 1) return (x & 0x00f000f0u) | 0x64006400u;
+    return sub_f16x2((x & 0x000f000fu) | 0x64006400u, 0x64086408u);
+}
+// 8 bits: 1024 + c of bytes 2i and 2i+1: one instruction; the accumulator starts 1024 + 128 times the queries' sum below.
+__device__ __forceinline__ uint32_t k_bytes(uint32_t w, int i) { return __byte_perm(w, 0x64646464u, i ? 0x4342 : 0x4140); }
+constexpr float kOddOffset = 1024.f + 128.f;
 
 // FMT 16: bf16 cache, rows of K and V; 8 or 4: groups of the quantised cache.
 template <int FMT, int D>
@@ -214,27 +291,33 @@ struct Layout {
     static constexpr int kPanels = kRowBytes / kPanel;
     static constexpr int kPanelDims = D / kPanels;
     static constexpr int kGroup = 2 * kRows * kRowBytes + 2 * kRows * 4;  // quantised: codes of K and V, then their scales
-    static constexpr int kRowStride = kRowBytes + 16;                     // bf16: rows in shared memory, off the bank period
-    static constexpr int kStage = FMT == 16 ? 2 * kRows * kRowStride : kGroup;
-    static constexpr int kStages = kStage > 8400 && D == 256 ? 2 : kStage > 8000 && FMT != 16 ? 2 : kStage > 4000 ? 3 : 4;
+    static constexpr int kBf16Panel = kRows * 128;                        // bf16: 64 values of 16 rows in shared memory
+    // slices a warp takes at a time: two of the codes' (twice the independent work between waits), one of bf16 rows
+    static constexpr int kUnits = FMT == 16 ? 1 : 2;
+    static constexpr int kUnit = FMT == 16 ? 2 * kRows * kRowBytes : kGroup;
+    static constexpr int kStage = kUnits * kUnit;
 };
 
 template <int FMT, int D, int NT, bool DUP>
 struct Traits {
     using L = Layout<FMT, D>;
     static constexpr int kCols = DUP ? 4 : 8 * NT;       // columns of a tile
+    // stages of a warp's ring: what keeps about twice the latency-bandwidth product of 45 KB in flight per SM and leaves
+    // room for the thread blocks that the registers allow
+    static constexpr int kStages = FMT == 16 && D <= 128 && NT == 1 ? 3 : 2;
     static constexpr int kKSteps = D / 16;
     static constexpr int kMTiles = D / 16;
     static constexpr bool kQReg = kKSteps * NT <= 16;    // query fragments in registers (else in shared memory)
     static constexpr int kMergeLd = D + 4;
     static constexpr int kMergeCols = 4;                 // columns joined at a time
     static constexpr int kMergeSteps = DUP ? 1 : 2 * NT;
-    static constexpr int kRingBytes = kWarps * L::kStages * L::kStage;
+    static constexpr int kRingBytes = kWarps * kStages * L::kStage;
     static constexpr int kMergeBytes = kWarps * kMergeCols * kMergeLd * 4;
     static constexpr int kStatBytes = kWarps * kCols * 3 * 4;
     static constexpr int kQBytes = kQReg ? 0 : kKSteps * NT * 32 * 8;
-    static constexpr int kBarBytes = 16 * kWarps * L::kStages;            // a barrier (8) and the stage's note (8)
-    static constexpr int kSmem = kRingBytes + kMergeBytes + kStatBytes + kQBytes + kBarBytes;
+    static constexpr int kBarStride = kStages * (8 + 8 * L::kUnits);     // a warp's barriers, and a note (8) per slice
+    static constexpr int kBarBytes = kWarps * kBarStride;
+    static constexpr int kSmem = 1024 + kRingBytes + kMergeBytes + kStatBytes + kQBytes + kBarBytes;   // (1024: alignment)
     static constexpr int kPart = kCols * (D + 2);        // floats of a partial result: m, l, then the rows
     // thread blocks per SM: what shared memory holds (228 KB, 1 KB of it per block), and the registers of the accumulators
     static constexpr int kBySmem = 233472 / (kSmem + 1024);
@@ -243,30 +326,32 @@ struct Traits {
 };
 
 template <int FMT, int D, int NT, bool DUP>
-__global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) attend_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) attend_kernel(const Params p, const __grid_constant__ Maps maps)
 {
     using X = Traits<FMT, D, NT, DUP>;
     using L = typename X::L;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(128) unsigned char smem_raw[];
+    unsigned char* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);   // the panels' pattern repeats every 1024 bytes
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, q4 = lane & 3;
 
-    unsigned char* const ring = smem + warp * (L::kStages * L::kStage);
+    unsigned char* const ring = smem + warp * (X::kStages * L::kStage);
     float* const merge = reinterpret_cast<float*>(smem + X::kRingBytes);
     float* const stat = reinterpret_cast<float*>(smem + X::kRingBytes + X::kMergeBytes);     // [warp][3][cols]
     uint2* const q_frag = reinterpret_cast<uint2*>(smem + X::kRingBytes + X::kMergeBytes + X::kStatBytes);
-    unsigned char* const bars = smem + X::kRingBytes + X::kMergeBytes + X::kStatBytes + X::kQBytes + warp * (16 * L::kStages);
+    unsigned char* const bars = smem + X::kRingBytes + X::kMergeBytes + X::kStatBytes + X::kQBytes + warp * X::kBarStride;
     uint64_t* const full = reinterpret_cast<uint64_t*>(bars);
-    int2* const note = reinterpret_cast<int2*>(bars + 8 * L::kStages);    // .x tokens copied (0: nothing), .y first position
+    int2* const note = reinterpret_cast<int2*>(bars + 8 * X::kStages);    // .x tokens copied (0: nothing), .y first position
 
     if (lane == 0) {
-        for (int s = 0; s < L::kStages; ++s) mbar_init(&full[s], 1);
+        for (int s = 0; s < X::kStages; ++s) mbar_init(&full[s], 1);
         mbar_init_fence();
     }
     __syncwarp();
 
-    const int64_t all = entries_total(p) * slices_per_entry(p);
-    const int64_t lo = cut(all, blockIdx.x, gridDim.x), hi = cut(all, blockIdx.x + 1, gridDim.x);
+    const int32_t all = entries_total(p) * slices_per_entry(p);
+    const int32_t size = part_size(all, gridDim.x);
+    const int32_t lo = min(all, (int32_t)blockIdx.x * size), hi = lo + min(size, all - lo);
     early_start_allow();
 
     // requests that list nothing have no slices: their rows are written here
@@ -282,26 +367,24 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     if (lo >= hi) return;
 
     // ---- the warp's loads run ahead of its arithmetic, across items: a cursor of their own
+    constexpr int kU = L::kUnits, kStep = kWarps * kU;
     Seg ps;
     ps.hi = -1;
-    int64_t p_at = 0;                  // next slice to load of segment ps
-    int64_t p_batch = 0;               // lane i knows slice p_batch + 4 i
-    int32_t my_id = -1, my_nv = 0, my_pos = 0;
-    int32_t p_sub = 0;                 // first token of my slice inside its block
+    int32_t p_at = 0;                  // next slice to load of segment ps
+    int32_t p_look = 32;               // lanes p_look .. p_look + kU - 1 know the slices to load next; 32: look again
+    int32_t p_entries = 0;             // entries of the request that count
+    int32_t p_end = 0;                 // first position that no column of the tile sees
+    int32_t my_id = 0, my_pos = 0;     // this lane's slice: block, first position,
+    uint32_t my_span = 0;              // first token inside the block * 32 + tokens to load
     bool p_done = false;
-    int64_t p_next = lo;               // where the next segment begins
-
+    int32_t p_next = lo;               // where the next segment begins
     // what this lane has to know of slice `at` of segment ps
-    auto look_up = [&](int64_t at) {
-        my_id = -1;
-        my_nv = 0;
+    auto look_up = [&](int32_t at) {
+        my_span = 0;
         if (at >= ps.hi) return;
-        const int32_t s = (int32_t)(at - ps.begin);
-        const int32_t e = s / p.spe, sub = s - e * p.spe;
-        p_sub = sub * kRows;
-        int32_t cnt = ps.n;
-        if (p.counts) cnt = min(cnt, __ldg(p.counts + ps.r));
-        if (e >= cnt) return;
+        const int32_t s = at - ps.begin;
+        const int32_t e = s / p.spe, sub = (s - e * p.spe) * kRows;
+        if (e >= p_entries) return;
         const int32_t at_list = ps.first + e;
         const int32_t pos_block = p.positions ? __ldg(p.positions + at_list) : e;
         if (pos_block < 0) return;
@@ -321,79 +404,90 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             if (p.err) atomicExch(p.err, 3);
             return;
         }
-        int32_t nv = min(kRows, p.T - p_sub);
+        int32_t nv = min(kRows, p.T - sub);
         if (p.ctx) {
-            int q0, nq;
-            queries_of(p, ps.r, q0, nq);
-            const int64_t pos = (int64_t)pos_block * p.T + p_sub;
-            const int32_t j = min(nq - 1, (ps.ct * X::kCols + X::kCols - 1) / p.G);     // the tile's last query token
-            const int64_t end = (int64_t)__ldg(p.ctx + ps.r) - (nq - 1 - j);
-            if (pos >= end) return;
-            nv = (int32_t)min((int64_t)nv, end - pos);
+            const int64_t pos = (int64_t)pos_block * p.T + sub;
+            if (pos >= p_end) return;
+            nv = (int32_t)min((int64_t)nv, p_end - pos);
             my_pos = (int32_t)pos;
         }
         my_id = id;
-        my_nv = nv;
+        my_span = (uint32_t)sub * 32u + (uint32_t)nv;
     };
-    // start the loads of the warp's next slice into stage s; false when the range is exhausted
+    // start the loads of the warp's next step into stage s; every step completes its barrier, with or without bytes
     auto issue = [&](int s) {
-        while (!p_done && p_at >= ps.hi) {
-            if (p_next >= hi) {
-                p_done = true;
-                break;
+        if (p_at >= ps.hi) {
+            while (!p_done && p_at >= ps.hi) {
+                if (p_next >= hi) {
+                    p_done = true;
+                    break;
+                }
+                ps = segment_at(p, p_next, hi);
+                p_next = ps.hi;
+                p_at = ps.lo + warp * kU;
+                p_look = 32;
+                p_entries = p.counts ? min(ps.n, __ldg(p.counts + ps.r)) : ps.n;
+                if (p.ctx) {
+                    int q0, nq;
+                    queries_of(p, ps.r, q0, nq);
+                    p_end = __ldg(p.ctx + ps.r) - (nq - 1 - min(nq - 1, (ps.ct * X::kCols + X::kCols - 1) / p.G));
+                }
             }
-            ps = segment_at(p, p_next, hi);
-            p_next = ps.hi;
-            p_at = ps.lo + warp;
-            p_batch = p_at;
-            look_up(p_at + (int64_t)lane * kWarps);
+            if (p_done) return;
         }
-        if (p_done) return;
-        if (p_at >= p_batch + 32 * kWarps) {
-            p_batch = p_at;
-            look_up(p_at + (int64_t)lane * kWarps);
+        if (p_look >= 32) {
+            look_up(p_at + (lane / kU) * kStep + lane % kU);
+            p_look = 0;
         }
-        const int src = (int)((p_at - p_batch) / kWarps);
-        const int32_t id = __shfl_sync(0xffffffffu, my_id, src);
-        const int32_t nv = __shfl_sync(0xffffffffu, my_nv, src);
-        const int32_t pos = __shfl_sync(0xffffffffu, my_pos, src);
-        const int32_t sub = __shfl_sync(0xffffffffu, p_sub, src);
-        p_at += kWarps;
-        if (lane == 0) note[s] = make_int2(nv, pos);
-        if (nv <= 0) return;
+        const int from = p_look + lane % kU;
+        const int32_t id = __shfl_sync(0xffffffffu, my_id, from);
+        const uint32_t span = __shfl_sync(0xffffffffu, my_span, from);
+        const int32_t pos = __shfl_sync(0xffffffffu, my_pos, from);
+        const int nv = span & 31u;
+        const int32_t sub = (int32_t)(span >> 5);
+        p_at += kStep;
+        p_look += kU;
         unsigned char* const dst = ring + s * L::kStage;
+        if (lane < kU) note[s * kU + lane] = make_int2(nv, pos);
         if (FMT == 16) {
-            if (lane == 0) mbar_expect_tx(&full[s], (uint32_t)(2 * nv) * L::kRowBytes);
-            __syncwarp();
-            const int row = lane & 15;
-            const bool is_v = lane >= 16;
-            unsigned char* const d = dst + (is_v ? kRows : 0) * L::kRowStride + row * L::kRowStride;
-            if (row < nv) {
-                const uint8_t* const srcp = is_v ? p.v + (int64_t)id * p.v_block + (int64_t)(sub + row) * p.v_token
-                                                 : p.k + (int64_t)id * p.k_block + (int64_t)(sub + row) * p.k_token;
-                bulk_g2s(d, srcp + (int64_t)ps.h * L::kRowBytes, L::kRowBytes, &full[s]);
-            } else if (is_v) {          // rows without a token: a weight of zero must meet a number
+            if (lane == 0) {
+                if (nv > 0) {
+                    mbar_expect_tx(&full[s], (uint32_t)(2 * p.box) * L::kRowBytes);
 #pragma unroll
-                for (int i = 0; i < L::kRowBytes / 16; ++i) *reinterpret_cast<uint4*>(d + i * 16) = make_uint4(0, 0, 0, 0);
-                fence_proxy_async();
+                    for (int i = 0; i < D / 64; ++i) {
+                        load_panel(dst + i * L::kBf16Panel, &maps.k, i * 64, ps.h, sub, id, &full[s]);
+                        load_panel(dst + (D / 64 + i) * L::kBf16Panel, &maps.v, i * 64, ps.h, sub, id, &full[s]);
+                    }
+                } else {
+                    mbar_arrive(&full[s]);
+                }
             }
-        } else if (lane == 0) {
-            mbar_expect_tx(&full[s], L::kGroup);
-            const int64_t groups = p.T / kRows;
-            bulk_g2s(dst, p.k + (int64_t)id * p.k_block + ((int64_t)ps.h * groups + sub / kRows) * L::kGroup, L::kGroup, &full[s]);
+        } else {
+            // two slices that follow one another in one block are one copy
+            const int32_t id1 = __shfl_sync(0xffffffffu, id, 1), sub1 = __shfl_sync(0xffffffffu, sub, 1), nv1 = __shfl_sync(0xffffffffu, nv, 1);
+            const bool both = id1 == __shfl_sync(0xffffffffu, id, 0) && sub1 == __shfl_sync(0xffffffffu, sub, 0) + kRows &&
+                              nv1 > 0 && __shfl_sync(0xffffffffu, nv, 0) > 0;
+            const uint8_t* const src = p.k + (int64_t)id * p.k_block + (int64_t)(ps.h * p.spe + (sub >> 4)) * L::kGroup;
+            if (lane == 0) {
+                const uint32_t bytes = nv > 0 ? (both ? 2 * L::kGroup : L::kGroup) : 0;
+                mbar_expect_tx(&full[s], bytes + (!both && nv1 > 0 ? L::kGroup : 0));
+                if (nv > 0) bulk_g2s(dst, src, bytes, &full[s]);
+            }
+            __syncwarp();
+            if (lane == 1 && !both && nv > 0) bulk_g2s(dst + L::kUnit, src, L::kGroup, &full[s]);
         }
     };
 
 #pragma unroll 1
-    for (int s = 0; s < L::kStages; ++s) issue(s);
+    for (int s = 0; s < X::kStages; ++s) issue(s);
     __syncwarp();
 
     int stage = 0;
-    uint32_t phases = 0;
+    uint32_t parity = 0;
     bool dead = false;
     const uint32_t ring_u = smem_u32(ring);
 
-    int64_t at = lo;
+    int32_t at = lo;
 #pragma unroll 1
     while (at < hi) {
         const Seg sg = segment_at(p, at, hi);
@@ -419,9 +513,10 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             for (int nt = 0; nt < NT; ++nt) limit[nt][0] = limit[nt][1] = INT32_MAX;
         }
 
-        // ---- query fragments (the order of the values follows that of the codes), and their sums for the zeros
+        // ---- query fragments.  bf16 cache: as they are.  Codes: in the order of the codes, scaled by a power of two per column
+        // to fp16; `qoff` is what the accumulators start from, `qsum` and `qmul` turn them into scores.
         uint32_t qf[X::kQReg ? X::kKSteps : 1][X::kQReg ? NT : 1][2];
-        float qsum[NT][2];
+        float qsum[NT][2], qmul[NT][2], qoff[NT][2];
         if (!X::kQReg) __syncthreads();            // the item before may still be read
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -430,9 +525,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             const bool live = cc < cols;
             const int j = live ? c / p.G : 0;
             const uint16_t* const qp = p.q + (int64_t)(q0 + j) * p.q_stride + (int64_t)(sg.h * p.G + (live ? c - j * p.G : 0)) * D;
-            float sum = 0.f;
             auto put = [&](int ks, uint32_t b0, uint32_t b1) {
-                if (FMT != 16) sum += (bf16lo(b0) + bf16hi(b0)) + (bf16lo(b1) + bf16hi(b1));
                 if (X::kQReg) {
                     qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][0] = b0;
                     qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][1] = b1;
@@ -447,42 +540,88 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                     const uint32_t b1 = live ? __ldg(reinterpret_cast<const uint32_t*>(qp + ks * 16 + 8 + 2 * q4)) : 0u;
                     put(ks, b0, b1);
                 }
-            } else if (FMT == 4) {
-                constexpr int kWords = L::kPanelDims / 32;       // words of 8 codes a lane has in a panel
-#pragma unroll
-                for (int i = 0; i < L::kPanels * kWords; ++i) {
-                    const int base = (i / kWords) * L::kPanelDims + q4 * (L::kPanelDims / 4) + (i % kWords) * 8;
-                    const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(qp + base)) : make_uint4(0, 0, 0, 0);
-                    put(2 * i, __byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632));
-                    put(2 * i + 1, __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
-                }
             } else {
+                // this lane's quarter of the column: pairs (values 2i, 2i+1) in the order of its code words
+                constexpr int kRun = L::kPanelDims / 4;          // neighbouring values a lane has in a panel
+                uint32_t raw[D / 8];
 #pragma unroll
-                for (int ks = 0; ks < X::kKSteps; ++ks) {
-                    const int base = (ks / 4) * L::kPanelDims + q4 * 16 + (ks % 4) * 4;
-                    const uint2 x = live ? __ldg(reinterpret_cast<const uint2*>(qp + base)) : make_uint2(0, 0);
-                    put(ks, __byte_perm(x.x, x.y, 0x5410), __byte_perm(x.x, x.y, 0x7632));
+                for (int i = 0; i < D / 32; ++i) {
+                    const int at = (i * 8 / kRun) * L::kPanelDims + q4 * kRun + (i * 8) % kRun;
+                    const uint4 x = live ? __ldg(reinterpret_cast<const uint4*>(qp + at)) : make_uint4(0, 0, 0, 0);
+                    raw[4 * i] = x.x;
+                    raw[4 * i + 1] = x.y;
+                    raw[4 * i + 2] = x.z;
+                    raw[4 * i + 3] = x.w;
                 }
-            }
-            if (FMT != 16) {
+                float most = 0.f;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) most = fmaxf(most, fmaxf(fabsf(bf16lo(raw[i])), fabsf(bf16hi(raw[i]))));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                const uint32_t ex = min(max(__float_as_uint(most) >> 23, 1u), 253u);
+                const float up = __uint_as_float((254u - ex) << 23), down = __uint_as_float(ex << 23);   // powers of two: exact
+                float sum = 0.f, odd = 0.f;                      // of the rounded values; `odd`: of those that meet 1024 + 16 c
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    uint32_t b[4];
+                    float f[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        f[2 * k] = bf16lo(raw[4 * i + k]) * up;
+                        f[2 * k + 1] = bf16hi(raw[4 * i + k]) * up;
+                    }
+                    if (FMT == 4) {
+                        // a code word's registers 0..3 hold values (0, 4), (1, 5), (2, 6), (3, 7)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float by = k & 1 ? 0.0625f : 1.f;
+                            b[k] = pack_f16(f[k] * by, f[k + 4] * by);
+                            const float both = f16lo(b[k]) + f16hi(b[k]);
+                            if (k & 1) odd += both;
+                            else sum += both;
+                        }
+                        put(2 * i, b[0], b[1]);
+                        put(2 * i + 1, b[2], b[3]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            b[k] = pack_f16(f[2 * k], f[2 * k + 1]);
+                            odd += f16lo(b[k]) + f16hi(b[k]);
+                        }
+                        put(2 * i, b[0], b[1]);
+                        put(2 * i + 1, b[2], b[3]);
+                    }
+                }
+                sum = FMT == 4 ? fmaf(odd, 16.f, sum) : odd;
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                qsum[nt][0] = __shfl_sync(0xffffffffu, sum, (2 * q4) * 4) * p.scale_log2;
-                qsum[nt][1] = __shfl_sync(0xffffffffu, sum, (2 * q4 + 1) * 4) * p.scale_log2;
+                odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+                odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+                const float mul = down * p.scale_log2;
+                sum *= mul;
+                odd *= -kOddOffset;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {                    // from the column's own lanes to those that hold its scores
+                    const int from = (2 * q4 + e) * 4;
+                    qsum[nt][e] = __shfl_sync(0xffffffffu, sum, from);
+                    qmul[nt][e] = __shfl_sync(0xffffffffu, mul, from);
+                    qoff[nt][e] = __shfl_sync(0xffffffffu, odd, from);
+                }
             }
         }
         if (!X::kQReg) __syncthreads();
 
         float o[X::kMTiles][NT][4];
-        float m[NT][2], l[NT][2], z[NT][2];       // m: what is taken off the scores (0 while nothing was seen)
-        bool seen[NT][2];
+        float m[NT][2], l[NT][2], z[NT][2];
+        float base[NT][2], pass[NT][2];           // what is taken off the scores (m, 0 before the first); what moves the maximum
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 m[nt][e] = -INFINITY;
                 l[nt][e] = z[nt][e] = 0.f;
-                seen[nt][e] = false;
+                base[nt][e] = 0.f;
+                pass[nt][e] = -INFINITY;
             }
 #pragma unroll
             for (int mt = 0; mt < X::kMTiles; ++mt)
@@ -492,227 +631,248 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
 
         // ---------------------------------------------------------------------------- the warp's slices of this item
 #pragma unroll 1
-        for (int64_t s = sg.lo + warp; s < sg.hi; s += kWarps) {
-            const int2 nt_ = note[stage];
-            const int nv = nt_.x, pos0 = nt_.y;
+        for (int32_t s = sg.lo + warp * kU; s < sg.hi; s += kStep) {
             const uint32_t st_u = ring_u + stage * L::kStage;
-            if (nv > 0 && !dead) {
-                if (!mbar_wait(&full[stage], (phases >> stage) & 1u)) {
-                    if (p.err && lane == 0) atomicExch(p.err, 1);
-                    dead = true;
-                }
-                phases ^= 1u << stage;
+            if (!dead && !mbar_wait(&full[stage], parity)) {
+                if (p.err && lane == 0) atomicExch(p.err, 1);
+                dead = true;
             }
-            if (nv > 0 && !dead) {
+            int nv[kU], pos0[kU];
+            bool any = false, masked = false;
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const int2 n = note[stage * kU + u];
+                nv[u] = n.x;
+                pos0[u] = n.y;
+                any |= nv[u] > 0;
+                masked |= nv[u] < kRows || (p.ctx != nullptr && pos0[u] + kRows > limit_min);
+            }
+            if (any && !dead) {
                 // ---- S^T = K Q^T
-                float sc[NT][4];
+                float sc[kU][NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[nt][i] = 0.f;
-                auto qk = [&](int ks, const uint32_t (&a)[4]) {
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        if (X::kQReg) {
-                            mma(sc[nt], a, qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][0], qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][1]);
-                        } else {
-                            const uint2 b = q_frag[(ks * NT + nt) * 32 + lane];
-                            mma(sc[nt], a, b.x, b.y);
-                        }
-                    }
-                };
-                if (FMT == 16) {
-                    const uint32_t ka = st_u + (lane & 15) * L::kRowStride + (lane >> 4) * 16;
-#pragma unroll
-                    for (int ks = 0; ks < X::kKSteps; ++ks) {
-                        uint32_t a[4];
-                        ldsm4(a, ka + ks * 32);
-                        qk(ks, a);
-                    }
-                } else {
-                    constexpr int kChunk = L::kPanel / 4;        // bytes of a row in a panel that a lane reads
-#pragma unroll
-                    for (int pn = 0; pn < L::kPanels; ++pn) {
-                        const uint32_t ka = st_u + pn * (kRows * L::kPanel) + g * L::kPanel + q4 * kChunk;
-                        uint32_t x[4], y[4];                     // rows g and g + 8
-                        if (kChunk == 16) {
-                            const uint4 u = lds16(ka), w = lds16(ka + 8 * L::kPanel);
-                            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-                            y[0] = w.x; y[1] = w.y; y[2] = w.z; y[3] = w.w;
-                        } else {
-                            const uint2 u = lds8(ka), w = lds8(ka + 8 * L::kPanel);
-                            x[0] = u.x; x[1] = u.y;
-                            y[0] = w.x; y[1] = w.y;
-                        }
-#pragma unroll
-                        for (int i = 0; i < kChunk / 4; ++i) {
-                            if (FMT == 4) {
-#pragma unroll
-                                for (int half = 0; half < 2; ++half) {
-                                    const uint32_t a[4] = {nibbles(x[i], 2 * half), nibbles(y[i], 2 * half),
-                                                           nibbles(x[i], 2 * half + 1), nibbles(y[i], 2 * half + 1)};
-                                    qk((pn * (kChunk / 4) + i) * 2 + half, a);
-                                }
-                            } else {
-                                const uint32_t a[4] = {bytes(x[i], 0), bytes(y[i], 0), bytes(x[i], 1), bytes(y[i], 1)};
-                                qk(pn * (kChunk / 4) + i, a);
-                            }
-                        }
-                    }
-                }
-
-                // ---- scores in powers of two; rows g (values 0, 1) and g + 8 (values 2, 3)
-                float ks0 = p.scale_log2, ks1 = p.scale_log2, kz0 = 0.f, kz1 = 0.f, vs0 = 1.f, vs1 = 1.f, vz0 = 0.f, vz1 = 0.f;
-                if (FMT != 16) {
-                    const float mid = FMT == 4 ? 8.f : 128.f;
-                    const uint32_t pa = st_u + 2 * kRows * L::kRowBytes + g * 4;
-                    const uint32_t k0 = lds4(pa), k1 = lds4(pa + 32), v0 = lds4(pa + 64), v1 = lds4(pa + 96);
-                    kz0 = fmaf(bf16lo(k0), mid, bf16hi(k0));     // the centred codes' zero
-                    kz1 = fmaf(bf16lo(k1), mid, bf16hi(k1));
-                    ks0 = bf16lo(k0) * p.scale_log2;
-                    ks1 = bf16lo(k1) * p.scale_log2;
-                    vs0 = bf16lo(v0);
-                    vs1 = bf16lo(v1);
-                    vz0 = fmaf(vs0, mid, bf16hi(v0));
-                    vz1 = fmaf(vs1, mid, bf16hi(v1));
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (FMT == 16) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[nt][i] *= ks0;
-                    } else {
-                        sc[nt][0] = fmaf(sc[nt][0], ks0, kz0 * qsum[nt][0]);
-                        sc[nt][1] = fmaf(sc[nt][1], ks0, kz0 * qsum[nt][1]);
-                        sc[nt][2] = fmaf(sc[nt][2], ks1, kz1 * qsum[nt][0]);
-                        sc[nt][3] = fmaf(sc[nt][3], ks1, kz1 * qsum[nt][1]);
-                    }
-                }
-                const bool masked = nv < kRows || (p.ctx != nullptr && pos0 + kRows > limit_min);
-                uint32_t hide = 0;                               // bit 4 nt + i: value i of tile nt is not seen
-                if (masked) {
+                for (int u = 0; u < kU; ++u) {
+                    const uint32_t un_u = st_u + u * L::kUnit;
+                    float s2[NT][4];                             // every other product: half the chain of dependent sums
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int row = g + (i >> 1) * 8;
-                            if (row >= nv || pos0 + row >= limit[nt][i & 1]) {
-                                sc[nt][i] = -INFINITY;
-                                hide |= 1u << (4 * nt + i);
+                            sc[u][nt][i] = FMT == 16 ? 0.f : qoff[nt][i & 1];
+                            s2[nt][i] = 0.f;
+                        }
+                    auto qk = [&](int ks, const uint32_t (&a)[4]) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            uint32_t b0, b1;
+                            if (X::kQReg) {
+                                b0 = qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][0];
+                                b1 = qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][1];
+                            } else {
+                                const uint2 b = q_frag[(ks * NT + nt) * 32 + lane];
+                                b0 = b.x;
+                                b1 = b.y;
+                            }
+                            float (&to)[4] = NT == 1 && (ks & 1) ? s2[nt] : sc[u][nt];
+                            if (FMT == 16) mma(to, a, b0, b1);
+                            else mma_f16(to, a, b0, b1);
+                        }
+                    };
+                    if (FMT == 16) {
+                        const uint32_t ka = un_u + (lane & 15) * 128;
+#pragma unroll
+                        for (int ks = 0; ks < X::kKSteps; ++ks) {
+                            uint32_t a[4];
+                            ldsm4(a, ka + (ks / 4) * L::kBf16Panel + ((((ks % 4) * 2 + (lane >> 4)) ^ (lane & 7)) << 4));
+                            qk(ks, a);
+                        }
+                    } else {
+                        constexpr int kChunk = L::kPanel / 4;    // bytes of a row in a panel that a lane reads
+#pragma unroll
+                        for (int pn = 0; pn < L::kPanels; ++pn) {
+                            const uint32_t ka = un_u + pn * (kRows * L::kPanel) + lane * kChunk;
+                            uint32_t x[4], y[4];                 // rows g and g + 8
+                            lds_words<kChunk>(x, ka);
+                            lds_words<kChunk>(y, ka + 8 * L::kPanel);
+#pragma unroll
+                            for (int i = 0; i < kChunk / 4; ++i) {
+                                if (FMT == 4) {
+#pragma unroll
+                                    for (int half = 0; half < 2; ++half) {
+                                        const uint32_t a[4] = {k_nibbles(x[i], 2 * half), k_nibbles(y[i], 2 * half),
+                                                               k_nibbles(x[i], 2 * half + 1), k_nibbles(y[i], 2 * half + 1)};
+                                        qk((pn * (kChunk / 4) + i) * 2 + half, a);
+                                    }
+                                } else {
+                                    const uint32_t a[4] = {k_bytes(x[i], 0), k_bytes(y[i], 0), k_bytes(x[i], 1), k_bytes(y[i], 1)};
+                                    qk(pn * (kChunk / 4) + i, a);
+                                }
                             }
                         }
+                    }
+                    if (NT == 1) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[u][0][i] += s2[0][i];
+                    }
+                }
+
+                // ---- scores in powers of two; rows g (values 0, 1) and g + 8 (values 2, 3)
+                float vs[kU][2], vz[kU][2];
+#pragma unroll
+                for (int u = 0; u < kU; ++u) {
+                    if (FMT == 16) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) sc[u][nt][i] *= p.scale_log2;
+                    } else {
+                        constexpr float mid = FMT == 4 ? 8.f : 128.f;
+                        const uint32_t pa = st_u + u * L::kUnit + 2 * kRows * L::kRowBytes + g * 4;
+#pragma unroll
+                        for (int row = 0; row < 2; ++row) {
+                            const uint32_t k0 = lds4(pa + row * 32), v0 = lds4(pa + 64 + row * 32);
+                            const float kz = fmaf(bf16lo(k0), mid, bf16hi(k0));      // the centred codes' zero
+                            const float ksc = bf16lo(k0);
+                            vs[u][row] = bf16lo(v0);
+                            vz[u][row] = fmaf(vs[u][row], mid, bf16hi(v0));
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    sc[u][nt][2 * row + e] = fmaf(sc[u][nt][2 * row + e], ksc * qmul[nt][e], kz * qsum[nt][e]);
+                        }
+                    }
+                }
+                uint32_t hide[kU];                               // bit 4 nt + i: value i of tile nt is not seen
+#pragma unroll
+                for (int u = 0; u < kU; ++u) hide[u] = 0;
+                if (masked) {
+#pragma unroll
+                    for (int u = 0; u < kU; ++u)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int row = g + (i >> 1) * 8;
+                                if (row >= nv[u] || pos0[u] + row >= limit[nt][i & 1]) {
+                                    sc[u][nt][i] = -INFINITY;
+                                    hide[u] |= 1u << (4 * nt + i);
+                                }
+                            }
                 }
                 // ---- running maximum: moved only when it is passed by more than the slack
                 bool passed = false;
+                float top[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        passed |= fmaxf(sc[nt][e], sc[nt][e + 2]) > (seen[nt][e] ? m[nt][e] + kMaxSlack : -INFINITY);
+                    for (int e = 0; e < 2; ++e) {
+                        top[nt][e] = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
+                        if (kU == 2) top[nt][e] = fmaxf(top[nt][e], fmaxf(sc[kU - 1][nt][e], sc[kU - 1][nt][e + 2]));
+                        passed |= top[nt][e] > pass[nt][e];
+                    }
                 if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float x = fmaxf(sc[nt][e], sc[nt][e + 2]);
+                            float x = top[nt][e];
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                             const float now = fmaxf(m[nt][e], x);
+                            // (before the first score nothing but zeros and NaN can have been added: both stay)
+                            const float f = m[nt][e] > -INFINITY ? exp2_fast(m[nt][e] - now) : 1.f;
                             if (now > -INFINITY) {
-                                const float f = seen[nt][e] ? exp2_fast(m[nt][e] - now) : 0.f;
-                                // (nothing but zeros and NaN can have been added before the first score)
-                                if (seen[nt][e]) {
-                                    l[nt][e] *= f;
-                                    z[nt][e] *= f;
+                                m[nt][e] = base[nt][e] = now;
+                                pass[nt][e] = now + kMaxSlack;
+                            }
+                            l[nt][e] *= f;
+                            z[nt][e] *= f;
 #pragma unroll
-                                    for (int mt = 0; mt < X::kMTiles; ++mt) {
-                                        o[mt][nt][e] *= f;
-                                        o[mt][nt][e + 2] *= f;
-                                    }
-                                }
-                                m[nt][e] = now;
-                                seen[nt][e] = true;
+                            for (int mt = 0; mt < X::kMTiles; ++mt) {
+                                o[mt][nt][e] *= f;
+                                o[mt][nt][e + 2] *= f;
                             }
                         }
                 }
                 // ---- weights, and their bf16 halves with tokens along the columns' other side
-                uint32_t ph[NT][2], pl[NT][2];
-                float wt[NT][4];
+                uint32_t ph[kU][NT][2], pl[kU][NT][2];
+                float wt[kU][NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float (&w)[4] = wt[nt];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float off = seen[nt][i & 1] ? m[nt][i & 1] : 0.f;
-                        w[i] = exp2_fast(sc[nt][i] - off);
-                    }
-                    l[nt][0] += w[0] + w[2];
-                    l[nt][1] += w[1] + w[3];
-                    if (FMT != 16) {
-                        if (masked) {                            // what stands in rows that are not seen may be anything
-                            const uint32_t hd = hide >> (4 * nt);
-                            z[nt][0] += ((hd & 1u) ? 0.f : w[0] * vz0) + ((hd & 4u) ? 0.f : w[2] * vz1);
-                            z[nt][1] += ((hd & 2u) ? 0.f : w[1] * vz0) + ((hd & 8u) ? 0.f : w[3] * vz1);
-                            w[0] = (hd & 1u) ? 0.f : w[0] * vs0;
-                            w[1] = (hd & 2u) ? 0.f : w[1] * vs0;
-                            w[2] = (hd & 4u) ? 0.f : w[2] * vs1;
-                            w[3] = (hd & 8u) ? 0.f : w[3] * vs1;
-                        } else {
-                            z[nt][0] = fmaf(w[0], vz0, fmaf(w[2], vz1, z[nt][0]));
-                            z[nt][1] = fmaf(w[1], vz0, fmaf(w[3], vz1, z[nt][1]));
-                            w[0] *= vs0;
-                            w[1] *= vs0;
-                            w[2] *= vs1;
-                            w[3] *= vs1;
-                        }
-                    }
-                    uint32_t a = pack_bf16(w[0], w[1]), b = pack_bf16(w[2], w[3]);
-                    const uint32_t al = pack_bf16(w[0] - bf16lo(a), w[1] - bf16hi(a));
-                    const uint32_t bl = pack_bf16(w[2] - bf16lo(b), w[3] - bf16hi(b));
-                    if (DUP) {
-                        ph[nt][0] = transpose8(q4 < 2 ? a : al);
-                        ph[nt][1] = transpose8(q4 < 2 ? b : bl);
-                    } else {
-                        ph[nt][0] = transpose8(a);
-                        ph[nt][1] = transpose8(b);
-                        pl[nt][0] = transpose8(al);
-                        pl[nt][1] = transpose8(bl);
-                    }
-                }
-                // ---- O^T += V^T P^T
-                auto pv = [&](int mt, const uint32_t (&a)[4]) {
+                for (int u = 0; u < kU; ++u)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma(o[mt][nt], a, ph[nt][0], ph[nt][1]);
-                        if (!DUP) mma(o[mt][nt], a, pl[nt][0], pl[nt][1]);
+                        float (&w)[4] = wt[u][nt];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = exp2_fast(sc[u][nt][i] - base[nt][i & 1]);
+                        l[nt][0] += w[0] + w[2];
+                        l[nt][1] += w[1] + w[3];
+                        if (FMT != 16) {
+                            if (masked) {                        // what stands in rows that are not seen may be anything
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const bool hd = (hide[u] >> (4 * nt + i)) & 1u;
+                                    z[nt][i & 1] += hd ? 0.f : w[i] * vz[u][i >> 1];
+                                    w[i] = hd ? 0.f : w[i] * vs[u][i >> 1];
+                                }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    z[nt][i & 1] = fmaf(w[i], vz[u][i >> 1], z[nt][i & 1]);
+                                    w[i] *= vs[u][i >> 1];
+                                }
+                            }
+                        }
+                        const uint32_t a = pack_bf16(w[0], w[1]), b = pack_bf16(w[2], w[3]);
+                        const uint32_t al = pack_bf16(w[0] - bf16lo(a), w[1] - bf16hi(a));
+                        const uint32_t bl = pack_bf16(w[2] - bf16lo(b), w[3] - bf16hi(b));
+                        if (DUP) {
+                            ph[u][nt][0] = transpose8(q4 < 2 ? a : al);
+                            ph[u][nt][1] = transpose8(q4 < 2 ? b : bl);
+                        } else {
+                            ph[u][nt][0] = transpose8(a);
+                            ph[u][nt][1] = transpose8(b);
+                            pl[u][nt][0] = transpose8(al);
+                            pl[u][nt][1] = transpose8(bl);
+                        }
                     }
-                };
                 // A row that some columns see and others do not may hold an infinity or a NaN, and a weight of zero would not
                 // keep it out of the product: such a slice (the last tokens of a request with several queries) is added up
                 // column by column instead.
                 bool wild = false;
-                if (FMT == 16 && masked && pos0 + nv > limit_min) {
-                    for (int i = lane; i < nv * (D / 8); i += 32) {
-                        const uint4 x = lds16(st_u + (kRows + i / (D / 8)) * L::kRowStride + (i % (D / 8)) * 16);
-                        const uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            wild |= (y[k] & 0x7f80u) == 0x7f80u || (y[k] & 0x7f800000u) == 0x7f800000u;
+                if (FMT == 16 && masked) {
+                    unsigned char* const v_rows = ring + stage * L::kStage + (D / 64) * L::kBf16Panel;
+                    // rows without a seen token: a weight of zero must meet a number
+                    for (int i = lane; i < (kRows - nv[0]) * (D / 8); i += 32) {
+                        const int row = nv[0] + i / (D / 8), x = i % (D / 8);
+                        *reinterpret_cast<uint4*>(v_rows + (x / 8) * L::kBf16Panel + row * 128 + (x % 8) * 16) = make_uint4(0, 0, 0, 0);
                     }
-                    wild = __any_sync(0xffffffffu, wild);
+                    fence_proxy_async();                         // (the next load into the stage comes behind these stores)
+                    if (pos0[0] + nv[0] > limit_min) {
+                        for (int i = lane; i < nv[0] * (D / 8); i += 32) {
+                            const int row = i / (D / 8), x = i % (D / 8);
+                            const uint4 q = *reinterpret_cast<const uint4*>(v_rows + (x / 8) * L::kBf16Panel + row * 128 + (x % 8) * 16);
+                            const uint32_t y[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                wild |= (y[k] & 0x7f80u) == 0x7f80u || (y[k] & 0x7f800000u) == 0x7f800000u;
+                        }
+                        wild = __any_sync(0xffffffffu, wild);
+                    }
+                    __syncwarp();
                 }
                 if (FMT == 16 && wild) {
 #pragma unroll 1
-                    for (int row = 0; row < nv; ++row) {
+                    for (int row = 0; row < nv[0]; ++row) {
                         const int src = (row & 7) * 4 + q4;
-                        const uint32_t hd = __shfl_sync(0xffffffffu, hide, src);
+                        const uint32_t hd = __shfl_sync(0xffffffffu, hide[0], src);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                const float w0 = __shfl_sync(0xffffffffu, wt[nt][e], src);
-                                const float w1 = __shfl_sync(0xffffffffu, wt[nt][e + 2], src);
+                                const float w0 = __shfl_sync(0xffffffffu, wt[0][nt][e], src);
+                                const float w1 = __shfl_sync(0xffffffffu, wt[0][nt][e + 2], src);
                                 const int bit = 4 * nt + e + (row >> 3) * 2;
                                 if (((hd >> bit) & 1u) || (DUP && q4 >= 2)) continue;
                                 const float w = row < 8 ? w0 : w1;
@@ -720,48 +880,57 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                                 for (int mt = 0; mt < X::kMTiles; ++mt)
 #pragma unroll
                                     for (int k = 0; k < 2; ++k) {
+                                        const int x = mt * 2 + k;        // the 16-byte piece of value mt * 16 + k * 8 + g
                                         const uint16_t b = *reinterpret_cast<const uint16_t*>(
-                                            ring + stage * L::kStage + (kRows + row) * L::kRowStride + (mt * 16 + g + k * 8) * 2);
+                                            ring + stage * L::kStage + (D / 64 + x / 8) * L::kBf16Panel + row * 128 +
+                                            (((x % 8) ^ (row & 7)) << 4) + g * 2);
                                         o[mt][nt][e + 2 * k] += w * __uint_as_float((uint32_t)b << 16);
                                     }
                             }
                     }
-                } else if (FMT == 16) {
-                    const uint32_t va = st_u + kRows * L::kRowStride + ((lane & 7) + ((lane >> 4) & 1) * 8) * L::kRowStride +
-                                        ((lane >> 3) & 1) * 16;
+                }
+                // ---- O^T += V^T P^T
 #pragma unroll
-                    for (int mt = 0; mt < X::kMTiles; ++mt) {
-                        uint32_t a[4];
-                        ldsm4_trans(a, va + mt * 32);
-                        pv(mt, a);
-                    }
-                } else {
-                    constexpr int kChunk = L::kPanel / 4;        // bytes of a lane in half a panel: 2 tokens, 1/8 of the values
+                for (int u = 0; u < kU; ++u) {
+                    const uint32_t un_u = st_u + u * L::kUnit;
+                    auto pv = [&](int mt, const uint32_t (&a)[4]) {
 #pragma unroll
-                    for (int pn = 0; pn < L::kPanels; ++pn) {
-                        const uint32_t va = st_u + kRows * L::kRowBytes + pn * (kRows * L::kPanel) + lane * kChunk;
-                        uint32_t x[4], y[4];                     // tokens 2 q4, 2 q4 + 1 and the two 8 behind them
-                        if (kChunk == 16) {
-                            const uint4 u = lds16(va), w = lds16(va + 8 * L::kPanel);
-                            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-                            y[0] = w.x; y[1] = w.y; y[2] = w.z; y[3] = w.w;
-                        } else {
-                            const uint2 u = lds8(va), w = lds8(va + 8 * L::kPanel);
-                            x[0] = u.x; x[1] = u.y;
-                            y[0] = w.x; y[1] = w.y;
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma(o[mt][nt], a, ph[u][nt][0], ph[u][nt][1]);
+                            if (!DUP) mma(o[mt][nt], a, pl[u][nt][0], pl[u][nt][1]);
                         }
+                    };
+                    if (FMT == 16) {
+                        if (!wild) {
+                            const uint32_t va = un_u + (D / 64) * L::kBf16Panel + ((lane & 7) + ((lane >> 4) & 1) * 8) * 128;
 #pragma unroll
-                        for (int i = 0; i < kChunk / 4; ++i) {
-                            if (FMT == 4) {
+                            for (int mt = 0; mt < X::kMTiles; ++mt) {
+                                uint32_t a[4];
+                                ldsm4_trans(a, va + (mt / 4) * L::kBf16Panel + ((((mt % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+                                pv(mt, a);
+                            }
+                        }
+                    } else {
+                        constexpr int kChunk = L::kPanel / 4;    // bytes of a lane in half a panel: 2 tokens, 1/8 of the values
 #pragma unroll
-                                for (int half = 0; half < 2; ++half) {
-                                    const uint32_t a[4] = {nibbles(x[i], 2 * half), nibbles(x[i], 2 * half + 1),
-                                                           nibbles(y[i], 2 * half), nibbles(y[i], 2 * half + 1)};
-                                    pv(pn * (L::kPanelDims / 16) + i * 2 + half, a);
+                        for (int pn = 0; pn < L::kPanels; ++pn) {
+                            const uint32_t va = un_u + kRows * L::kRowBytes + pn * (kRows * L::kPanel) + lane * kChunk;
+                            uint32_t x[4], y[4];                 // tokens 2 q4, 2 q4 + 1 and the two 8 behind them
+                            lds_words<kChunk>(x, va);
+                            lds_words<kChunk>(y, va + 8 * L::kPanel);
+#pragma unroll
+                            for (int i = 0; i < kChunk / 4; ++i) {
+                                if (FMT == 4) {
+#pragma unroll
+                                    for (int half = 0; half < 2; ++half) {
+                                        const uint32_t a[4] = {v_nibbles(x[i], 2 * half), v_nibbles(x[i], 2 * half + 1),
+                                                               v_nibbles(y[i], 2 * half), v_nibbles(y[i], 2 * half + 1)};
+                                        pv(pn * (L::kPanelDims / 16) + i * 2 + half, a);
+                                    }
+                                } else {
+                                    const uint32_t a[4] = {v_bytes(x[i], 0), v_bytes(x[i], 1), v_bytes(y[i], 0), v_bytes(y[i], 1)};
+                                    pv(pn * (L::kPanelDims / 16) + i, a);
                                 }
-                            } else {
-                                const uint32_t a[4] = {bytes(x[i], 0), bytes(x[i], 1), bytes(y[i], 0), bytes(y[i], 1)};
-                                pv(pn * (L::kPanelDims / 16) + i, a);
                             }
                         }
                     }
@@ -770,7 +939,10 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             __syncwarp();                                        // every lane is done with the stage
             if (!dead) issue(stage);
             __syncwarp();
-            stage = stage + 1 == L::kStages ? 0 : stage + 1;
+            if (++stage == X::kStages) {
+                stage = 0;
+                parity ^= 1u;
+            }
         }
 
         // ---------------------------------------------------------------------------------- join the four warps
@@ -850,9 +1022,10 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         __syncthreads();
     }
     // a wait that ran out leaves copies behind: give them one more bounded wait before the block's memory is reused
-    if (dead)
-        for (int s = 0; s < L::kStages; ++s)
-            if (note[s].x > 0) mbar_wait(&full[s], (phases >> s) & 1u);
+    if (dead) {
+        for (int s = stage; s < X::kStages; ++s) mbar_wait(&full[s], parity);
+        for (int s = 0; s < stage; ++s) mbar_wait(&full[s], parity ^ 1u);
+    }
 }
 
 // Joins the partial results of the item that crosses the cut between thread blocks blockIdx.x and blockIdx.x + 1 (the
@@ -867,15 +1040,14 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const 
     __shared__ float buf[kJoinWarps][kC][D];
     early_start_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t all = entries_total(p) * slices_per_entry(p);
+    const int32_t all = entries_total(p) * slices_per_entry(p);
+    const int32_t size = part_size(all, n_parts);
     const int b = blockIdx.x;
-    const int64_t at = cut(all, b + 1, n_parts);
-    if (at <= 0 || at >= all) return;
+    const int32_t at = (b + 1) * size;
+    if (at >= all) return;
     const Seg s = segment_at(p, at, all);
-    if (s.begin == at || s.begin < cut(all, b, n_parts)) return;     // nothing crosses here, or an earlier cut does it
-    if (cut(all, b, n_parts) == at) return;                          // an empty range: the cut was an earlier one
-    int last = b + 1;
-    while (last + 1 < n_parts && cut(all, last + 1, n_parts) < s.end) ++last;
+    if (s.begin == at || s.begin < at - size) return;     // nothing crosses here, or an earlier cut does it
+    const int last = (s.end - 1) / size;
     int q0, nq;
     queries_of(p, s.r, q0, nq);
     const int y0 = blockIdx.y * 8;
@@ -890,7 +1062,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const 
     for (int c = 0; c < kC; ++c) {
         float x = -INFINITY;
         for (int i = lane; i < n; i += 32)
-            if (cut(all, b + i, n_parts) < cut(all, b + i + 1, n_parts)) x = fmaxf(x, part_of(i)[y0 + c]);
+            x = fmaxf(x, part_of(i)[y0 + c]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
         top[c] = x;
@@ -900,7 +1072,6 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const 
     }
     if (warp < kJoinWarps)
         for (int i = warp; i < n; i += kJoinWarps) {
-            if (cut(all, b + i, n_parts) == cut(all, b + i + 1, n_parts)) continue;
             const float* const part = part_of(i);
 #pragma unroll
             for (int c = 0; c < kC; ++c) {
@@ -956,7 +1127,7 @@ inline int tile_cols(int cols, int head_dim)
     return 32;
 }
 
-// what a launch needs for one shape
+// what a launch needs for one shape (asked for without maps: nothing is launched)
 struct Plan {
     int32_t ctas;                      // thread blocks resident on the device at once
     int32_t part;                      // floats of a partial result
@@ -964,21 +1135,21 @@ struct Plan {
 };
 
 template <int FMT, int D, int NT, bool DUP>
-int32_t run(const Params& p, bool launch, Plan* plan, cudaStream_t st)
+int32_t run(const Params& p, const Maps* maps, Plan* plan, cudaStream_t st)
 {
     using X = Traits<FMT, D, NT, DUP>;
     plan->ctas = sm_count() * X::kOcc;
     plan->part = X::kPart;
     plan->cols = X::kCols;
-    if (!launch) return UCMX_OK;
+    if (!maps) return UCMX_OK;
     auto kern = attend_kernel<FMT, D, NT, DUP>;
     UCMX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, X::kSmem));
-    const int64_t all = (int64_t)p.total * p.spe * p.H * p.col_tiles;
+    const int64_t all = (int64_t)p.total * p.spe * p.H * p.col_tiles;      // (attend_common has bounded it)
     // at least one slice per warp: below that more blocks only add partial results
     int64_t grid = (all + kWarps - 1) / kWarps;
     if (grid > plan->ctas) grid = plan->ctas;
     if (grid < 1) grid = 1;
-    kern<<<(unsigned)grid, kThreads, X::kSmem, st>>>(p);
+    kern<<<(unsigned)grid, kThreads, X::kSmem, st>>>(p, *maps);
     UCMX_LAUNCH_CHECK("attend_kernel");
     if (grid == 1) return UCMX_OK;
     cudaLaunchConfig_t cfg = {};
@@ -996,33 +1167,33 @@ int32_t run(const Params& p, bool launch, Plan* plan, cudaStream_t st)
 }
 
 template <int FMT, int D>
-int32_t run_cols(const Params& p, int cols, bool launch, Plan* plan, cudaStream_t st)
+int32_t run_cols(const Params& p, int cols, const Maps* maps, Plan* plan, cudaStream_t st)
 {
     switch (tile_cols(cols, D)) {
-        case 4: return run<FMT, D, 1, true>(p, launch, plan, st);
-        case 8: return run<FMT, D, 1, false>(p, launch, plan, st);
-        case 16: return run<FMT, D, 2, false>(p, launch, plan, st);
+        case 4: return run<FMT, D, 1, true>(p, maps, plan, st);
+        case 8: return run<FMT, D, 1, false>(p, maps, plan, st);
+        case 16: return run<FMT, D, 2, false>(p, maps, plan, st);
         default:
-            if constexpr (D != 256) return run<FMT, D, 4, false>(p, launch, plan, st);
+            if constexpr (D != 256) return run<FMT, D, 4, false>(p, maps, plan, st);
             return UCMX_EUNSUPPORTED;
     }
 }
 
 template <int FMT>
-int32_t run_format(const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st)
+int32_t run_format(const Params& p, int head_dim, int cols, const Maps* maps, Plan* plan, cudaStream_t st)
 {
     switch (head_dim) {
-        case 64: return run_cols<FMT, 64>(p, cols, launch, plan, st);
-        case 128: return run_cols<FMT, 128>(p, cols, launch, plan, st);
-        case 256: return run_cols<FMT, 256>(p, cols, launch, plan, st);
+        case 64: return run_cols<FMT, 64>(p, cols, maps, plan, st);
+        case 128: return run_cols<FMT, 128>(p, cols, maps, plan, st);
+        case 256: return run_cols<FMT, 256>(p, cols, maps, plan, st);
         default: return UCMX_EUNSUPPORTED;
     }
 }
 
 // the three formats live in files of their own
-int32_t run_bf16(const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st);
-int32_t run_q8(const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st);
-int32_t run_q4(const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st);
+int32_t run_bf16(const Params& p, int head_dim, int cols, const Maps* maps, Plan* plan, cudaStream_t st);
+int32_t run_q8(const Params& p, int head_dim, int cols, const Maps* maps, Plan* plan, cudaStream_t st);
+int32_t run_q4(const Params& p, int head_dim, int cols, const Maps* maps, Plan* plan, cudaStream_t st);
 
 }  // namespace attend
 }  // namespace ucmx

@@ -3,9 +3,9 @@
 
 namespace ucmx {
 namespace attend {
-int32_t run_q8(const Params& p, int head_dim, int cols, bool launch, Plan* plan, cudaStream_t st)
+int32_t run_q8(const Params& p, int head_dim, int cols, const Maps* maps, Plan* plan, cudaStream_t st)
 {
-    return run_format<8>(p, head_dim, cols, launch, plan, st);
+    return run_format<8>(p, head_dim, cols, maps, plan, st);
 }
 }  // namespace attend
 }  // namespace ucmx

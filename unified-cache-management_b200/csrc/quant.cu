@@ -8,10 +8,10 @@
 // V's layout puts the codes of tokens 2i and 2i+1 side by side in pairs of bytes: neighbouring rows of the warp exchange words, so
 // that V moves in 32-bit words like K (a token whose partner is not in the call stores 16-bit pieces).
 //
-// Arithmetic.  The differences are taken of halves (exact, and no overflow for any finite row).  A reciprocal and one residual
-// give the quotient's nearest integer: the residual x - code*scale is exact in fp32, so a step in the wrong direction shows and
-// is taken back; a tie, where the rounding of x - zero might have decided, is settled in fp64.  (A division per value was the
-// bound of this kernel.)
+// Arithmetic.  The range comes from packed bf16 maxima (of x and of -x; NaN wins).  Differences are taken of halves: exact, and no
+// overflow for any finite row.  A reciprocal, a rounding to the integers by adding 2^23, and the residual x - code*scale, which is
+// exact in fp32: where it is half a step or more (ties, and quotients the reciprocal put on the wrong side) the code is settled in
+// fp64.  A division per value was the bound of this kernel.
 #include "common.cuh"
 
 namespace ucmx {
@@ -45,9 +45,12 @@ struct QuantParams {
     const int32_t* out_slots;
     int32_t T, H;
     int64_t n;                         // tokens or blocks
-    int64_t units;                     // warp-sized pieces of work
+    uint32_t items;                    // pieces of work, one per warp
+    uint32_t head_chunks;              // pieces that the heads are cut into
     int32_t* err;
 };
+
+constexpr float kMagic = 8388608.f;    // 2^23: floats of this size count in ones
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi)
 {
@@ -55,17 +58,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-
-// nearest integer to (x - zero) / scale, ties to even; inv = 1 / (scale / 2)
-__device__ __forceinline__ int code_of(float x, float half_zero, float half_scale, float inv, float zero, float scale)
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b)
 {
-    const float hx = fmaf(x, 0.5f, -half_zero);
-    float c = rintf(hx * inv);
-    const float e = fmaf(-c, half_scale, hx);
-    const float off = fabsf(e), half = 0.5f * half_scale;
-    if (off > half) c += e > 0.f ? 1.f : -1.f;
-    if (off == half) c = (float)rint(((double)x - (double)zero) / (double)scale);
-    return (int)c;
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b)
+{
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 
 // byte offset of a lane's codes inside K's part of a group / of unit u (2 bytes of a row) inside V's part
@@ -86,108 +89,142 @@ __device__ __forceinline__ int v_at(int t, int u)
            (b % kChunk) / 2 * 4 + (t & 1) * 2;
 }
 
-// Unit -> (token group, K or V, head); heads are innermost, neighbouring warps read neighbouring rows of the same tokens.
-struct Unit {
-    int64_t tg;
+// Piece of work -> (token group, K or V, first head); heads are innermost, neighbouring warps read neighbouring rows.
+struct Piece {
+    uint32_t tg;
     int32_t kv, h;
 };
-__device__ __forceinline__ Unit unit_of(int64_t u, int H)
+template <int HC>
+__device__ __forceinline__ Piece piece_of(uint32_t item, uint32_t head_chunks)
 {
-    Unit x;
-    const int64_t a = u / H;
-    x.h = (int32_t)(u - a * H);
+    Piece x;
+    const uint32_t a = item / head_chunks;
+    x.h = (int32_t)(item - a * head_chunks) * HC;
     x.kv = (int32_t)(a & 1);
     x.tg = a >> 1;
     return x;
 }
 
-template <int BITS, int D, bool BLOCKS>
+// HC heads of one token group per warp, their loads all in flight at once.
+template <int BITS, int D, bool BLOCKS, int HC>
 __global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
 {
     using X = Q<BITS, D>;
     const int lane = threadIdx.x & 31, lr = lane % X::kLanes, row = lane / X::kLanes;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    const int per_block = (p.T + X::kTokens - 1) / X::kTokens;
-    for (int64_t un = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); un < p.units; un += step) {
-        const Unit x = unit_of(un, p.H);
-        // ---- where the row comes from and where it goes
-        const uint16_t* src = x.kv ? p.v : p.k;
-        int64_t block = -1;
-        int t = 0;
-        if (BLOCKS) {
-            const int64_t i = x.tg / per_block;
-            t = (int)(x.tg - i * per_block) * X::kTokens + row;
-            const int id = checked_block_id(p.ids, i, p.n_src, lr == 0 && row == 0 ? p.err : nullptr);
-            const int64_t out = checked_out_row(p.out_slots, i, p.n_blocks, lr == 0 && row == 0 ? p.err : nullptr);
-            if (id >= 0 && out >= 0) block = out;
-            src += (int64_t)(id < 0 ? 0 : id) * (x.kv ? p.v_block : p.k_block) + (int64_t)t * (x.kv ? p.v_token : p.k_token);
-        } else {
-            const int64_t i = x.tg * X::kTokens + row;
-            int64_t slot = i < p.n ? __ldg(p.slots + i) : -1;
-            if (slot >= p.n_blocks * p.T) {
-                if (p.err && lr == 0) atomicExch(p.err, 3);
-                slot = -1;
-            }
-            if (slot >= 0) {
-                block = slot / p.T;
-                t = (int)(slot - block * p.T);
-            }
-            src += i * (x.kv ? p.v_token : p.k_token);
+    const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (item >= p.items) return;
+    const Piece x = piece_of<HC>(item, p.head_chunks);
+    // ---- where the rows come from and where they go
+    const uint16_t* src = x.kv ? p.v : p.k;
+    int64_t block = -1;
+    int t = 0;
+    if (BLOCKS) {
+        const uint32_t per_block = (uint32_t)p.T / X::kTokens;
+        const uint32_t i = x.tg / per_block;
+        t = (int)(x.tg - i * per_block) * X::kTokens + row;
+        const int id = checked_block_id(p.ids, i, p.n_src, lane == 0 ? p.err : nullptr);
+        const int64_t out = checked_out_row(p.out_slots, i, p.n_blocks, lane == 0 ? p.err : nullptr);
+        if (id < 0 || out < 0) return;                   // (the same for the whole warp)
+        block = out;
+        src += (int64_t)id * (x.kv ? p.v_block : p.k_block) + (int64_t)t * (x.kv ? p.v_token : p.k_token);
+    } else {
+        const int64_t i = (int64_t)x.tg * X::kTokens + row;
+        int64_t slot = i < p.n ? __ldg(p.slots + i) : -1;
+        if (slot >= p.n_blocks * p.T) {
+            if (p.err && lr == 0) atomicExch(p.err, 3);
+            slot = -1;
         }
-        src += (int64_t)x.h * D + lr * X::kDims;
-        const bool live = block >= 0;
-        uint4 raw[X::kDims / 8];
+        if (slot >= 0) {
+            block = slot < (1ll << 32) ? (int64_t)((uint32_t)slot / (uint32_t)p.T) : slot / p.T;
+            t = (int)(slot - block * p.T);
+        }
+        src += i * (x.kv ? p.v_token : p.k_token);
+    }
+    const bool live = block >= 0;
+    src += (int64_t)x.h * D + lr * X::kDims;
+    uint4 raw[HC][X::kDims / 8];
 #pragma unroll
-        for (int i = 0; i < X::kDims / 8; ++i) raw[i] = live ? ld_stream16(src + i * 8) : make_uint4(0, 0, 0, 0);
-        float f[X::kDims];
+    for (int c = 0; c < HC; ++c)
+#pragma unroll
+        for (int i = 0; i < X::kDims / 8; ++i)
+            raw[c][i] = live && x.h + c < p.H ? ld_stream16(src + c * D + i * 8) : make_uint4(0, 0, 0, 0);
+    // is the neighbouring row the other token of a pair?
+    const int64_t place = live ? block * p.T + t : -2 - row;
+    const int64_t other = __shfl_xor_sync(0xffffffffu, place, X::kLanes);
+    const bool paired = live && other == (place ^ 1) && (place & 1) == (row & 1);
+    const int tt = t % kRows;
+    const int group_step = (p.T / kRows) * X::kGroup;
+    uint8_t* group = p.cache + block * p.block_stride + (int64_t)x.h * group_step + (t / kRows) * X::kGroup;
+#pragma unroll
+    for (int c = 0; c < HC; ++c, group += group_step) {
+        if (x.h + c >= p.H) break;
+        uint32_t q[X::kDims / 2];
 #pragma unroll
         for (int i = 0; i < X::kDims / 8; ++i) {
-            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[i * 8 + 2 * j] = bf16lo(w[j]);
-                f[i * 8 + 2 * j + 1] = bf16hi(w[j]);
-            }
+            q[4 * i] = raw[c][i].x;
+            q[4 * i + 1] = raw[c][i].y;
+            q[4 * i + 2] = raw[c][i].z;
+            q[4 * i + 3] = raw[c][i].w;
         }
-        // ---- the row's range; x - x is 0 for a number and NaN for anything else
-        float lo = f[0], hi = f[0], odd = 0.f;
+        // ---- the row's range: (max x, max -x) in one register
+        uint32_t hi2 = q[0], lo2 = q[0];
 #pragma unroll
-        for (int i = 0; i < X::kDims; ++i) {
-            lo = fminf(lo, f[i]);
-            hi = fmaxf(hi, f[i]);
-            odd += f[i] - f[i];
+        for (int i = 1; i < X::kDims / 2; ++i) {
+            hi2 = max2(hi2, q[i]);
+            lo2 = min2(lo2, q[i]);
         }
+        lo2 ^= 0x80008000u;
+        uint32_t range = max2(__byte_perm(hi2, lo2, 0x5410), __byte_perm(hi2, lo2, 0x7632));
 #pragma unroll
-        for (int o = 1; o < X::kLanes; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            odd += __shfl_xor_sync(0xffffffffu, odd, o);
-        }
-        const bool bad = !(odd == 0.f);
+        for (int o = 1; o < X::kLanes; o <<= 1) range = max2(range, __shfl_xor_sync(0xffffffffu, range, o));
+        const float hi = bf16lo(range), lo = -bf16hi(range);
+        const bool bad = !((hi - hi) + (lo - lo) == 0.f);
         const float half_lo = 0.5f * lo;
         const uint32_t sb = bad ? 0x7fc0u : f32_to_bf16_bits(fmaf(0.5f, hi, -half_lo) / (0.5f * (float)X::kTop));
         const uint32_t zb = bad ? 0x7fc0u : __float_as_uint(lo) >> 16;
         const float scale = __uint_as_float(sb << 16), half_scale = 0.5f * scale;
-        // ---- codes
-        uint32_t w[X::kWords];
-#pragma unroll
-        for (int i = 0; i < X::kWords; ++i) w[i] = 0u;
+        // ---- codes, as floats
+        float f[X::kDims];
         if (!bad && scale > 0.f) {
             const bool tiny = scale < 1e-30f;            // the reciprocal would leave the range: everything in fp64
-            const float inv = tiny ? 0.f : 1.f / half_scale;
+            const float inv = __fdividef(1.f, half_scale), most = (float)X::kTop * half_scale;
+            const float half = 0.5f * half_scale;
+            float worst = 0.f;
+            float e[X::kDims];
 #pragma unroll
             for (int i = 0; i < X::kDims; ++i) {
-                int c;
-                if (tiny)
-                    c = (int)fmin(rint(((double)f[i] - (double)lo) / (double)scale), (double)X::kTop);
-                else
-                    c = code_of(f[i], half_lo, half_scale, inv, lo, scale);
-                c = min(max(c, 0), X::kTop);
-                w[i * BITS / 32] |= (uint32_t)c << (i * BITS % 32);
+                const float v = i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]);
+                const float hx = fminf(fmaf(v, 0.5f, -half_lo), most);
+                f[i] = fmaf(hx, inv, kMagic) - kMagic;
+                e[i] = fabsf(fmaf(-f[i], half_scale, hx));
+                worst = fmaxf(worst, e[i]);
             }
+            if (tiny || worst >= half) {
+#pragma unroll
+                for (int i = 0; i < X::kDims; ++i) {
+                    const float v = i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]);
+                    if (tiny || e[i] >= half) f[i] = (float)fmin(rint(((double)v - (double)lo) / (double)scale), (double)X::kTop);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < X::kDims; ++i) f[i] = 0.f;
         }
-        uint8_t* const group = p.cache + block * p.block_stride + ((int64_t)x.h * (p.T / kRows) + t / kRows) * X::kGroup;
-        const int tt = t % kRows;
+        // ---- 16 bits at a time: the codes side by side in one float of 2^23
+        uint32_t w[X::kWords];
+        constexpr int kIn16 = 16 / BITS;
+#pragma unroll
+        for (int i = 0; i < X::kWords; ++i) {
+            uint32_t part[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float a = kMagic + f[(2 * i + j) * kIn16];
+#pragma unroll
+                for (int k = 1; k < kIn16; ++k) a = fmaf(f[(2 * i + j) * kIn16 + k], (float)(1 << (BITS * k)), a);
+                part[j] = __float_as_uint(a);
+            }
+            w[i] = __byte_perm(part[0], part[1], 0x5410);
+        }
         if (x.kv == 0) {
             if (live) {
                 uint8_t* const d = group + k_at<BITS, D>(tt, lr);
@@ -197,10 +234,6 @@ __global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
             }
         } else {
             uint8_t* const part = group + kRows * X::kRowBytes;
-            // is the neighbouring row the other token of the pair?
-            const int64_t place = live ? block * p.T + t : -2 - row;
-            const int64_t other = __shfl_xor_sync(0xffffffffu, place, X::kLanes);
-            const bool paired = live && other == (place ^ 1) && (place & 1) == (row & 1);
 #pragma unroll
             for (int i = 0; i < X::kWords; ++i) {
                 const uint32_t y = __shfl_xor_sync(0xffffffffu, w[i], X::kLanes);
@@ -219,86 +252,117 @@ __global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
     }
 }
 
-template <int BITS, int D>
+template <int BITS, int D, int HC>
 __global__ void __launch_bounds__(256) quant_read_kernel(const QuantParams p)
 {
     using X = Q<BITS, D>;
     const int lane = threadIdx.x & 31, lr = lane % X::kLanes, row = lane / X::kLanes;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    const int per_block = p.T / X::kTokens;
-    for (int64_t un = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); un < p.units; un += step) {
-        const Unit x = unit_of(un, p.H);
-        const int64_t i = x.tg / per_block;
-        const int t = (int)(x.tg - i * per_block) * X::kTokens + row;
-        const int id = checked_block_id(p.ids, i, p.n_blocks, lane == 0 ? p.err : nullptr);
-        const int64_t out = checked_out_row(p.out_slots, i, p.n_src, lane == 0 ? p.err : nullptr);
-        if (id < 0 || out < 0) continue;                 // (the same for the whole warp)
-        const uint8_t* const group = p.cache + (int64_t)id * p.block_stride + ((int64_t)x.h * (p.T / kRows) + t / kRows) * X::kGroup;
-        const int tt = t % kRows;
-        uint32_t w[X::kWords];
+    const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (item >= p.items) return;
+    const Piece x = piece_of<HC>(item, p.head_chunks);
+    const uint32_t per_block = (uint32_t)p.T / X::kTokens;
+    const uint32_t i = x.tg / per_block;
+    const int t = (int)(x.tg - i * per_block) * X::kTokens + row;
+    const int id = checked_block_id(p.ids, i, p.n_blocks, lane == 0 ? p.err : nullptr);
+    const int64_t out = checked_out_row(p.out_slots, i, p.n_src, lane == 0 ? p.err : nullptr);
+    if (id < 0 || out < 0) return;                       // (the same for the whole warp)
+    const int group_step = (p.T / kRows) * X::kGroup;
+    const uint8_t* const group = p.cache + (int64_t)id * p.block_stride + (int64_t)x.h * group_step + (t / kRows) * X::kGroup;
+    const int tt = t % kRows;
+    uint32_t w[HC][X::kWords], sz[HC];
+#pragma unroll
+    for (int c = 0; c < HC; ++c) {
+        if (x.h + c >= p.H) break;
+        const uint8_t* const g = group + c * group_step;
         if (x.kv == 0) {
-            const uint8_t* const s = group + k_at<BITS, D>(tt, lr);
-            if (X::kWords == 1) w[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+            const uint8_t* const s = g + k_at<BITS, D>(tt, lr);
+            if (X::kWords == 1) w[c][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
             if (X::kWords == 2) {
                 const uint2 y = __ldg(reinterpret_cast<const uint2*>(s));
-                w[0] = y.x;
-                w[X::kWords - 1] = y.y;
+                w[c][0] = y.x;
+                w[c][X::kWords - 1] = y.y;
             }
             if (X::kWords == 4) {
                 const uint4 y = __ldg(reinterpret_cast<const uint4*>(s));
-                w[0] = y.x;
-                w[1 % X::kWords] = y.y;
-                w[2 % X::kWords] = y.z;
-                w[3 % X::kWords] = y.w;
+                w[c][0] = y.x;
+                w[c][1 % X::kWords] = y.y;
+                w[c][2 % X::kWords] = y.z;
+                w[c][3 % X::kWords] = y.w;
             }
         } else {
-            const uint8_t* const part = group + kRows * X::kRowBytes;
+#pragma unroll
+            for (int j = 0; j < X::kWords; ++j)
+                w[c][j] = __ldg(reinterpret_cast<const uint32_t*>(g + kRows * X::kRowBytes +
+                                                                   v_at<BITS, D>(tt & ~1, (lr * X::kWords + j) * 2 + (row & 1))));
+        }
+        sz[c] = __ldg(reinterpret_cast<const uint32_t*>(g + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4));
+    }
+    uint16_t* const dst = const_cast<uint16_t*>(x.kv ? p.v : p.k) + out * (x.kv ? p.v_block : p.k_block) +
+                          (int64_t)t * (x.kv ? p.v_token : p.k_token) + (int64_t)x.h * D + lr * X::kDims;
+#pragma unroll
+    for (int c = 0; c < HC; ++c) {
+        if (x.h + c >= p.H) break;
+        if (x.kv) {
 #pragma unroll
             for (int j = 0; j < X::kWords; ++j) {
-                const int u = (lr * X::kWords + j) * 2;
-                const uint32_t mine = __ldg(reinterpret_cast<const uint32_t*>(part + v_at<BITS, D>(tt & ~1, u + (row & 1))));
-                const uint32_t y = __shfl_xor_sync(0xffffffffu, mine, X::kLanes);
-                w[j] = (row & 1) ? __byte_perm(y, mine, 0x7632) : __byte_perm(mine, y, 0x5410);
+                const uint32_t y = __shfl_xor_sync(0xffffffffu, w[c][j], X::kLanes);
+                w[c][j] = (row & 1) ? __byte_perm(y, w[c][j], 0x7632) : __byte_perm(w[c][j], y, 0x5410);
             }
         }
-        const uint32_t sz = __ldg(reinterpret_cast<const uint32_t*>(group + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4));
-        const float scale = bf16lo(sz), zero = bf16hi(sz);
-        uint16_t* const dst = const_cast<uint16_t*>(x.kv ? p.v : p.k) + out * (x.kv ? p.v_block : p.k_block) +
-                              (int64_t)t * (x.kv ? p.v_token : p.k_token) + (int64_t)x.h * D + lr * X::kDims;
+        const float scale = bf16lo(sz[c]), zero = bf16hi(sz[c]);
+        float f[X::kDims];
 #pragma unroll
-        for (int j = 0; j < X::kDims / 8; ++j) {
-            uint32_t o[4];
+        for (int j = 0; j < X::kWords; ++j) {
+            const uint32_t even = BITS == 4 ? w[c][j] & 0x0f0f0f0fu : w[c][j], odd = BITS == 4 ? (w[c][j] >> 4) & 0x0f0f0f0fu : 0u;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int a = j * 8 + 2 * k;
-                const uint32_t c0 = (w[a * BITS / 32] >> (a * BITS % 32)) & X::kTop;
-                const uint32_t c1 = (w[(a + 1) * BITS / 32] >> ((a + 1) * BITS % 32)) & X::kTop;
-                o[k] = pack2(fmaf((float)c0, scale, zero), fmaf((float)c1, scale, zero));
+                const float a = __uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + k)) - kMagic;
+                if (BITS == 4) {
+                    const float b = __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + k)) - kMagic;
+                    f[(j * 8 + 2 * k) % X::kDims] = fmaf(a, scale, zero);
+                    f[(j * 8 + 2 * k + 1) % X::kDims] = fmaf(b, scale, zero);
+                } else {
+                    f[(j * 4 + k) % X::kDims] = fmaf(a, scale, zero);
+                }
             }
-            st_stream16(dst + j * 8, make_uint4(o[0], o[1], o[2], o[3]));
         }
+#pragma unroll
+        for (int j = 0; j < X::kDims / 8; ++j)
+            st_stream16(dst + c * D + j * 8, make_uint4(pack2(f[8 * j], f[8 * j + 1]), pack2(f[8 * j + 2], f[8 * j + 3]),
+                                                        pack2(f[8 * j + 4], f[8 * j + 5]), pack2(f[8 * j + 6], f[8 * j + 7])));
     }
 }
 
 enum Form { kTokensForm, kBlocksForm, kReadForm };
+
+template <int BITS, int D, int HC>
+int32_t launch_heads(QuantParams& p, Form form, int64_t groups, cudaStream_t st)
+{
+    p.head_chunks = (uint32_t)((p.H + HC - 1) / HC);
+    const int64_t items = groups * 2 * p.head_chunks;
+    if (items > INT32_MAX) return UCMX_EUNSUPPORTED;     // (more rows than any memory holds)
+    p.items = (uint32_t)items;
+    const unsigned grid = (unsigned)((items + 7) / 8);
+    if (form == kTokensForm)
+        quant_write_kernel<BITS, D, false, HC><<<grid, 256, 0, st>>>(p);
+    else if (form == kBlocksForm)
+        quant_write_kernel<BITS, D, true, HC><<<grid, 256, 0, st>>>(p);
+    else
+        quant_read_kernel<BITS, D, HC><<<grid, 256, 0, st>>>(p);
+    UCMX_LAUNCH_CHECK("quant_cache_kernel");
+    return UCMX_OK;
+}
 
 template <int BITS, int D>
 int32_t launch(QuantParams& p, Form form, cudaStream_t st)
 {
     using X = Q<BITS, D>;
     const int64_t groups = form == kTokensForm ? (p.n + X::kTokens - 1) / X::kTokens : p.n * (p.T / X::kTokens);
-    p.units = groups * 2 * p.H;
-    int64_t grid = (p.units + 7) / 8;
-    const int64_t most = (int64_t)sm_count() * 8;
-    if (grid > most) grid = most;
-    if (form == kTokensForm)
-        quant_write_kernel<BITS, D, false><<<(unsigned)grid, 256, 0, st>>>(p);
-    else if (form == kBlocksForm)
-        quant_write_kernel<BITS, D, true><<<(unsigned)grid, 256, 0, st>>>(p);
-    else
-        quant_read_kernel<BITS, D><<<(unsigned)grid, 256, 0, st>>>(p);
-    UCMX_LAUNCH_CHECK("quant_cache_kernel");
-    return UCMX_OK;
+    // Four rows of a lane in flight (two of the double-width ones) as soon as that still gives every SM its warps; with the few
+    // tokens of a decode step one row per lane, over as many warps as there are rows.
+    constexpr int kMany = D == 256 ? 2 : 4;
+    if (groups * 2 * ((p.H + kMany - 1) / kMany) >= (int64_t)sm_count() * 32) return launch_heads<BITS, D, kMany>(p, form, groups, st);
+    return launch_heads<BITS, D, 1>(p, form, groups, st);
 }
 
 int32_t dispatch(QuantParams& p, const ucmx_quant_geometry* g, Form form, cudaStream_t st)

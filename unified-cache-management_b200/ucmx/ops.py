@@ -674,7 +674,7 @@ def block_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     block_ids are physical blocks (what topk_ragged returns with id_map, or remap_resident's table); or positions are places in
     the sequence (topk_ragged without id_map) and block_table / table_offsets the requests' block tables.  Negative = skip.
     With both block_ids and positions the latter only say where the blocks stand; without positions the i-th stands at i.
-    ctx_lens: lengths of the sequences; tokens at or beyond are not seen (nor read), and of a request's n query tokens the j-th
+    ctx_lens: lengths of the sequences; tokens at or beyond are not seen, and of a request's n query tokens the j-th
     sees n-1-j fewer.  Without it every token of every listed block is seen.
     q_offsets, max_q_tokens: each request's query tokens (one each without).  A query that sees nothing gives zeros.
     lse: fp32 [n_query_tokens, n_q_heads], receives the logarithm of the softmax's sum.  scale defaults to head_dim ** -0.5."""
