@@ -26,6 +26,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ucmx {
@@ -160,6 +162,13 @@ __device__ __forceinline__ void load_panel(unsigned char* dst, const CUtensorMap
             smem_u32(dst)),
         "l"(map), "r"(x), "r"(h), "r"(token), "r"(block), "r"(smem_u32(bar))
         : "memory");
+}
+// One lane of a converged warp.  (Told this way the compiler issues a copy once; behind `lane == 0` it loops over the lanes.)
+__device__ __forceinline__ bool one_lane()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar)
 {
@@ -374,13 +383,18 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     int32_t p_look = 32;               // lanes p_look .. p_look + kU - 1 know the slices to load next; 32: look again
     int32_t p_entries = 0;             // entries of the request that count
     int32_t p_end = 0;                 // first position that no column of the tile sees
-    int32_t my_id = 0, my_pos = 0;     // this lane's slice: block, first position,
-    uint32_t my_span = 0;              // first token inside the block * 32 + tokens to load
+    int32_t p_all = 0;                 // first position that some column of the tile does not see
+    // this lane's slice: where it lies (bf16: block and first token, codes: byte address), its first position, and
+    // bits 0..4 tokens to load, bit 5 every column sees all 16, bit 6 the next lane's slice follows it in memory
+    int32_t my_id = 0, my_sub = 0, my_pos = 0;
+    const uint8_t* my_src = nullptr;
+    uint32_t my_flags = 0;
     bool p_done = false;
     int32_t p_next = lo;               // where the next segment begins
+    uint32_t plain = 0;                // bit s: the step in stage s needs no masks
     // what this lane has to know of slice `at` of segment ps
     auto look_up = [&](int32_t at) {
-        my_span = 0;
+        my_flags = 0;
         if (at >= ps.hi) return;
         const int32_t s = at - ps.begin;
         const int32_t e = s / p.spe, sub = (s - e * p.spe) * kRows;
@@ -405,14 +419,21 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             return;
         }
         int32_t nv = min(kRows, p.T - sub);
+        bool seen = nv == kRows;
         if (p.ctx) {
             const int64_t pos = (int64_t)pos_block * p.T + sub;
             if (pos >= p_end) return;
             nv = (int32_t)min((int64_t)nv, p_end - pos);
             my_pos = (int32_t)pos;
+            seen = seen && pos + kRows <= p_all;
         }
-        my_id = id;
-        my_span = (uint32_t)sub * 32u + (uint32_t)nv;
+        if (FMT == 16) {
+            my_id = id;
+            my_sub = sub;
+        } else {
+            my_src = p.k + (int64_t)id * p.k_block + (int64_t)(ps.h * p.spe + (sub >> 4)) * L::kGroup;
+        }
+        my_flags = (uint32_t)nv | (seen ? 32u : 0u);
     };
     // start the loads of the warp's next step into stage s; every step completes its barrier, with or without bytes
     auto issue = [&](int s) {
@@ -430,7 +451,9 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                 if (p.ctx) {
                     int q0, nq;
                     queries_of(p, ps.r, q0, nq);
-                    p_end = __ldg(p.ctx + ps.r) - (nq - 1 - min(nq - 1, (ps.ct * X::kCols + X::kCols - 1) / p.G));
+                    const int32_t ctx = __ldg(p.ctx + ps.r) - (nq - 1);
+                    p_end = ctx + min(nq - 1, (ps.ct * X::kCols + X::kCols - 1) / p.G);
+                    p_all = ctx + ps.ct * X::kCols / p.G;
                 }
             }
             if (p_done) return;
@@ -438,20 +461,19 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         if (p_look >= 32) {
             look_up(p_at + (lane / kU) * kStep + lane % kU);
             p_look = 0;
+            if (kU == 2) {
+                const unsigned long long next = __shfl_down_sync(0xffffffffu, (unsigned long long)my_src, 1);
+                const uint32_t other = __shfl_down_sync(0xffffffffu, my_flags, 1);
+                if ((my_flags & 31u) && (other & 31u) && next == (unsigned long long)my_src + L::kGroup) my_flags |= 64u;
+            }
         }
         const int from = p_look + lane % kU;
-        const int32_t id = __shfl_sync(0xffffffffu, my_id, from);
-        const uint32_t span = __shfl_sync(0xffffffffu, my_span, from);
-        const int32_t pos = __shfl_sync(0xffffffffu, my_pos, from);
-        const int nv = span & 31u;
-        const int32_t sub = (int32_t)(span >> 5);
-        p_at += kStep;
-        p_look += kU;
+        const uint32_t flags = __shfl_sync(0xffffffffu, my_flags, from);
         unsigned char* const dst = ring + s * L::kStage;
-        if (lane < kU) note[s * kU + lane] = make_int2(nv, pos);
         if (FMT == 16) {
-            if (lane == 0) {
-                if (nv > 0) {
+            const int32_t id = __shfl_sync(0xffffffffu, my_id, p_look), sub = __shfl_sync(0xffffffffu, my_sub, p_look);
+            if (one_lane()) {
+                if (flags & 31u) {
                     mbar_expect_tx(&full[s], (uint32_t)(2 * p.box) * L::kRowBytes);
 #pragma unroll
                     for (int i = 0; i < D / 64; ++i) {
@@ -463,19 +485,31 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                 }
             }
         } else {
-            // two slices that follow one another in one block are one copy
-            const int32_t id1 = __shfl_sync(0xffffffffu, id, 1), sub1 = __shfl_sync(0xffffffffu, sub, 1), nv1 = __shfl_sync(0xffffffffu, nv, 1);
-            const bool both = id1 == __shfl_sync(0xffffffffu, id, 0) && sub1 == __shfl_sync(0xffffffffu, sub, 0) + kRows &&
-                              nv1 > 0 && __shfl_sync(0xffffffffu, nv, 0) > 0;
-            const uint8_t* const src = p.k + (int64_t)id * p.k_block + (int64_t)(ps.h * p.spe + (sub >> 4)) * L::kGroup;
-            if (lane == 0) {
-                const uint32_t bytes = nv > 0 ? (both ? 2 * L::kGroup : L::kGroup) : 0;
-                mbar_expect_tx(&full[s], bytes + (!both && nv1 > 0 ? L::kGroup : 0));
-                if (nv > 0) bulk_g2s(dst, src, bytes, &full[s]);
+            const unsigned long long src = __shfl_sync(0xffffffffu, (unsigned long long)my_src, p_look);
+            if (__any_sync(0xffffffffu, flags & 64u)) {          // two slices side by side: one copy
+                if (one_lane()) {
+                    mbar_expect_tx(&full[s], 2 * L::kGroup);
+                    bulk_g2s(dst, (const void*)src, 2 * L::kGroup, &full[s]);
+                }
+            } else {
+                const unsigned long long src1 = __shfl_sync(0xffffffffu, (unsigned long long)my_src, p_look + kU - 1);
+                const uint32_t have = __ballot_sync(0xffffffffu, (flags & 31u) != 0u);       // bits 0 and 1: the two slices
+                if (one_lane()) {
+                    mbar_expect_tx(&full[s], __popc(have & 3u) * L::kGroup);
+                    if (have & 1u) bulk_g2s(dst, (const void*)src, L::kGroup, &full[s]);
+                    if (have & 2u) bulk_g2s(dst + L::kUnit, (const void*)src1, L::kGroup, &full[s]);
+                }
             }
-            __syncwarp();
-            if (lane == 1 && !both && nv > 0) bulk_g2s(dst + L::kUnit, src, L::kGroup, &full[s]);
         }
+        if (__all_sync(0xffffffffu, flags & 32u)) {
+            plain |= 1u << s;
+        } else {
+            plain &= ~(1u << s);
+            const int32_t pos = __shfl_sync(0xffffffffu, my_pos, from);
+            if (lane < kU) note[s * kU + lane] = make_int2((int)(flags & 31u), pos);
+        }
+        p_at += kStep;
+        p_look += kU;
     };
 
 #pragma unroll 1
@@ -629,312 +663,321 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                 for (int i = 0; i < 4; ++i) o[mt][nt][i] = 0.f;
         }
 
-        // ---------------------------------------------------------------------------- the warp's slices of this item
-#pragma unroll 1
-        for (int32_t s = sg.lo + warp * kU; s < sg.hi; s += kStep) {
+        // One step over the slices in the current stage.  MASKED: some column does not see some token of it (the ends of
+        // sequences, blocks shorter than a slice); a form of its own, so that the others carry none of that.
+        auto step = [&](auto masked_) {
+            constexpr bool MASKED = decltype(masked_)::value;
             const uint32_t st_u = ring_u + stage * L::kStage;
-            if (!dead && !mbar_wait(&full[stage], parity)) {
-                if (p.err && lane == 0) atomicExch(p.err, 1);
-                dead = true;
-            }
             int nv[kU], pos0[kU];
-            bool any = false, masked = false;
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int2 n = note[stage * kU + u];
-                nv[u] = n.x;
-                pos0[u] = n.y;
-                any |= nv[u] > 0;
-                masked |= nv[u] < kRows || (p.ctx != nullptr && pos0[u] + kRows > limit_min);
-            }
-            if (any && !dead) {
-                // ---- S^T = K Q^T
-                float sc[kU][NT][4];
+            if (MASKED) {
+                bool any = false;
 #pragma unroll
                 for (int u = 0; u < kU; ++u) {
-                    const uint32_t un_u = st_u + u * L::kUnit;
-                    float s2[NT][4];                             // every other product: half the chain of dependent sums
+                    const int2 n = note[stage * kU + u];
+                    nv[u] = n.x;
+                    pos0[u] = n.y;
+                    any |= nv[u] > 0;
+                }
+                if (!any) return;
+            }
+            // ---- S^T = K Q^T
+            float sc[kU][NT][4];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                const uint32_t un_u = st_u + u * L::kUnit;
+                float s2[NT][4];                             // every other product: half the chain of dependent sums
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sc[u][nt][i] = FMT == 16 ? 0.f : qoff[nt][i & 1];
+                        s2[nt][i] = 0.f;
+                    }
+                auto qk = [&](int ks, const uint32_t (&a)[4]) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        uint32_t b0, b1;
+                        if (X::kQReg) {
+                            b0 = qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][0];
+                            b1 = qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][1];
+                        } else {
+                            const uint2 b = q_frag[(ks * NT + nt) * 32 + lane];
+                            b0 = b.x;
+                            b1 = b.y;
+                        }
+                        float (&to)[4] = NT == 1 && (ks & 1) ? s2[nt] : sc[u][nt];
+                        if (FMT == 16) mma(to, a, b0, b1);
+                        else mma_f16(to, a, b0, b1);
+                    }
+                };
+                if (FMT == 16) {
+                    const uint32_t ka = un_u + (lane & 15) * 128;
+#pragma unroll
+                    for (int ks = 0; ks < X::kKSteps; ++ks) {
+                        uint32_t a[4];
+                        ldsm4(a, ka + (ks / 4) * L::kBf16Panel + ((((ks % 4) * 2 + (lane >> 4)) ^ (lane & 7)) << 4));
+                        qk(ks, a);
+                    }
+                } else {
+                    constexpr int kChunk = L::kPanel / 4;    // bytes of a row in a panel that a lane reads
+#pragma unroll
+                    for (int pn = 0; pn < L::kPanels; ++pn) {
+                        const uint32_t ka = un_u + pn * (kRows * L::kPanel) + lane * kChunk;
+                        uint32_t x[4], y[4];                 // rows g and g + 8
+                        lds_words<kChunk>(x, ka);
+                        lds_words<kChunk>(y, ka + 8 * L::kPanel);
+#pragma unroll
+                        for (int i = 0; i < kChunk / 4; ++i) {
+                            if (FMT == 4) {
+#pragma unroll
+                                for (int half = 0; half < 2; ++half) {
+                                    const uint32_t a[4] = {k_nibbles(x[i], 2 * half), k_nibbles(y[i], 2 * half),
+                                                           k_nibbles(x[i], 2 * half + 1), k_nibbles(y[i], 2 * half + 1)};
+                                    qk((pn * (kChunk / 4) + i) * 2 + half, a);
+                                }
+                            } else {
+                                const uint32_t a[4] = {k_bytes(x[i], 0), k_bytes(y[i], 0), k_bytes(x[i], 1), k_bytes(y[i], 1)};
+                                qk(pn * (kChunk / 4) + i, a);
+                            }
+                        }
+                    }
+                }
+                if (NT == 1) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[u][0][i] += s2[0][i];
+                }
+            }
+
+            // ---- scores in powers of two; rows g (values 0, 1) and g + 8 (values 2, 3)
+            float vs[kU][2], vz[kU][2];
+#pragma unroll
+            for (int u = 0; u < kU; ++u) {
+                if (FMT == 16) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[u][nt][i] *= p.scale_log2;
+                } else {
+                    constexpr float mid = FMT == 4 ? 8.f : 128.f;
+                    const uint32_t pa = st_u + u * L::kUnit + 2 * kRows * L::kRowBytes + g * 4;
+#pragma unroll
+                    for (int row = 0; row < 2; ++row) {
+                        const uint32_t k0 = lds4(pa + row * 32), v0 = lds4(pa + 64 + row * 32);
+                        const float kz = fmaf(bf16lo(k0), mid, bf16hi(k0));      // the centred codes' zero
+                        const float ksc = bf16lo(k0);
+                        vs[u][row] = bf16lo(v0);
+                        vz[u][row] = fmaf(vs[u][row], mid, bf16hi(v0));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                sc[u][nt][2 * row + e] = fmaf(sc[u][nt][2 * row + e], ksc * qmul[nt][e], kz * qsum[nt][e]);
+                    }
+                }
+            }
+            uint32_t hide[kU];                               // bit 4 nt + i: value i of tile nt is not seen
+#pragma unroll
+            for (int u = 0; u < kU; ++u) hide[u] = 0;
+            if (MASKED) {
+#pragma unroll
+                for (int u = 0; u < kU; ++u)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            sc[u][nt][i] = FMT == 16 ? 0.f : qoff[nt][i & 1];
-                            s2[nt][i] = 0.f;
-                        }
-                    auto qk = [&](int ks, const uint32_t (&a)[4]) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            uint32_t b0, b1;
-                            if (X::kQReg) {
-                                b0 = qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][0];
-                                b1 = qf[X::kQReg ? ks : 0][X::kQReg ? nt : 0][1];
-                            } else {
-                                const uint2 b = q_frag[(ks * NT + nt) * 32 + lane];
-                                b0 = b.x;
-                                b1 = b.y;
-                            }
-                            float (&to)[4] = NT == 1 && (ks & 1) ? s2[nt] : sc[u][nt];
-                            if (FMT == 16) mma(to, a, b0, b1);
-                            else mma_f16(to, a, b0, b1);
-                        }
-                    };
-                    if (FMT == 16) {
-                        const uint32_t ka = un_u + (lane & 15) * 128;
-#pragma unroll
-                        for (int ks = 0; ks < X::kKSteps; ++ks) {
-                            uint32_t a[4];
-                            ldsm4(a, ka + (ks / 4) * L::kBf16Panel + ((((ks % 4) * 2 + (lane >> 4)) ^ (lane & 7)) << 4));
-                            qk(ks, a);
-                        }
-                    } else {
-                        constexpr int kChunk = L::kPanel / 4;    // bytes of a row in a panel that a lane reads
-#pragma unroll
-                        for (int pn = 0; pn < L::kPanels; ++pn) {
-                            const uint32_t ka = un_u + pn * (kRows * L::kPanel) + lane * kChunk;
-                            uint32_t x[4], y[4];                 // rows g and g + 8
-                            lds_words<kChunk>(x, ka);
-                            lds_words<kChunk>(y, ka + 8 * L::kPanel);
-#pragma unroll
-                            for (int i = 0; i < kChunk / 4; ++i) {
-                                if (FMT == 4) {
-#pragma unroll
-                                    for (int half = 0; half < 2; ++half) {
-                                        const uint32_t a[4] = {k_nibbles(x[i], 2 * half), k_nibbles(y[i], 2 * half),
-                                                               k_nibbles(x[i], 2 * half + 1), k_nibbles(y[i], 2 * half + 1)};
-                                        qk((pn * (kChunk / 4) + i) * 2 + half, a);
-                                    }
-                                } else {
-                                    const uint32_t a[4] = {k_bytes(x[i], 0), k_bytes(y[i], 0), k_bytes(x[i], 1), k_bytes(y[i], 1)};
-                                    qk(pn * (kChunk / 4) + i, a);
-                                }
+                            const int row = g + (i >> 1) * 8;
+                            if (row >= nv[u] || pos0[u] + row >= limit[nt][i & 1]) {
+                                sc[u][nt][i] = -INFINITY;
+                                hide[u] |= 1u << (4 * nt + i);
                             }
                         }
-                    }
-                    if (NT == 1) {
+            }
+            // ---- running maximum: moved only when it is passed by more than the slack
+            bool passed = false;
+            float top[NT][2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) sc[u][0][i] += s2[0][i];
-                    }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    top[nt][e] = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
+                    if (kU == 2) top[nt][e] = fmaxf(top[nt][e], fmaxf(sc[kU - 1][nt][e], sc[kU - 1][nt][e + 2]));
+                    passed |= top[nt][e] > pass[nt][e];
                 }
-
-                // ---- scores in powers of two; rows g (values 0, 1) and g + 8 (values 2, 3)
-                float vs[kU][2], vz[kU][2];
-#pragma unroll
-                for (int u = 0; u < kU; ++u) {
-                    if (FMT == 16) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) sc[u][nt][i] *= p.scale_log2;
-                    } else {
-                        constexpr float mid = FMT == 4 ? 8.f : 128.f;
-                        const uint32_t pa = st_u + u * L::kUnit + 2 * kRows * L::kRowBytes + g * 4;
-#pragma unroll
-                        for (int row = 0; row < 2; ++row) {
-                            const uint32_t k0 = lds4(pa + row * 32), v0 = lds4(pa + 64 + row * 32);
-                            const float kz = fmaf(bf16lo(k0), mid, bf16hi(k0));      // the centred codes' zero
-                            const float ksc = bf16lo(k0);
-                            vs[u][row] = bf16lo(v0);
-                            vz[u][row] = fmaf(vs[u][row], mid, bf16hi(v0));
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e)
-                                    sc[u][nt][2 * row + e] = fmaf(sc[u][nt][2 * row + e], ksc * qmul[nt][e], kz * qsum[nt][e]);
-                        }
-                    }
-                }
-                uint32_t hide[kU];                               // bit 4 nt + i: value i of tile nt is not seen
-#pragma unroll
-                for (int u = 0; u < kU; ++u) hide[u] = 0;
-                if (masked) {
-#pragma unroll
-                    for (int u = 0; u < kU; ++u)
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int row = g + (i >> 1) * 8;
-                                if (row >= nv[u] || pos0[u] + row >= limit[nt][i & 1]) {
-                                    sc[u][nt][i] = -INFINITY;
-                                    hide[u] |= 1u << (4 * nt + i);
-                                }
-                            }
-                }
-                // ---- running maximum: moved only when it is passed by more than the slack
-                bool passed = false;
-                float top[NT][2];
+            if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        top[nt][e] = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
-                        if (kU == 2) top[nt][e] = fmaxf(top[nt][e], fmaxf(sc[kU - 1][nt][e], sc[kU - 1][nt][e + 2]));
-                        passed |= top[nt][e] > pass[nt][e];
+                        float x = top[nt][e];
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        const float now = fmaxf(m[nt][e], x);
+                        // (before the first score nothing but zeros and NaN can have been added: both stay)
+                        const float f = m[nt][e] > -INFINITY ? exp2_fast(m[nt][e] - now) : 1.f;
+                        if (now > -INFINITY) {
+                            m[nt][e] = base[nt][e] = now;
+                            pass[nt][e] = now + kMaxSlack;
+                        }
+                        l[nt][e] *= f;
+                        z[nt][e] *= f;
+#pragma unroll
+                        for (int mt = 0; mt < X::kMTiles; ++mt) {
+                            o[mt][nt][e] *= f;
+                            o[mt][nt][e + 2] *= f;
+                        }
                     }
-                if (__any_sync(0xffffffffu, passed)) {
+            }
+            // ---- weights, and their bf16 halves with tokens along the columns' other side
+            uint32_t ph[kU][NT][2], pl[kU][NT][2];
+            float wt[kU][NT][4];
+#pragma unroll
+            for (int u = 0; u < kU; ++u)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float (&w)[4] = wt[u][nt];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = exp2_fast(sc[u][nt][i] - base[nt][i & 1]);
+                    l[nt][0] += w[0] + w[2];
+                    l[nt][1] += w[1] + w[3];
+                    if (FMT != 16) {
+                        if (MASKED) {                        // what stands in rows that are not seen may be anything
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const bool hd = (hide[u] >> (4 * nt + i)) & 1u;
+                                z[nt][i & 1] += hd ? 0.f : w[i] * vz[u][i >> 1];
+                                w[i] = hd ? 0.f : w[i] * vs[u][i >> 1];
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                z[nt][i & 1] = fmaf(w[i], vz[u][i >> 1], z[nt][i & 1]);
+                                w[i] *= vs[u][i >> 1];
+                            }
+                        }
+                    }
+                    const uint32_t a = pack_bf16(w[0], w[1]), b = pack_bf16(w[2], w[3]);
+                    const uint32_t al = pack_bf16(w[0] - bf16lo(a), w[1] - bf16hi(a));
+                    const uint32_t bl = pack_bf16(w[2] - bf16lo(b), w[3] - bf16hi(b));
+                    if (DUP) {
+                        ph[u][nt][0] = transpose8(q4 < 2 ? a : al);
+                        ph[u][nt][1] = transpose8(q4 < 2 ? b : bl);
+                    } else {
+                        ph[u][nt][0] = transpose8(a);
+                        ph[u][nt][1] = transpose8(b);
+                        pl[u][nt][0] = transpose8(al);
+                        pl[u][nt][1] = transpose8(bl);
+                    }
+                }
+            // A row that some columns see and others do not may hold an infinity or a NaN, and a weight of zero would not
+            // keep it out of the product: such a slice (the last tokens of a request with several queries) is added up
+            // column by column instead.
+            bool wild = false;
+            if (FMT == 16 && MASKED) {
+                unsigned char* const v_rows = ring + stage * L::kStage + (D / 64) * L::kBf16Panel;
+                // rows without a seen token: a weight of zero must meet a number
+                for (int i = lane; i < (kRows - nv[0]) * (D / 8); i += 32) {
+                    const int row = nv[0] + i / (D / 8), x = i % (D / 8);
+                    *reinterpret_cast<uint4*>(v_rows + (x / 8) * L::kBf16Panel + row * 128 + (x % 8) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async();                         // (the next load into the stage comes behind these stores)
+                if (pos0[0] + nv[0] > limit_min) {
+                    for (int i = lane; i < nv[0] * (D / 8); i += 32) {
+                        const int row = i / (D / 8), x = i % (D / 8);
+                        const uint4 q = *reinterpret_cast<const uint4*>(v_rows + (x / 8) * L::kBf16Panel + row * 128 + (x % 8) * 16);
+                        const uint32_t y[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            wild |= (y[k] & 0x7f80u) == 0x7f80u || (y[k] & 0x7f800000u) == 0x7f800000u;
+                    }
+                    wild = __any_sync(0xffffffffu, wild);
+                }
+                __syncwarp();
+            }
+            if (FMT == 16 && wild) {
+#pragma unroll 1
+                for (int row = 0; row < nv[0]; ++row) {
+                    const int src = (row & 7) * 4 + q4;
+                    const uint32_t hd = __shfl_sync(0xffffffffu, hide[0], src);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float x = top[nt][e];
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                            const float now = fmaxf(m[nt][e], x);
-                            // (before the first score nothing but zeros and NaN can have been added: both stay)
-                            const float f = m[nt][e] > -INFINITY ? exp2_fast(m[nt][e] - now) : 1.f;
-                            if (now > -INFINITY) {
-                                m[nt][e] = base[nt][e] = now;
-                                pass[nt][e] = now + kMaxSlack;
-                            }
-                            l[nt][e] *= f;
-                            z[nt][e] *= f;
+                            const float w0 = __shfl_sync(0xffffffffu, wt[0][nt][e], src);
+                            const float w1 = __shfl_sync(0xffffffffu, wt[0][nt][e + 2], src);
+                            const int bit = 4 * nt + e + (row >> 3) * 2;
+                            if (((hd >> bit) & 1u) || (DUP && q4 >= 2)) continue;
+                            const float w = row < 8 ? w0 : w1;
 #pragma unroll
-                            for (int mt = 0; mt < X::kMTiles; ++mt) {
-                                o[mt][nt][e] *= f;
-                                o[mt][nt][e + 2] *= f;
-                            }
+                            for (int mt = 0; mt < X::kMTiles; ++mt)
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    const int x = mt * 2 + k;        // the 16-byte piece of value mt * 16 + k * 8 + g
+                                    const uint16_t b = *reinterpret_cast<const uint16_t*>(
+                                        ring + stage * L::kStage + (D / 64 + x / 8) * L::kBf16Panel + row * 128 +
+                                        (((x % 8) ^ (row & 7)) << 4) + g * 2);
+                                    o[mt][nt][e + 2 * k] += w * __uint_as_float((uint32_t)b << 16);
+                                }
                         }
                 }
-                // ---- weights, and their bf16 halves with tokens along the columns' other side
-                uint32_t ph[kU][NT][2], pl[kU][NT][2];
-                float wt[kU][NT][4];
+            }
+            // ---- O^T += V^T P^T
 #pragma unroll
-                for (int u = 0; u < kU; ++u)
+            for (int u = 0; u < kU; ++u) {
+                const uint32_t un_u = st_u + u * L::kUnit;
+                auto pv = [&](int mt, const uint32_t (&a)[4]) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float (&w)[4] = wt[u][nt];
+                        mma(o[mt][nt], a, ph[u][nt][0], ph[u][nt][1]);
+                        if (!DUP) mma(o[mt][nt], a, pl[u][nt][0], pl[u][nt][1]);
+                    }
+                };
+                if (FMT == 16) {
+                    if (!wild) {
+                        const uint32_t va = un_u + (D / 64) * L::kBf16Panel + ((lane & 7) + ((lane >> 4) & 1) * 8) * 128;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = exp2_fast(sc[u][nt][i] - base[nt][i & 1]);
-                        l[nt][0] += w[0] + w[2];
-                        l[nt][1] += w[1] + w[3];
-                        if (FMT != 16) {
-                            if (masked) {                        // what stands in rows that are not seen may be anything
+                        for (int mt = 0; mt < X::kMTiles; ++mt) {
+                            uint32_t a[4];
+                            ldsm4_trans(a, va + (mt / 4) * L::kBf16Panel + ((((mt % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+                            pv(mt, a);
+                        }
+                    }
+                } else {
+                    constexpr int kChunk = L::kPanel / 4;    // bytes of a lane in half a panel: 2 tokens, 1/8 of the values
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const bool hd = (hide[u] >> (4 * nt + i)) & 1u;
-                                    z[nt][i & 1] += hd ? 0.f : w[i] * vz[u][i >> 1];
-                                    w[i] = hd ? 0.f : w[i] * vs[u][i >> 1];
+                    for (int pn = 0; pn < L::kPanels; ++pn) {
+                        const uint32_t va = un_u + kRows * L::kRowBytes + pn * (kRows * L::kPanel) + lane * kChunk;
+                        uint32_t x[4], y[4];                 // tokens 2 q4, 2 q4 + 1 and the two 8 behind them
+                        lds_words<kChunk>(x, va);
+                        lds_words<kChunk>(y, va + 8 * L::kPanel);
+#pragma unroll
+                        for (int i = 0; i < kChunk / 4; ++i) {
+                            if (FMT == 4) {
+#pragma unroll
+                                for (int half = 0; half < 2; ++half) {
+                                    const uint32_t a[4] = {v_nibbles(x[i], 2 * half), v_nibbles(x[i], 2 * half + 1),
+                                                           v_nibbles(y[i], 2 * half), v_nibbles(y[i], 2 * half + 1)};
+                                    pv(pn * (L::kPanelDims / 16) + i * 2 + half, a);
                                 }
                             } else {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    z[nt][i & 1] = fmaf(w[i], vz[u][i >> 1], z[nt][i & 1]);
-                                    w[i] *= vs[u][i >> 1];
-                                }
+                                const uint32_t a[4] = {v_bytes(x[i], 0), v_bytes(x[i], 1), v_bytes(y[i], 0), v_bytes(y[i], 1)};
+                                pv(pn * (L::kPanelDims / 16) + i, a);
                             }
                         }
-                        const uint32_t a = pack_bf16(w[0], w[1]), b = pack_bf16(w[2], w[3]);
-                        const uint32_t al = pack_bf16(w[0] - bf16lo(a), w[1] - bf16hi(a));
-                        const uint32_t bl = pack_bf16(w[2] - bf16lo(b), w[3] - bf16hi(b));
-                        if (DUP) {
-                            ph[u][nt][0] = transpose8(q4 < 2 ? a : al);
-                            ph[u][nt][1] = transpose8(q4 < 2 ? b : bl);
-                        } else {
-                            ph[u][nt][0] = transpose8(a);
-                            ph[u][nt][1] = transpose8(b);
-                            pl[u][nt][0] = transpose8(al);
-                            pl[u][nt][1] = transpose8(bl);
-                        }
                     }
-                // A row that some columns see and others do not may hold an infinity or a NaN, and a weight of zero would not
-                // keep it out of the product: such a slice (the last tokens of a request with several queries) is added up
-                // column by column instead.
-                bool wild = false;
-                if (FMT == 16 && masked) {
-                    unsigned char* const v_rows = ring + stage * L::kStage + (D / 64) * L::kBf16Panel;
-                    // rows without a seen token: a weight of zero must meet a number
-                    for (int i = lane; i < (kRows - nv[0]) * (D / 8); i += 32) {
-                        const int row = nv[0] + i / (D / 8), x = i % (D / 8);
-                        *reinterpret_cast<uint4*>(v_rows + (x / 8) * L::kBf16Panel + row * 128 + (x % 8) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async();                         // (the next load into the stage comes behind these stores)
-                    if (pos0[0] + nv[0] > limit_min) {
-                        for (int i = lane; i < nv[0] * (D / 8); i += 32) {
-                            const int row = i / (D / 8), x = i % (D / 8);
-                            const uint4 q = *reinterpret_cast<const uint4*>(v_rows + (x / 8) * L::kBf16Panel + row * 128 + (x % 8) * 16);
-                            const uint32_t y[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                wild |= (y[k] & 0x7f80u) == 0x7f80u || (y[k] & 0x7f800000u) == 0x7f800000u;
-                        }
-                        wild = __any_sync(0xffffffffu, wild);
-                    }
-                    __syncwarp();
                 }
-                if (FMT == 16 && wild) {
+            }
+        };
+        // ---------------------------------------------------------------------------- the warp's slices of this item
 #pragma unroll 1
-                    for (int row = 0; row < nv[0]; ++row) {
-                        const int src = (row & 7) * 4 + q4;
-                        const uint32_t hd = __shfl_sync(0xffffffffu, hide[0], src);
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float w0 = __shfl_sync(0xffffffffu, wt[0][nt][e], src);
-                                const float w1 = __shfl_sync(0xffffffffu, wt[0][nt][e + 2], src);
-                                const int bit = 4 * nt + e + (row >> 3) * 2;
-                                if (((hd >> bit) & 1u) || (DUP && q4 >= 2)) continue;
-                                const float w = row < 8 ? w0 : w1;
-#pragma unroll
-                                for (int mt = 0; mt < X::kMTiles; ++mt)
-#pragma unroll
-                                    for (int k = 0; k < 2; ++k) {
-                                        const int x = mt * 2 + k;        // the 16-byte piece of value mt * 16 + k * 8 + g
-                                        const uint16_t b = *reinterpret_cast<const uint16_t*>(
-                                            ring + stage * L::kStage + (D / 64 + x / 8) * L::kBf16Panel + row * 128 +
-                                            (((x % 8) ^ (row & 7)) << 4) + g * 2);
-                                        o[mt][nt][e + 2 * k] += w * __uint_as_float((uint32_t)b << 16);
-                                    }
-                            }
-                    }
-                }
-                // ---- O^T += V^T P^T
-#pragma unroll
-                for (int u = 0; u < kU; ++u) {
-                    const uint32_t un_u = st_u + u * L::kUnit;
-                    auto pv = [&](int mt, const uint32_t (&a)[4]) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            mma(o[mt][nt], a, ph[u][nt][0], ph[u][nt][1]);
-                            if (!DUP) mma(o[mt][nt], a, pl[u][nt][0], pl[u][nt][1]);
-                        }
-                    };
-                    if (FMT == 16) {
-                        if (!wild) {
-                            const uint32_t va = un_u + (D / 64) * L::kBf16Panel + ((lane & 7) + ((lane >> 4) & 1) * 8) * 128;
-#pragma unroll
-                            for (int mt = 0; mt < X::kMTiles; ++mt) {
-                                uint32_t a[4];
-                                ldsm4_trans(a, va + (mt / 4) * L::kBf16Panel + ((((mt % 4) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
-                                pv(mt, a);
-                            }
-                        }
-                    } else {
-                        constexpr int kChunk = L::kPanel / 4;    // bytes of a lane in half a panel: 2 tokens, 1/8 of the values
-#pragma unroll
-                        for (int pn = 0; pn < L::kPanels; ++pn) {
-                            const uint32_t va = un_u + kRows * L::kRowBytes + pn * (kRows * L::kPanel) + lane * kChunk;
-                            uint32_t x[4], y[4];                 // tokens 2 q4, 2 q4 + 1 and the two 8 behind them
-                            lds_words<kChunk>(x, va);
-                            lds_words<kChunk>(y, va + 8 * L::kPanel);
-#pragma unroll
-                            for (int i = 0; i < kChunk / 4; ++i) {
-                                if (FMT == 4) {
-#pragma unroll
-                                    for (int half = 0; half < 2; ++half) {
-                                        const uint32_t a[4] = {v_nibbles(x[i], 2 * half), v_nibbles(x[i], 2 * half + 1),
-                                                               v_nibbles(y[i], 2 * half), v_nibbles(y[i], 2 * half + 1)};
-                                        pv(pn * (L::kPanelDims / 16) + i * 2 + half, a);
-                                    }
-                                } else {
-                                    const uint32_t a[4] = {v_bytes(x[i], 0), v_bytes(x[i], 1), v_bytes(y[i], 0), v_bytes(y[i], 1)};
-                                    pv(pn * (L::kPanelDims / 16) + i, a);
-                                }
-                            }
-                        }
-                    }
-                }
+        for (int32_t s = sg.lo + warp * kU; s < sg.hi; s += kStep) {
+            if (!dead && !mbar_wait(&full[stage], parity)) {
+                if (p.err && lane == 0) atomicExch(p.err, 1);
+                dead = true;
+            }
+            if (!dead) {
+                if ((plain >> stage) & 1u) step(std::false_type());
+                else step(std::true_type());
             }
             __syncwarp();                                        // every lane is done with the stage
             if (!dead) issue(stage);
