@@ -264,18 +264,25 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[4], uint32_t a)
     }
 }
 
+// (x & mask) | base in one instruction (written out it became two, each with a constant of its own)
+__device__ __forceinline__ uint32_t mask_or(uint32_t x, uint32_t mask, uint32_t base)
+{
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(x), "r"(mask), "r"(base));
+    return r;
+}
 // V's codes as centred integers in bf16 (exact): 4 bits: c - 8, two per register from bits [4i, 4i+4) of both halves.
 // 0x4300 is 128.0 and a bf16 of that size counts in ones, so or-ing the code in adds it.
 __device__ __forceinline__ uint32_t v_nibbles(uint32_t w, int i)
 {
-    return sub_bf16x2(((w >> (4 * i)) & 0x000f000fu) | 0x43004300u, 0x43084308u);
+    return sub_bf16x2(mask_or(w >> (4 * i), 0x000f000fu, 0x43004300u), 0x43084308u);
 }
 // 8 bits: c - 128 from bytes i and i+2.  The low seven bits are or-ed into 128.0; the top bit chooses what is taken off:
 // 256.0 (0x4380) where it is clear, 128.0 (0x4300) where it is set.
 __device__ __forceinline__ uint32_t v_bytes(uint32_t w, int i)
 {
     const uint32_t x = w >> (8 * i);
-    return sub_bf16x2((x & 0x007f007fu) | 0x43004300u, (~x & 0x00800080u) | 0x43004300u);
+    return sub_bf16x2(mask_or(x, 0x007f007fu, 0x43004300u), mask_or(~x, 0x00800080u, 0x43004300u));
 }
 // K's codes become fp16, whose eleven bits hold two nibble positions: half the shifts, and half or none of the subtractions.
 // (The queries can follow: a column scaled by a power of two fits fp16 to 2^-25 of its largest value.  The weights cannot:
@@ -285,8 +292,8 @@ __device__ __forceinline__ uint32_t v_bytes(uint32_t w, int i)
 __device__ __forceinline__ uint32_t k_nibbles(uint32_t w, int i)
 {
     const uint32_t x = i < 2 ? w : w >> 8;
-    if (i & 1) return (x & 0x00f000f0u) | 0x64006400u;
-    return sub_f16x2((x & 0x000f000fu) | 0x64006400u, 0x64086408u);
+    if (i & 1) return mask_or(x, 0x00f000f0u, 0x64006400u);
+    return sub_f16x2(mask_or(x, 0x000f000fu, 0x64006400u), 0x64086408u);
 }
 // 8 bits: 1024 + c of bytes 2i and 2i+1: one instruction; the accumulator starts 1024 + 128 times the queries' sum below.
 __device__ __forceinline__ uint32_t k_bytes(uint32_t w, int i) { return __byte_perm(w, 0x64646464u, i ? 0x4342 : 0x4140); }
