@@ -26,6 +26,7 @@
 
 #include <cuda.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -1193,7 +1194,14 @@ int32_t run(const Params& p, const Maps* maps, Plan* plan, cudaStream_t st)
     plan->cols = X::kCols;
     if (!maps) return UCMX_OK;
     auto kern = attend_kernel<FMT, D, NT, DUP>;
-    UCMX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, X::kSmem));
+    // the attribute sticks to the function on a device: once is enough (2 us of host time a call)
+    static std::atomic<uint64_t> set{0};
+    int dev = 0;
+    UCMX_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !((set.load(std::memory_order_acquire) >> dev) & 1u)) {
+        UCMX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, X::kSmem));
+        if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_release);
+    }
     const int64_t all = (int64_t)p.total * p.spe * p.H * p.col_tiles;      // (attend_common has bounded it)
     // at least one slice per warp: below that more blocks only add partial results
     int64_t grid = (all + kWarps - 1) / kWarps;

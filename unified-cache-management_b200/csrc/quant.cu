@@ -10,8 +10,8 @@
 //
 // Arithmetic.  The range comes from packed bf16 maxima (of x and of -x; NaN wins).  Differences are taken of halves: exact, and no
 // overflow for any finite row.  A reciprocal, a rounding to the integers by adding 2^23, and the residual x - code*scale, which is
-// exact in fp32: where it is half a step or more (ties, and quotients the reciprocal put on the wrong side) the code is settled in
-// fp64.  A division per value was the bound of this kernel.
+// exact in fp32: where it is half a step or more (ties, and quotients the reciprocal put on the wrong side) the code is settled by
+// it and by what the difference x - zero was rounded by.  A division per value, and fp64 for the ties, were the bound of this kernel.
 #include "common.cuh"
 
 namespace ucmx {
@@ -69,6 +69,44 @@ __device__ __forceinline__ uint32_t min2(uint32_t a, uint32_t b)
     uint32_t r;
     asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
+}
+
+// two fp32 operations in one instruction
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
+{
+    F2 r;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b)
+{
+    F2 r;
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+
+// Settles a code whose residual is half a step or more.  c: the code so far; v, lo: the value and the row's smallest.
+__device__ __noinline__ float settle(float c, float v, float lo, float half_scale)
+{
+    const float a = 0.5f * v, b = -0.5f * lo, hx = a + b;
+    const float r = fmaf(-c, half_scale, hx);
+    if (fabsf(r) > 0.5f * half_scale) return r > 0.f ? c + 1.f : c - 1.f;
+    // a tie of the rounded difference: which side the exact one lies on (as far as fp64 would see it), else the even code
+    const float bb = hx - a;
+    const float err = (a - (hx - bb)) + (b - bb);
+    const float unit = __uint_as_float(__float_as_uint(hx) & 0x7f800000u) * 1.1102230246251565e-16f;     // 2^-53 of hx's power of two
+    const float low = r > 0.f ? c : c - 1.f;
+    if (err > unit) return low + 1.f;
+    if (err < -unit) return low;
+    return (int)low & 1 ? low + 1.f : low;
 }
 
 // byte offset of a lane's codes inside K's part of a group / of unit u (2 bytes of a row) inside V's part
@@ -155,9 +193,41 @@ __global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
     const int tt = t % kRows;
     const int group_step = (p.T / kRows) * X::kGroup;
     uint8_t* group = p.cache + block * p.block_stride + (int64_t)x.h * group_step + (t / kRows) * X::kGroup;
+    // ---- each row's range: (max x, max -x) in one register
+    uint32_t range[HC];
+#pragma unroll
+    for (int c = 0; c < HC; ++c) {
+        uint32_t hi2 = raw[c][0].x, lo2 = raw[c][0].x;
+#pragma unroll
+        for (int i = 0; i < X::kDims / 8; ++i) {
+            hi2 = max2(max2(max2(max2(hi2, raw[c][i].x), raw[c][i].y), raw[c][i].z), raw[c][i].w);
+            lo2 = min2(min2(min2(min2(lo2, raw[c][i].x), raw[c][i].y), raw[c][i].z), raw[c][i].w);
+        }
+        lo2 ^= 0x80008000u;
+        range[c] = max2(__byte_perm(hi2, lo2, 0x5410), __byte_perm(hi2, lo2, 0x7632));
+#pragma unroll
+        for (int o = 1; o < X::kLanes; o <<= 1) range[c] = max2(range[c], __shfl_xor_sync(0xffffffffu, range[c], o));
+    }
+    // ---- scale and zero: lane lr works them out for head lr % HC, the others fetch them
+    uint32_t my_sz;
+    float my_inv;
+    {
+        uint32_t r = range[0];
+#pragma unroll
+        for (int c = 1; c < HC; ++c)
+            if (lr % HC == c) r = range[c];
+        const float hi = bf16lo(r), lo = -bf16hi(r);
+        const bool bad = !((hi - hi) + (lo - lo) == 0.f);
+        my_sz = f32_to_bf16_bits(fmaf(0.5f, hi, -0.5f * lo) / (0.5f * (float)X::kTop)) | (__float_as_uint(lo) & 0xffff0000u);
+        if (bad) my_sz = 0x7fc07fc0u;
+        my_inv = __fdividef(1.f, 0.5f * bf16lo(my_sz));
+    }
 #pragma unroll
     for (int c = 0; c < HC; ++c, group += group_step) {
         if (x.h + c >= p.H) break;
+        const uint32_t sz = HC == 1 ? my_sz : __shfl_sync(0xffffffffu, my_sz, row * X::kLanes + c);
+        const float inv = HC == 1 ? my_inv : __shfl_sync(0xffffffffu, my_inv, row * X::kLanes + c);
+        const float scale = bf16lo(sz), half_scale = 0.5f * scale, lo = bf16hi(sz), half_lo = 0.5f * lo;
         uint32_t q[X::kDims / 2];
 #pragma unroll
         for (int i = 0; i < X::kDims / 8; ++i) {
@@ -166,45 +236,39 @@ __global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
             q[4 * i + 2] = raw[c][i].z;
             q[4 * i + 3] = raw[c][i].w;
         }
-        // ---- the row's range: (max x, max -x) in one register
-        uint32_t hi2 = q[0], lo2 = q[0];
-#pragma unroll
-        for (int i = 1; i < X::kDims / 2; ++i) {
-            hi2 = max2(hi2, q[i]);
-            lo2 = min2(lo2, q[i]);
-        }
-        lo2 ^= 0x80008000u;
-        uint32_t range = max2(__byte_perm(hi2, lo2, 0x5410), __byte_perm(hi2, lo2, 0x7632));
-#pragma unroll
-        for (int o = 1; o < X::kLanes; o <<= 1) range = max2(range, __shfl_xor_sync(0xffffffffu, range, o));
-        const float hi = bf16lo(range), lo = -bf16hi(range);
-        const bool bad = !((hi - hi) + (lo - lo) == 0.f);
-        const float half_lo = 0.5f * lo;
-        const uint32_t sb = bad ? 0x7fc0u : f32_to_bf16_bits(fmaf(0.5f, hi, -half_lo) / (0.5f * (float)X::kTop));
-        const uint32_t zb = bad ? 0x7fc0u : __float_as_uint(lo) >> 16;
-        const float scale = __uint_as_float(sb << 16), half_scale = 0.5f * scale;
         // ---- codes, as floats
         float f[X::kDims];
-        if (!bad && scale > 0.f) {
+        if (scale > 0.f) {                               // (not for a scale of 0, not for NaN)
             const bool tiny = scale < 1e-30f;            // the reciprocal would leave the range: everything in fp64
-            const float inv = __fdividef(1.f, half_scale), most = (float)X::kTop * half_scale;
+            const float most = (float)X::kTop * half_scale;
             const float half = 0.5f * half_scale;
             float worst = 0.f;
             float e[X::kDims];
 #pragma unroll
-            for (int i = 0; i < X::kDims; ++i) {
-                const float v = i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]);
-                const float hx = fminf(fmaf(v, 0.5f, -half_lo), most);
-                f[i] = fmaf(hx, inv, kMagic) - kMagic;
-                e[i] = fabsf(fmaf(-f[i], half_scale, hx));
-                worst = fmaxf(worst, e[i]);
+            for (int i = 0; i < X::kDims; i += 2) {
+                F2 hx = fma2({bf16lo(q[i / 2]), bf16hi(q[i / 2])}, {0.5f, 0.5f}, {-half_lo, -half_lo});
+                if (BITS == 8) {                         // 255 steps of a scale that was rounded down may end beyond 255.5; 15 cannot
+                    hx.x = fminf(hx.x, most);
+                    hx.y = fminf(hx.y, most);
+                }
+                const F2 c = add2(fma2(hx, {inv, inv}, {kMagic, kMagic}), {-kMagic, -kMagic});
+                const F2 r = fma2(c, {-half_scale, -half_scale}, hx);
+                f[i] = c.x;
+                f[i + 1] = c.y;
+                e[i] = fabsf(r.x);
+                e[i + 1] = fabsf(r.y);
+                worst = fmaxf(worst, fmaxf(e[i], e[i + 1]));
             }
-            if (tiny || worst >= half) {
+            if (tiny) {
 #pragma unroll
                 for (int i = 0; i < X::kDims; ++i) {
                     const float v = i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]);
-                    if (tiny || e[i] >= half) f[i] = (float)fmin(rint(((double)v - (double)lo) / (double)scale), (double)X::kTop);
+                    f[i] = (float)fmin(rint(((double)v - (double)lo) / (double)scale), (double)X::kTop);
                 }
+            } else if (worst >= half) {
+#pragma unroll
+                for (int i = 0; i < X::kDims; ++i)
+                    if (e[i] >= half) f[i] = settle(f[i], i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]), lo, half_scale);
             }
         } else {
 #pragma unroll
@@ -239,7 +303,7 @@ __global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
                 const uint32_t y = __shfl_xor_sync(0xffffffffu, w[i], X::kLanes);
                 const int u = (lr * X::kWords + i) * 2;
                 if (paired) {
-                    const uint32_t z = (row & 1) ? __byte_perm(y, w[i], 0x7632) : __byte_perm(w[i], y, 0x5410);
+                    const uint32_t z = __byte_perm(w[i], y, (row & 1) ? 0x3276 : 0x5410);
                     *reinterpret_cast<uint32_t*>(part + v_at<BITS, D>(tt & ~1, u + (row & 1))) = z;
                 } else if (live) {
                     *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u)) = (uint16_t)w[i];
@@ -248,7 +312,7 @@ __global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
             }
         }
         if (live && lr == 0)
-            *reinterpret_cast<uint32_t*>(group + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4) = sb | (zb << 16);
+            *reinterpret_cast<uint32_t*>(group + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4) = sz;
     }
 }
 

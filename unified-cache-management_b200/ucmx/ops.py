@@ -541,18 +541,50 @@ class QuantKvCache:
         return int(N.lib.ucmx_quant_block_bytes(C.byref(self.geometry)))
 
 
-def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]):
-    """All tensors on the device of `first`, made current for the launch where it is not."""
+class _on_device:
+    """Makes the device of `t` current for a launch where it is not (nothing at all in the usual case)."""
+    __slots__ = ("index", "guard")
+
+    def __init__(self, t: torch.Tensor):
+        self.index, self.guard = t.device.index, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.index:
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _need_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """CUDA tensors, all of them on one device."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("ucmx ops take CUDA tensors; there is no CPU path")
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError("all tensors of a call must be on the same device")
-    return torch.cuda.device(first.device)
+        if t is not None and t.device != dev:
+            raise ValueError("all tensors of a call must be on the same CUDA device")
+
+
+def _index(t: Optional[torch.Tensor], name: str, dev: torch.device, n: int = -1) -> int:
+    """Address of a contiguous int32 tensor of n entries on `dev`; 0 for None."""
+    if t is None:
+        return 0
+    if t.dtype is not torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor")
+    if t.device != dev:
+        raise ValueError("all tensors of a call must be on the same CUDA device")
+    if n >= 0 and t.numel() != n:
+        raise ValueError(f"{name} must hold {n} entries")
+    return t.data_ptr()
 
 
 def quant_write_tokens(cache: QuantKvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantise the K and V rows of new tokens into the cache: k, v bf16 [n, n_kv_heads, head_dim] (rows of a wider tensor are
     fine), slots int64 [n] = block * block_tokens + token, all different; a negative slot skips its token."""
-    _need_cuda(cache.data, k, v, slots)
+    _need_device(cache.data, k, v, slots)
     g = cache.geometry
     n = slots.numel()
     for x in (k, v):
@@ -560,7 +592,7 @@ def quant_write_tokens(cache: QuantKvCache, k: torch.Tensor, v: torch.Tensor, sl
             raise ValueError("k and v must be bf16 [n, n_kv_heads, head_dim] with contiguous heads")
     if slots.dtype != torch.int64 or not slots.is_contiguous():
         raise ValueError("slots must be contiguous int64")
-    with _same_device(cache.data, k, v, slots):
+    with _on_device(cache.data):
         strides = [x.stride(0) if n > 1 else g.n_kv_heads * g.head_dim for x in (k, v)]
         st = N.lib.ucmx_quant_write_tokens(_ptr(k), _ptr(v), strides[0], strides[1], n, _ptr(slots), _ptr(cache.data), C.byref(g),
                                            _stream(cache.data))
@@ -570,12 +602,12 @@ def quant_write_tokens(cache: QuantKvCache, k: torch.Tensor, v: torch.Tensor, sl
 def quant_write_blocks(cache: QuantKvCache, k_cache: torch.Tensor, v_cache: torch.Tensor, block_ids: torch.Tensor, *,
                        out_slots: Optional[torch.Tensor] = None) -> None:
     """Quantise blocks block_ids[i] of a bf16 paged cache into block out_slots[i] (or i) of the quantised one."""
-    _need_cuda(cache.data, k_cache, v_cache, block_ids, out_slots)
+    _need_device(cache.data, k_cache, v_cache, block_ids, out_slots)
     ids = _i32(block_ids, "block_ids")
     n = ids.numel()
     if out_slots is not None and out_slots.numel() != n:
         raise ValueError("one out_slots entry per block id")
-    with _same_device(cache.data, k_cache, v_cache, block_ids, out_slots):
+    with _on_device(cache.data):
         st = N.lib.ucmx_quant_write_blocks(_ptr(k_cache), C.byref(kv_geometry(k_cache)), _ptr(v_cache), C.byref(kv_geometry(v_cache)),
                                            _ptr(ids), _ptr(_i32(out_slots, "out_slots")), n, _ptr(cache.data), C.byref(cache.geometry),
                                            _stream(cache.data))
@@ -586,7 +618,7 @@ def quant_read_blocks(cache: QuantKvCache, block_ids: torch.Tensor, *, k_out: Op
                       v_out: Optional[torch.Tensor] = None, out_slots: Optional[torch.Tensor] = None):
     """Blocks block_ids[i] of the quantised cache -> block out_slots[i] (or i) of bf16 paged caches, which are allocated
     ([n, block_tokens, n_kv_heads, head_dim]) where none are given.  Returns (k_out, v_out)."""
-    _need_cuda(cache.data, block_ids, k_out, v_out, out_slots)
+    _need_device(cache.data, block_ids, k_out, v_out, out_slots)
     g = cache.geometry
     ids = _i32(block_ids, "block_ids")
     n = ids.numel()
@@ -597,65 +629,73 @@ def quant_read_blocks(cache: QuantKvCache, block_ids: torch.Tensor, *, k_out: Op
     if k_out is None:
         k_out, v_out = (torch.zeros((n, g.block_tokens, g.n_kv_heads, g.head_dim), dtype=torch.bfloat16, device=cache.data.device)
                         for _ in range(2))
-    with _same_device(cache.data, block_ids, k_out, v_out, out_slots):
+    with _on_device(cache.data):
         st = N.lib.ucmx_quant_read_blocks(_ptr(cache.data), C.byref(g), _ptr(ids), _ptr(_i32(out_slots, "out_slots")), n, _ptr(k_out),
                                           C.byref(kv_geometry(k_out)), _ptr(v_out), C.byref(kv_geometry(v_out)), _stream(cache.data))
     N.check("ucmx_quant_read_blocks", st, 1 if n else 0)
     return k_out, v_out
 
 
+_workspace_bytes = {}     # (device, bits, query heads, KV heads, head_dim, query tokens) -> bytes
+
+
 def attention_workspace(query: torch.Tensor, n_kv_heads: int, *, max_q_tokens: int = 1, bits: int = 16) -> torch.Tensor:
     """Scratch for block_attention (bits 16) or quant_block_attention (bits of the cache) with queries of this shape, whatever the
     lists; to be kept where the calls must not allocate.  Calls that may overlap need one each."""
-    with torch.cuda.device(query.device):
-        need = int(N.lib.ucmx_attention_workspace_bytes(bits, query.shape[1], n_kv_heads, query.shape[2], max_q_tokens))
-    if need == 0:
-        raise ValueError("unsupported attention shape: head_dim 64, 128 or 256, query heads a multiple of the KV heads")
-    return torch.empty((need,), dtype=torch.uint8, device=query.device)
+    key = (query.device.index, bits, query.shape[1], n_kv_heads, query.shape[2], max_q_tokens)
+    need = _workspace_bytes.get(key)
+    if need is None:
+        with _on_device(query):
+            need = int(N.lib.ucmx_attention_workspace_bytes(*key[1:]))
+        if need == 0:
+            raise ValueError("unsupported attention shape: head_dim 64, 128 or 256, query heads a multiple of the KV heads")
+        _workspace_bytes[key] = need
+    return torch.empty(need, dtype=torch.uint8, device=query.device)
 
 
-def _attend(name: str, bits: int, n_kv_heads: int, head_dim: int, cache_args, caches, query, req_offsets, block_ids, positions,
+def _attend(name: str, fn, bits: int, n_kv_heads: int, head_dim: int, cache_args, cache, query, req_offsets, block_ids, positions,
             block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out, lse, workspace):
-    _need_cuda(query, req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, out, lse,
-               workspace, *caches)
-    if query.dim() != 3 or query.dtype != torch.bfloat16 or query.shape[2] != head_dim:
+    _need_device(query, cache, out, lse, workspace)
+    dev = query.device
+    if query.dim() != 3 or query.dtype is not torch.bfloat16 or query.shape[2] != head_dim:
         raise ValueError(f"query must be bf16 [n_query_tokens, n_q_heads, {head_dim}]")
     n_tok, Hq, D = query.shape
-    if query.stride()[1:] != (D, 1) or (n_tok > 1 and query.stride(0) % 8):
-        query = query.contiguous()
+    q_stride, sh, sd = query.stride()
+    if n_tok == 1:
+        q_stride = Hq * D
+    if sd != 1 or sh != D or q_stride % 8 or q_stride < Hq * D or query.data_ptr() % 16:
+        query = query.clone(memory_format=torch.contiguous_format)
+        q_stride = Hq * D
     n_req = req_offsets.numel() - 1
     if n_req < 0:
         raise ValueError("req_offsets must hold n_req + 1 entries")
+    entries = positions if block_ids is None else block_ids
     if block_ids is None and (positions is None or block_table is None or table_offsets is None):
         raise ValueError("give block_ids, or positions with block_table and table_offsets")
-    if block_ids is not None and block_table is not None:
-        raise ValueError("give block_ids or block_table, not both")
-    entries = block_ids if block_ids is not None else positions
-    for t, n, what in ((block_ids, entries.numel(), "block_ids"), (positions, entries.numel(), "positions"), (req_counts, n_req, "req_counts"),
-                       (ctx_lens, n_req, "ctx_lens"), (q_offsets, n_req + 1, "q_offsets"), (table_offsets, n_req + 1, "table_offsets")):
-        if t is not None and t.numel() != n:
-            raise ValueError(f"{what} must hold {n} entries")
+    if block_ids is not None and (block_table is not None or table_offsets is not None):
+        raise ValueError("give block_ids or block_table with table_offsets, not both")
+    total = entries.numel()
+    lists = N.BlockLists(_index(req_offsets, "req_offsets", dev), _index(req_counts, "req_counts", dev, n_req),
+                         _index(block_ids, "block_ids", dev, total), _index(positions, "positions", dev, total),
+                         _index(block_table, "block_table", dev), _index(table_offsets, "table_offsets", dev, n_req + 1),
+                         _index(ctx_lens, "ctx_lens", dev, n_req), n_req, total)
+    q_off = _index(q_offsets, "q_offsets", dev, n_req + 1)
     if q_offsets is None and (n_tok != n_req or max_q_tokens != 1):
         raise ValueError("without q_offsets there is one query token per request")
     if out is None:
-        out = torch.empty((n_tok, Hq, D), dtype=torch.bfloat16, device=query.device)
-    elif out.dtype != torch.bfloat16 or not out.is_contiguous() or tuple(out.shape) != (n_tok, Hq, D):
+        out = torch.empty((n_tok, Hq, D), dtype=torch.bfloat16, device=dev)
+    elif out.dtype is not torch.bfloat16 or not out.is_contiguous() or tuple(out.shape) != (n_tok, Hq, D):
         raise ValueError("out must be contiguous bf16 of the query's shape")
-    if lse is not None and (lse.dtype != torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (n_tok, Hq)):
+    if lse is not None and (lse.dtype is not torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (n_tok, Hq)):
         raise ValueError("lse must be contiguous fp32 [n_query_tokens, n_q_heads]")
     if n_req == 0 or n_tok == 0:
         return out
-    with _same_device(query, req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, out, lse,
-                      workspace, *caches):
-        if workspace is None:
-            workspace = attention_workspace(query, n_kv_heads, max_q_tokens=max_q_tokens, bits=bits)
-        adr = lambda t, what: 0 if t is None else _i32(t, what).data_ptr()  # noqa: E731
-        lists = N.BlockLists(adr(req_offsets, "req_offsets"), adr(req_counts, "req_counts"), adr(block_ids, "block_ids"),
-                             adr(positions, "positions"), adr(block_table, "block_table"), adr(table_offsets, "table_offsets"),
-                             adr(ctx_lens, "ctx_lens"), n_req, entries.numel())
-        st = getattr(N.lib, name)(_ptr(query), query.stride(0) if n_tok > 1 else Hq * D, Hq, _ptr(_i32(q_offsets, "q_offsets")), n_tok,
-                                  max_q_tokens, *cache_args, C.byref(lists), float(D ** -0.5 if scale is None else scale), _ptr(out),
-                                  _ptr(lse), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(query))
+    if workspace is None:
+        workspace = attention_workspace(query, n_kv_heads, max_q_tokens=max_q_tokens, bits=bits)
+    with _on_device(query):
+        st = fn(query.data_ptr(), q_stride, Hq, q_off, n_tok, max_q_tokens, *cache_args, C.byref(lists),
+                D ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(),
+                workspace.nbytes, torch.cuda.current_stream(dev).cuda_stream)
     N.check(name, st, 2)
     return out
 
@@ -679,8 +719,10 @@ def block_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     q_offsets, max_q_tokens: each request's query tokens (one each without).  A query that sees nothing gives zeros.
     lse: fp32 [n_query_tokens, n_q_heads], receives the logarithm of the softmax's sum.  scale defaults to head_dim ** -0.5."""
     kg, vg = kv_geometry(k_cache), kv_geometry(v_cache)
-    args = (_ptr(k_cache), C.byref(kg), _ptr(v_cache), C.byref(vg))
-    return _attend("ucmx_block_attention", 16, kg.n_kv_heads, kg.head_dim, args, (k_cache, v_cache), query, req_offsets, block_ids, positions,
+    if v_cache.device != k_cache.device:
+        raise ValueError("all tensors of a call must be on the same CUDA device")
+    args = (k_cache.data_ptr(), C.byref(kg), v_cache.data_ptr(), C.byref(vg))
+    return _attend("ucmx_block_attention", N.lib.ucmx_block_attention, 16, kg.n_kv_heads, kg.head_dim, args, k_cache, query, req_offsets, block_ids, positions,
                    block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out, lse, workspace)
 
 
@@ -693,6 +735,6 @@ def quant_block_attention(query: torch.Tensor, cache: QuantKvCache, req_offsets:
                           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """block_attention over a quantised cache: the codes are read in place and never written out as bf16."""
     g = cache.geometry
-    return _attend("ucmx_quant_block_attention", g.bits, g.n_kv_heads, g.head_dim, (_ptr(cache.data), C.byref(g)), (cache.data,), query,
-                   req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out,
+    return _attend("ucmx_quant_block_attention", N.lib.ucmx_quant_block_attention, g.bits, g.n_kv_heads, g.head_dim,
+                   (cache.data.data_ptr(), C.byref(g)), cache.data, query, req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out,
                    lse, workspace)
