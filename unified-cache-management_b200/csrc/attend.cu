@@ -58,6 +58,8 @@ int32_t run_any(int bits, const Params& p, int head_dim, int cols, const Maps* m
                       : run_q4(p, head_dim, cols, maps, plan, st);
 }
 
+size_t plan_bytes(const Plan& plan) { return (size_t)plan.ctas * (2 * plan.part * sizeof(float) + sizeof(Rec)); }
+
 // what both entries check and fill in; the cache's part of `p` is set by the caller
 int32_t attend_common(Params& p, int bits, int32_t head_dim, const void* q, int64_t q_stride, int32_t n_q_heads, int32_t n_kv_heads,
                       const int32_t* q_offsets, int32_t n_q_tokens, int32_t max_q_tokens, const ucmx_block_lists* l, float scale,
@@ -102,7 +104,7 @@ int32_t attend_common(Params& p, int bits, int32_t head_dim, const void* q, int6
     Plan plan;
     const int32_t rc = run_any(bits, p, head_dim, cols, nullptr, &plan, nullptr);
     if (rc != UCMX_OK) return refuse("attention: head_dim must be 64, 128 or 256", rc);
-    if (workspace_bytes < (size_t)plan.ctas * 2 * plan.part * sizeof(float)) return refuse("attention: workspace too small");
+    if (workspace_bytes < plan_bytes(plan)) return refuse("attention: workspace too small");
     p.cols_per_tile = plan.cols;
     p.col_tiles = (cols + plan.cols - 1) / plan.cols;
     // the slices of all requests, heads and tiles are numbered in 32 bits
@@ -132,7 +134,7 @@ extern "C" size_t ucmx_attention_workspace_bytes(int32_t bits, int32_t n_q_heads
     Params p = {};
     const int64_t cols = (int64_t)max_q_tokens * (n_q_heads / n_kv_heads);
     if (run_any(bits, p, head_dim, cols > 64 ? 64 : (int)cols, nullptr, &plan, nullptr) != UCMX_OK) return 0;
-    return (size_t)plan.ctas * 2 * plan.part * sizeof(float);
+    return plan_bytes(plan);
 }
 
 extern "C" int32_t ucmx_block_attention(const void* q, int64_t q_stride, int32_t n_q_heads, const int32_t* q_offsets, int32_t n_q_tokens,

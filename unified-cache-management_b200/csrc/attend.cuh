@@ -11,9 +11,10 @@
 //
 // Split.  The unit is a slice: up to 16 consecutive tokens of one listed block.  All slices of all (request, KV head,
 // column tile) items are laid end to end and cut into equal parts, one per thread block, whatever the lengths of the
-// requests are; an item that crosses cuts leaves partial results (running maximum, sum, unnormalised output) in the
-// workspace, which a second small kernel joins in order.  The workspace needs no initial state, and the order of the
-// sums is fixed by the shapes, so results do not change from run to run.
+// requests are.  A short item stays with the thread block that it begins in; a longer one that crosses cuts leaves partial
+// results (running maximum, sum, unnormalised output) in the workspace, which a second small kernel joins in order.  The
+// workspace needs no initial state, and the order of the sums is fixed by the shapes, so results do not change from run to
+// run.
 //
 // Within a thread block each of the four warps takes every fourth slice with a ring of its own: one lane per row starts
 // an asynchronous bulk copy, the warp waits on its own barrier, no other warp is involved until the item ends.
@@ -68,13 +69,20 @@ struct Params {
     float scale_log2;
     uint16_t* out;                     // [n_q_tokens, Hq, D]
     float* lse;                        // [n_q_tokens, Hq] or NULL
-    float* ws;                         // partial results: 2 per thread block
+    float* ws;                         // partial results: 2 per thread block, then a Rec per thread block
     int32_t* err;
 };
 
 // K and V of the bf16 cache as tensors [block][token][head][value]; unused for the quantised cache.
 struct Maps {
     CUtensorMap k, v;
+};
+
+// What a thread block tells the joining kernel about the item that begins in its range and goes on behind it.
+struct __align__(32) Rec {
+    int32_t parts;                     // 0: there is none
+    int32_t q0, c0, cols, h;
+    int32_t pad[3];
 };
 
 // One item's part inside a thread block's range.
@@ -86,50 +94,41 @@ struct Seg {
     int32_t n;                         // entries of the request's list
 };
 
-// The last r with offsets[r] <= e (a warp probes 32 places at a time).  All lanes get it.
-__device__ __forceinline__ int request_of(const int32_t* __restrict__ offsets, int n_req, int32_t e)
+constexpr int kWhole = 32;             // items up to this many slices are not split (nor up to an eighth of a thread block's share)
+constexpr int kMaxScan = 1023;         // requests whose column tiles are counted exactly
+
+// How the slices are shared out.  `start` holds the requests' beginnings in order: the lists' offsets, each entry counting for
+// every column tile there may be; or, with several tiles, the exact sums of entries x tiles of each request (built in shared
+// memory: the tiles of a request depend on its number of query tokens).
+struct Share {
+    const int32_t* start;
+    int32_t per;                       // slices of one entry of `start`
+    int32_t tiles;                     // 0: exact
+    int32_t all, size, lo, hi;         // all slices; a thread block's share; this one's
+    int32_t whole;
+    int32_t step;                      // the first level of the search: every step-th entry of `start`,
+    const int32_t* probes;             // 32 of them in shared memory
+};
+
+// The last r with start[r] <= e, and start[r], start[r+1]; 31 intervals a step, the first of them at hand.
+__device__ __forceinline__ int request_of(const Share& w, int n_req, int32_t e, int32_t& first, int32_t& next)
 {
     const int lane = threadIdx.x & 31;
-    int lo = 0, n = n_req;
-    while (n > 1) {
-        const int step = (n + 31) >> 5;
-        const int at = lo + lane * step;
-        const bool below = lane * step < n && __ldg(offsets + at) <= e;
-        const int c = __popc(__ballot_sync(0xffffffffu, below));
+    int lo = 0, n = n_req, step = w.step;
+    int32_t v = w.probes[lane];
+    for (;;) {
+        const int c = __popc(__ballot_sync(0xffffffffu, lane * step < n && v <= e));
         const int adv = (c > 0 ? c - 1 : 0) * step;
+        if (step == 1) {
+            first = __shfl_sync(0xffffffffu, v, c > 0 ? c - 1 : 0);
+            next = __shfl_sync(0xffffffffu, v, c > 0 ? c : 1);
+            return lo + adv;
+        }
         lo += adv;
         n = min(step, n - adv);
+        step = (n + 30) / 31;
+        v = w.start[lo + min(lane * step, n)];
     }
-    return lo;
-}
-
-__device__ __forceinline__ int32_t entries_total(const Params& p)
-{
-    const int32_t n = __ldg(p.offsets + p.n_req);      // a captured batch may use less than its capacity
-    return n < 0 ? 0 : n < p.total ? n : p.total;
-}
-__device__ __forceinline__ int32_t slices_per_entry(const Params& p) { return p.spe * p.H * p.col_tiles; }
-
-// Part c of n equal parts begins at min(all, c * ceil(all / n)).  (The host keeps all + n below 2^31.)
-__device__ __forceinline__ int32_t part_size(int32_t all, int32_t n) { return (int32_t)(((uint32_t)all + (uint32_t)n - 1u) / (uint32_t)n); }
-
-// The item that holds position `at` (< hi); called by whole warps.
-__device__ __forceinline__ Seg segment_at(const Params& p, int32_t at, int32_t hi)
-{
-    Seg s;
-    const int32_t spe = slices_per_entry(p);
-    s.r = request_of(p.offsets, p.n_req, at / spe);
-    s.first = __ldg(p.offsets + s.r);
-    s.n = min(__ldg(p.offsets + s.r + 1), p.total) - s.first;
-    const int32_t item = s.n * p.spe;                  // slices of one (KV head, column tile)
-    const int32_t i = (at - s.first * spe) / item;
-    s.h = i / p.col_tiles;
-    s.ct = i - s.h * p.col_tiles;
-    s.begin = s.first * spe + i * item;
-    s.end = s.begin + item;
-    s.lo = at;
-    s.hi = s.end < hi ? s.end : hi;
-    return s;
 }
 
 // Query rows of request r: first row and how many (clamped to the query tensor and to max_q).
@@ -146,6 +145,34 @@ __device__ __forceinline__ void queries_of(const Params& p, int r, int& q0, int&
         if (p.err && threadIdx.x == 0) atomicExch(p.err, 3);
         nq = q0 < 0 || q0 >= p.n_q_tokens ? 0 : max(0, min(min(nq, p.max_q), p.n_q_tokens - q0));
     }
+}
+
+// The item that holds position `at` (below w.hi) and this thread block's part of it; called by whole warps.
+template <int COLS>
+__device__ __forceinline__ Seg segment_at(const Params& p, const Share& w, int32_t at)
+{
+    Seg s;
+    int32_t a, b, tiles = w.tiles;
+    s.r = request_of(w, p.n_req, at / w.per, a, b);
+    if (tiles == 0) {
+        int q0, nq;
+        queries_of(p, s.r, q0, nq);
+        tiles = max(1, (nq * p.G + COLS - 1) / COLS);
+        s.first = __ldg(p.offsets + s.r);
+        s.n = (b - a) / tiles;
+    } else {
+        s.first = a;
+        s.n = min(b, p.total) - a;
+    }
+    const int32_t item = s.n * p.spe;                  // slices of one (KV head, column tile)
+    const int32_t i = (at - a * w.per) / item;
+    s.h = i / tiles;
+    s.ct = i - s.h * tiles;
+    s.begin = a * w.per + i * item;
+    s.end = s.begin + item;
+    s.lo = at;
+    s.hi = item <= w.whole || s.end < w.hi ? s.end : w.hi;
+    return s;
 }
 
 // 2^x for a weight: x is at most kMaxSlack, and what is below 2^-126 of the largest weight is nothing
@@ -326,15 +353,17 @@ struct Traits {
     static constexpr int kMTiles = D / 16;
     static constexpr bool kQReg = kKSteps * NT <= 16;    // query fragments in registers (else in shared memory)
     static constexpr int kMergeLd = D + 4;
-    static constexpr int kMergeCols = 4;                 // columns joined at a time
-    static constexpr int kMergeSteps = DUP ? 1 : 2 * NT;
+    static constexpr int kMergeCols = D <= 128 && NT > 1 ? 8 : 4;         // columns joined at a time
+    static constexpr int kMergeSteps = kCols / kMergeCols;
     static constexpr int kRingBytes = kWarps * kStages * L::kStage;
     static constexpr int kMergeBytes = kWarps * kMergeCols * kMergeLd * 4;
     static constexpr int kStatBytes = kWarps * kCols * 3 * 4;
+    static constexpr bool kTiled = NT == 4 || (D == 256 && NT == 2);      // the widest tile: requests may need several
+    static constexpr int kScanBytes = kTiled ? (kMaxScan + 1) * 4 : 0;
     static constexpr int kQBytes = kQReg ? 0 : kKSteps * NT * 32 * 8;
-    static constexpr int kBarStride = kStages * (8 + 8 * L::kUnits);     // a warp's barriers, and a note (8) per slice
+    static constexpr int kBarStride = kStages * (8 + 8 * L::kUnits) + 128;    // a warp's barriers, a note (8) per slice, 32 probes
     static constexpr int kBarBytes = kWarps * kBarStride;
-    static constexpr int kSmem = 1024 + kRingBytes + kMergeBytes + kStatBytes + kQBytes + kBarBytes;   // (1024: alignment)
+    static constexpr int kSmem = 1024 + kRingBytes + kMergeBytes + kStatBytes + kQBytes + kScanBytes + kBarBytes;   // (1024: alignment)
     static constexpr int kPart = kCols * (D + 2);        // floats of a partial result: m, l, then the rows
     // thread blocks per SM: what shared memory holds (228 KB, 1 KB of it per block), and the registers of the accumulators
     static constexpr int kBySmem = 233472 / (kSmem + 1024);
@@ -356,7 +385,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     float* const merge = reinterpret_cast<float*>(smem + X::kRingBytes);
     float* const stat = reinterpret_cast<float*>(smem + X::kRingBytes + X::kMergeBytes);     // [warp][3][cols]
     uint2* const q_frag = reinterpret_cast<uint2*>(smem + X::kRingBytes + X::kMergeBytes + X::kStatBytes);
-    unsigned char* const bars = smem + X::kRingBytes + X::kMergeBytes + X::kStatBytes + X::kQBytes + warp * X::kBarStride;
+    int32_t* const scan = reinterpret_cast<int32_t*>(smem + X::kRingBytes + X::kMergeBytes + X::kStatBytes + X::kQBytes);
+    unsigned char* const bars = reinterpret_cast<unsigned char*>(scan) + X::kScanBytes + warp * X::kBarStride;
     uint64_t* const full = reinterpret_cast<uint64_t*>(bars);
     int2* const note = reinterpret_cast<int2*>(bars + 8 * X::kStages);    // .x tokens copied (0: nothing), .y first position
 
@@ -366,22 +396,68 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     }
     __syncwarp();
 
-    const int32_t all = entries_total(p) * slices_per_entry(p);
-    const int32_t size = part_size(all, gridDim.x);
-    const int32_t lo = min(all, (int32_t)blockIdx.x * size), hi = lo + min(size, all - lo);
     early_start_allow();
 
-    // requests that list nothing have no slices: their rows are written here
-    for (int r = blockIdx.x; r < p.n_req; r += gridDim.x) {
-        if (__ldg(p.offsets + r + 1) > __ldg(p.offsets + r) && __ldg(p.offsets + r) < p.total) continue;
-        int q0, nq;
-        queries_of(p, r, q0, nq);
-        for (int64_t i = tid; i < (int64_t)nq * p.Hq * (D / 2); i += kThreads)
-            reinterpret_cast<uint32_t*>(p.out)[(int64_t)q0 * p.Hq * (D / 2) + i] = 0u;
-        if (p.lse)
-            for (int i = tid; i < nq * p.Hq; i += kThreads) p.lse[(int64_t)q0 * p.Hq + i] = -INFINITY;
+    // ---- this thread block's share
+    Share w;
+    w.start = p.offsets;
+    w.tiles = p.col_tiles;
+    w.per = p.spe * p.H * p.col_tiles;
+    if (X::kTiled && p.col_tiles > 1 && p.n_req <= kMaxScan) {
+        constexpr int kEach = (kMaxScan + kThreads) / kThreads;
+        int32_t v[kEach], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int r = tid * kEach + i;
+            v[i] = 0;
+            if (r < p.n_req) {
+                int q0, nq;
+                queries_of(p, r, q0, nq);
+                v[i] = max(0, min(__ldg(p.offsets + r + 1), p.total) - __ldg(p.offsets + r)) * ((nq * p.G + X::kCols - 1) / X::kCols);
+            }
+            sum += v[i];
+        }
+        int32_t before = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t y = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += y;
+        }
+        int32_t* const warp_sum = reinterpret_cast<int32_t*>(stat);
+        if (lane == 31) warp_sum[warp] = before;
+        __syncthreads();
+        before -= sum;
+        for (int i = 0; i < warp; ++i) before += warp_sum[i];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int r = tid * kEach + i;
+            if (r <= p.n_req) scan[r] = before;
+            before += v[i];
+        }
+        __syncthreads();
+        w.start = scan;
+        w.tiles = 0;
+        w.per = p.spe * p.H;
     }
-    if (lo >= hi) return;
+    w.step = (p.n_req + 30) / 31;
+    int32_t* const probes = reinterpret_cast<int32_t*>(note + X::kStages * L::kUnits);
+    const int32_t probe = w.start[min(lane * w.step, p.n_req)];
+    probes[lane] = probe;
+    __syncwarp();
+    w.probes = probes;
+    const int32_t entries = __shfl_sync(0xffffffffu, probe, 31);          // a captured batch may use less than its capacity
+    w.all = (w.tiles == 0 ? entries : max(0, min(entries, p.total))) * w.per;
+    w.size = (int32_t)(((uint32_t)w.all + gridDim.x - 1u) / gridDim.x);   // (the host keeps all + grid below 2^31)
+    w.lo = min(w.all, (int32_t)blockIdx.x * w.size);
+    w.hi = w.lo + min(w.size, w.all - w.lo);
+    w.whole = max(kWhole, w.size / 8);
+    int32_t begin = w.lo;
+    if (begin < w.hi) {
+        const Seg s = segment_at<X::kCols>(p, w, begin);
+        if (s.begin < begin && s.end - s.begin <= w.whole) begin = s.end;     // the thread block before takes all of it
+    }
+    Rec* const rec = reinterpret_cast<Rec*>(p.ws + (int64_t)2 * gridDim.x * X::kPart) + blockIdx.x;
+    if (tid == 0) rec->parts = 0;
 
     // ---- the warp's loads run ahead of its arithmetic, across items: a cursor of their own
     constexpr int kU = L::kUnits, kStep = kWarps * kU;
@@ -398,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     const uint8_t* my_src = nullptr;
     uint32_t my_flags = 0;
     bool p_done = false;
-    int32_t p_next = lo;               // where the next segment begins
+    int32_t p_next = begin;            // where the next segment begins
     uint32_t plain = 0;                // bit s: the step in stage s needs no masks
     // what this lane has to know of slice `at` of segment ps
     auto look_up = [&](int32_t at) {
@@ -406,14 +482,10 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         if (at >= ps.hi) return;
         const int32_t s = at - ps.begin;
         const int32_t e = s / p.spe, sub = (s - e * p.spe) * kRows;
-        if (e >= p_entries) return;
-        const int32_t at_list = ps.first + e;
-        const int32_t pos_block = p.positions ? __ldg(p.positions + at_list) : e;
-        if (pos_block < 0) return;
-        int32_t id;
-        if (p.block_ids) {
-            id = __ldg(p.block_ids + at_list);
-        } else {
+        const int32_t pos_block = p.positions ? __ldg(p.positions + ps.first + e) : e;
+        int32_t id = p.block_ids ? __ldg(p.block_ids + ps.first + e) : -1;
+        if (e >= p_entries || pos_block < 0) return;
+        if (!p.block_ids) {
             const int32_t t0 = __ldg(p.table_offsets + ps.r), t1 = __ldg(p.table_offsets + ps.r + 1);
             if (pos_block >= t1 - t0) {
                 if (p.err) atomicExch(p.err, 3);
@@ -447,11 +519,11 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     auto issue = [&](int s) {
         if (p_at >= ps.hi) {
             while (!p_done && p_at >= ps.hi) {
-                if (p_next >= hi) {
+                if (p_next >= w.hi) {
                     p_done = true;
                     break;
                 }
-                ps = segment_at(p, p_next, hi);
+                ps = segment_at<X::kCols>(p, w, p_next);
                 p_next = ps.hi;
                 p_at = ps.lo + warp * kU;
                 p_look = 32;
@@ -529,10 +601,10 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     bool dead = false;
     const uint32_t ring_u = smem_u32(ring);
 
-    int32_t at = lo;
+    int32_t at = begin;
 #pragma unroll 1
-    while (at < hi) {
-        const Seg sg = segment_at(p, at, hi);
+    while (at < w.hi) {
+        const Seg sg = segment_at<X::kCols>(p, w, at);
         at = sg.hi;
         int q0, nq;
         queries_of(p, sg.r, q0, nq);
@@ -1015,54 +1087,62 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                 }
             }
         const bool whole = sg.lo == sg.begin && sg.hi == sg.end;
+        if (tid == 0 && sg.lo == sg.begin && sg.hi < sg.end)
+            *rec = Rec{(sg.end - 1) / w.size - (int32_t)blockIdx.x + 1, q0, c0, cols, sg.h, {0, 0, 0}};
         float* const part = p.ws + (int64_t)(2 * blockIdx.x + (sg.lo == sg.begin ? 1 : 0)) * X::kPart;
 #pragma unroll
         for (int step = 0; step < X::kMergeSteps; ++step) {
             if (step) __syncthreads();
 #pragma unroll
-            for (int k = 0; k < NT; ++k) {
-                if (k != step >> 1) continue;
+            for (int nt = 0; nt < NT; ++nt) {
+                if (nt != step * X::kMergeCols / 8) continue;
 #pragma unroll
                 for (int mt = 0; mt < X::kMTiles; ++mt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float x = o[mt][k][i];
+                        float x = o[mt][nt][i];
                         if (DUP) x += __shfl_xor_sync(0xffffffffu, x, 2);
                         const int row = i >> 1;                  // rows g and g + 8 of the tile
                         const int d = FMT == 16 ? mt * 16 + g + row * 8
                                                 : (mt / (L::kPanelDims / 16)) * L::kPanelDims + g * (L::kPanelDims / 8) +
                                                       (mt % (L::kPanelDims / 16)) * 2 + row;
-                        if ((q4 >> 1) == (step & 1)) merge[(warp * X::kMergeCols + ((2 * q4 + (i & 1)) & 3)) * X::kMergeLd + d] = x;
+                        if (X::kMergeCols == 8 || (q4 >> 1) == (step & 1))
+                            merge[(warp * X::kMergeCols + (2 * q4 + (i & 1)) % X::kMergeCols) * X::kMergeLd + d] = x;
                     }
             }
             __syncthreads();
-            for (int i = tid; i < X::kMergeCols * (D / 2); i += kThreads) {
-                const int cl = i / (D / 2), d = (i - cl * (D / 2)) * 2, cc = step * 4 + cl;
+            for (int i = tid; i < X::kMergeCols * (D / 4); i += kThreads) {
+                const int cl = i / (D / 4), d = (i - cl * (D / 4)) * 4, cc = step * X::kMergeCols + cl;
                 if (cc >= cols) continue;
                 float mw[kWarps], top = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, mw[w] = stat[(w * 3) * X::kCols + cc]);
+                for (int k = 0; k < kWarps; ++k) top = fmaxf(top, mw[k] = stat[(k * 3) * X::kCols + cc]);
                 const float off = top == -INFINITY ? 0.f : top;
-                float sum = 0.f, zero = 0.f, a = 0.f, b = 0.f;
+                float sum = 0.f, zero = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float f = exp2_fast(mw[w] - off);
-                    const float* const row = merge + (w * X::kMergeCols + cl) * X::kMergeLd + d;
-                    sum += f * stat[(w * 3 + 1) * X::kCols + cc];
-                    if (FMT != 16) zero += f * stat[(w * 3 + 2) * X::kCols + cc];
-                    a += f * row[0];
-                    b += f * row[1];
+                for (int k = 0; k < kWarps; ++k) {
+                    const float f = exp2_fast(mw[k] - off);
+                    const float4 x = *reinterpret_cast<const float4*>(merge + (k * X::kMergeCols + cl) * X::kMergeLd + d);
+                    sum = fmaf(f, stat[(k * 3 + 1) * X::kCols + cc], sum);
+                    if (FMT != 16) zero = fmaf(f, stat[(k * 3 + 2) * X::kCols + cc], zero);
+                    a[0] = fmaf(f, x.x, a[0]);
+                    a[1] = fmaf(f, x.y, a[1]);
+                    a[2] = fmaf(f, x.z, a[2]);
+                    a[3] = fmaf(f, x.w, a[3]);
                 }
-                a += zero;
-                b += zero;
+                if (FMT != 16) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a[k] += zero;
+                }
                 if (whole) {
                     const int c = c0 + cc, j = c / p.G;
                     const int64_t row = (int64_t)(q0 + j) * p.Hq + sg.h * p.G + (c - j * p.G);
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                    reinterpret_cast<uint32_t*>(p.out)[row * (D / 2) + d / 2] = sum == 0.f ? 0u : pack_bf16(a * inv, b * inv);
+                    const uint2 y = sum == 0.f ? make_uint2(0u, 0u) : make_uint2(pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[2] * inv, a[3] * inv));
+                    *reinterpret_cast<uint2*>(p.out + row * D + d) = y;
                     if (d == 0 && p.lse) p.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
                 } else {
-                    *reinterpret_cast<float2*>(part + 2 * X::kCols + cc * D + d) = make_float2(a, b);
+                    *reinterpret_cast<float4*>(part + 2 * X::kCols + cc * D + d) = make_float4(a[0], a[1], a[2], a[3]);
                     if (d == 0) {
                         part[cc] = top;
                         part[X::kCols + cc] = sum;
@@ -1072,6 +1152,16 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         }
         __syncthreads();
     }
+    // requests that list nothing have no slices: their rows are written here
+    for (int r = blockIdx.x; r < p.n_req; r += gridDim.x) {
+        if (__ldg(p.offsets + r + 1) > __ldg(p.offsets + r) && __ldg(p.offsets + r) < p.total) continue;
+        int q0, nq;
+        queries_of(p, r, q0, nq);
+        for (int64_t i = tid; i < (int64_t)nq * p.Hq * (D / 2); i += kThreads)
+            reinterpret_cast<uint32_t*>(p.out)[(int64_t)q0 * p.Hq * (D / 2) + i] = 0u;
+        if (p.lse)
+            for (int i = tid; i < nq * p.Hq; i += kThreads) p.lse[(int64_t)q0 * p.Hq + i] = -INFINITY;
+    }
     // a wait that ran out leaves copies behind: give them one more bounded wait before the block's memory is reused
     if (dead) {
         for (int s = stage; s < X::kStages; ++s) mbar_wait(&full[s], parity);
@@ -1079,41 +1169,31 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     }
 }
 
-// Joins the partial results of the item that crosses the cut between thread blocks blockIdx.x and blockIdx.x + 1 (the
-// first cut of the item does it), eight columns per blockIdx.y.
+// Joins the partial results of the item that begins in thread block blockIdx.x and ends in a later one, eight columns per
+// blockIdx.y.  Part 0 is that block's trailing result, the others are leading ones.
 template <int D, int COLS>
-__global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const int n_parts)
+__global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const int n_blocks)
 {
     constexpr int kC = COLS < 8 ? COLS : 8;
     constexpr int kJoinWarps = D == 256 ? 4 : 8;
     constexpr int kPart = COLS * (D + 2);
     constexpr int kV = D / 32;                        // values of a row per lane
     __shared__ float buf[kJoinWarps][kC][D];
+    __shared__ float sums[kJoinWarps][kC];
     early_start_wait();
+    const Rec rec = reinterpret_cast<const Rec*>(p.ws + (int64_t)2 * n_blocks * kPart)[blockIdx.x];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int32_t all = entries_total(p) * slices_per_entry(p);
-    const int32_t size = part_size(all, n_parts);
-    const int b = blockIdx.x;
-    const int32_t at = (b + 1) * size;
-    if (at >= all) return;
-    const Seg s = segment_at(p, at, all);
-    if (s.begin == at || s.begin < at - size) return;     // nothing crosses here, or an earlier cut does it
-    const int last = (s.end - 1) / size;
-    int q0, nq;
-    queries_of(p, s.r, q0, nq);
     const int y0 = blockIdx.y * 8;
-    const int cols = min(COLS, nq * p.G - s.ct * COLS);
-    if (y0 >= cols) return;
+    if (rec.parts == 0 || y0 >= rec.cols) return;
 
-    // part i of the item: thread block b + i; the first one's is its trailing part, the others' are leading ones
-    auto part_of = [&](int i) { return p.ws + (int64_t)(2 * (b + i) + (i == 0 ? 1 : 0)) * kPart; };
-    const int n = last - b + 1;
+    const float* const first = p.ws + (int64_t)(2 * blockIdx.x + 1) * kPart;
+    const float* const rest = p.ws + (int64_t)2 * blockIdx.x * kPart;
+    auto part_of = [&](int i) { return i == 0 ? first : rest + (int64_t)2 * i * kPart; };
     float top[kC], sum[kC], acc[kC][kV];
 #pragma unroll
     for (int c = 0; c < kC; ++c) {
         float x = -INFINITY;
-        for (int i = lane; i < n; i += 32)
-            x = fmaxf(x, part_of(i)[y0 + c]);
+        for (int i = lane; i < rec.parts; i += 32) x = fmaxf(x, part_of(i)[y0 + c]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
         top[c] = x;
@@ -1121,8 +1201,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const 
 #pragma unroll
         for (int v = 0; v < kV; ++v) acc[c][v] = 0.f;
     }
-    if (warp < kJoinWarps)
-        for (int i = warp; i < n; i += kJoinWarps) {
+    if (warp < kJoinWarps) {
+        for (int i = warp; i < rec.parts; i += kJoinWarps) {
             const float* const part = part_of(i);
 #pragma unroll
             for (int c = 0; c < kC; ++c) {
@@ -1132,8 +1212,6 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const 
                 for (int v = 0; v < kV; ++v) acc[c][v] += f * part[2 * COLS + (y0 + c) * D + v * 32 + lane];
             }
         }
-    __shared__ float sums[kJoinWarps][kC];
-    if (warp < kJoinWarps) {
 #pragma unroll
         for (int c = 0; c < kC; ++c) {
             if (lane == 0) sums[warp][c] = sum[c];
@@ -1144,16 +1222,16 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const 
     __syncthreads();
     for (int i = tid; i < kC * (D / 2); i += 256) {
         const int cl = i / (D / 2), d = (i - cl * (D / 2)) * 2, cc = y0 + cl;
-        if (cc >= cols) continue;
+        if (cc >= rec.cols) continue;
         float l = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) {
-            l += sums[w][cl];
-            x += buf[w][cl][d];
-            y += buf[w][cl][d + 1];
+        for (int k = 0; k < kJoinWarps; ++k) {
+            l += sums[k][cl];
+            x += buf[k][cl][d];
+            y += buf[k][cl][d + 1];
         }
-        const int c = s.ct * COLS + cc, j = c / p.G;
-        const int64_t row = (int64_t)(q0 + j) * p.Hq + s.h * p.G + (c - j * p.G);
+        const int c = rec.c0 + cc, j = c / p.G;
+        const int64_t row = (int64_t)(rec.q0 + j) * p.Hq + rec.h * p.G + (c - j * p.G);
         const float inv = l == 0.f ? 0.f : 1.f / l;
         reinterpret_cast<uint32_t*>(p.out)[row * (D / 2) + d / 2] = l == 0.f ? 0u : pack_bf16(x * inv, y * inv);
         if (d == 0 && p.lse) {
@@ -1203,13 +1281,16 @@ int32_t run(const Params& p, const Maps* maps, Plan* plan, cudaStream_t st)
         if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_release);
     }
     const int64_t all = (int64_t)p.total * p.spe * p.H * p.col_tiles;      // (attend_common has bounded it)
-    // at least one slice per warp: below that more blocks only add partial results
-    int64_t grid = (all + kWarps - 1) / kWarps;
+    // a thread block per item, or one per kShare slices where that is more: further ones would only add partial results
+    constexpr int kShare = 4 * kWarps;
+    int64_t grid = (all + kShare - 1) / kShare;
+    if (grid < (int64_t)p.n_req * p.H * p.col_tiles) grid = (int64_t)p.n_req * p.H * p.col_tiles;
+    if (grid > all) grid = all;
     if (grid > plan->ctas) grid = plan->ctas;
     if (grid < 1) grid = 1;
     kern<<<(unsigned)grid, kThreads, X::kSmem, st>>>(p, *maps);
     UCMX_LAUNCH_CHECK("attend_kernel");
-    if (grid == 1) return UCMX_OK;
+    if (grid == 1 || (int64_t)p.total * p.spe <= kWhole) return UCMX_OK;      // no item can be split
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid - 1, X::kCols <= 8 ? 1 : X::kCols / 8);
     cfg.blockDim = dim3(256);

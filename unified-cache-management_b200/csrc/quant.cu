@@ -145,7 +145,7 @@ __device__ __forceinline__ Piece piece_of(uint32_t item, uint32_t head_chunks)
 
 // HC heads of one token group per warp, their loads all in flight at once.
 template <int BITS, int D, bool BLOCKS, int HC>
-__global__ void __launch_bounds__(256) quant_write_kernel(const QuantParams p)
+__global__ void __launch_bounds__(256, D == 256 ? 3 : 4) quant_write_kernel(const QuantParams p)
 {
     using X = Q<BITS, D>;
     const int lane = threadIdx.x & 31, lr = lane % X::kLanes, row = lane / X::kLanes;
