@@ -10,8 +10,8 @@
 // are the wide operand straight from shared memory, and one column's softmax statistics live in one register per thread.
 //
 // Split.  The unit is a slice: up to 16 consecutive tokens of one listed block.  All slices of all (request, KV head,
-// column tile) items are laid end to end and cut into equal parts, one per thread block, whatever the lengths of the
-// requests are.  A short item stays with the thread block that it begins in; a longer one that crosses cuts leaves partial
+// column tile) items are laid end to end, each item behind a lead of kLead units (what beginning and ending an item costs),
+// and cut into equal parts, one per thread block, whatever the lengths of the requests are.  A short item stays with the thread block that it begins in; a longer one that crosses cuts leaves partial
 // results (running maximum, sum, unnormalised output) in the workspace, which a second small kernel joins in order.  The
 // workspace needs no initial state, and the order of the sums is fixed by the shapes, so results do not change from run to
 // run.
@@ -85,36 +85,43 @@ struct __align__(32) Rec {
     int32_t pad[3];
 };
 
-// One item's part inside a thread block's range.
+// One item's part inside a thread block's range, in units (leads included).
 struct Seg {
-    int32_t begin, end;                // of the whole item, in the order of all slices
+    int32_t begin, end;                // of the whole item
     int32_t lo, hi;                    // the part of it
+    int32_t from, to;                  // that part's slices, counted from the item's first
     int32_t r, h, ct;
     int32_t first;                     // offsets[r]
     int32_t n;                         // entries of the request's list
 };
 
-constexpr int kWhole = 32;             // items up to this many slices are not split (nor up to an eighth of a thread block's share)
+constexpr int kLead = 16;              // an item's fixed cost in slices: queries in, four warps' results joined, result out
+constexpr int kWhole = 48;             // items up to this many units are not split (nor up to an eighth of a thread block's share)
 constexpr int kMaxScan = 1023;         // requests whose column tiles are counted exactly
 
-// How the slices are shared out.  `start` holds the requests' beginnings in order: the lists' offsets, each entry counting for
-// every column tile there may be; or, with several tiles, the exact sums of entries x tiles of each request (built in shared
-// memory: the tiles of a request depend on its number of query tokens).
+// How the units are shared out.  Request r begins at base(r) * mult: base(r) = offsets[r] * spe + r * kLead with mult = KV heads x
+// column tiles; or, where requests may need several tiles, base(r) = the sum of (slices + lead) x tiles of the requests before it,
+// built in shared memory, with mult = KV heads (the tiles of a request depend on its number of query tokens).
 struct Share {
-    const int32_t* start;
-    int32_t per;                       // slices of one entry of `start`
-    int32_t tiles;                     // 0: exact
-    int32_t all, size, lo, hi;         // all slices; a thread block's share; this one's
+    const int32_t* scan;               // nullptr: from the offsets
+    int32_t mult, tiles;
+    int32_t lo, hi;                    // this thread block's units
+    int32_t size;                      // units of a thread block
     int32_t whole;
-    int32_t step;                      // the first level of the search: every step-th entry of `start`,
+    int32_t step;                      // the first level of the search: every step-th base,
     const int32_t* probes;             // 32 of them in shared memory
 };
 
-// The last r with start[r] <= e, and start[r], start[r+1]; 31 intervals a step, the first of them at hand.
-__device__ __forceinline__ int request_of(const Share& w, int n_req, int32_t e, int32_t& first, int32_t& next)
+__device__ __forceinline__ int32_t base_of(const Params& p, const int32_t* scan, int32_t r)
+{
+    return scan ? scan[r] : max(0, min(__ldg(p.offsets + r), p.total)) * p.spe + r * kLead;
+}
+
+// The last r with base(r) <= e, and base(r), base(r+1); 31 intervals a step, the first of them at hand.
+__device__ __forceinline__ int request_of(const Params& p, const Share& w, int32_t e, int32_t& first, int32_t& next)
 {
     const int lane = threadIdx.x & 31;
-    int lo = 0, n = n_req, step = w.step;
+    int lo = 0, n = p.n_req, step = w.step;
     int32_t v = w.probes[lane];
     for (;;) {
         const int c = __popc(__ballot_sync(0xffffffffu, lane * step < n && v <= e));
@@ -127,7 +134,7 @@ __device__ __forceinline__ int request_of(const Share& w, int n_req, int32_t e, 
         lo += adv;
         n = min(step, n - adv);
         step = (n + 30) / 31;
-        v = w.start[lo + min(lane * step, n)];
+        v = base_of(p, w.scan, lo + min(lane * step, n));
     }
 }
 
@@ -147,33 +154,38 @@ __device__ __forceinline__ void queries_of(const Params& p, int r, int& q0, int&
     }
 }
 
-// The item that holds position `at` (below w.hi) and this thread block's part of it; called by whole warps.
+// The item that holds unit `at` and the part of it that ends in this thread block; called by whole warps.
 template <int COLS>
 __device__ __forceinline__ Seg segment_at(const Params& p, const Share& w, int32_t at)
 {
     Seg s;
     int32_t a, b, tiles = w.tiles;
-    s.r = request_of(w, p.n_req, at / w.per, a, b);
-    if (tiles == 0) {
+    s.r = request_of(p, w, at / w.mult, a, b);
+    if (w.scan) {
         int q0, nq;
         queries_of(p, s.r, q0, nq);
         tiles = max(1, (nq * p.G + COLS - 1) / COLS);
         s.first = __ldg(p.offsets + s.r);
-        s.n = (b - a) / tiles;
     } else {
-        s.first = a;
-        s.n = min(b, p.total) - a;
+        s.first = (a - s.r * kLead) / p.spe;
     }
-    const int32_t item = s.n * p.spe;                  // slices of one (KV head, column tile)
-    const int32_t i = (at - a * w.per) / item;
+    const int32_t item = w.scan ? (b - a) / tiles : b - a;       // units of one (KV head, column tile)
+    s.n = (item - kLead) / p.spe;
+    const int32_t i = (at - a * w.mult) / item;
     s.h = i / tiles;
     s.ct = i - s.h * tiles;
-    s.begin = a * w.per + i * item;
+    s.begin = a * w.mult + i * item;
     s.end = s.begin + item;
     s.lo = at;
     s.hi = item <= w.whole || s.end < w.hi ? s.end : w.hi;
+    s.from = max(0, at - s.begin - kLead);
+    s.to = s.hi - s.begin - kLead;
     return s;
 }
+
+// Does the part that begins with the item belong to this thread block?  A split item's first part goes to the one that holds its
+// first slice.
+__device__ __forceinline__ bool begins_here(const Share& w, const Seg& s) { return s.end - s.begin <= w.whole || s.begin + kLead < w.hi; }
 
 // 2^x for a weight: x is at most kMaxSlack, and what is below 2^-126 of the largest weight is nothing
 __device__ __forceinline__ float exp2_fast(float x)
@@ -400,9 +412,9 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
 
     // ---- this thread block's share
     Share w;
-    w.start = p.offsets;
+    w.scan = nullptr;
     w.tiles = p.col_tiles;
-    w.per = p.spe * p.H * p.col_tiles;
+    w.mult = p.H * p.col_tiles;
     if (X::kTiled && p.col_tiles > 1 && p.n_req <= kMaxScan) {
         constexpr int kEach = (kMaxScan + kThreads) / kThreads;
         int32_t v[kEach], sum = 0;
@@ -413,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             if (r < p.n_req) {
                 int q0, nq;
                 queries_of(p, r, q0, nq);
-                v[i] = max(0, min(__ldg(p.offsets + r + 1), p.total) - __ldg(p.offsets + r)) * ((nq * p.G + X::kCols - 1) / X::kCols);
+                v[i] = (base_of(p, nullptr, r + 1) - base_of(p, nullptr, r)) * ((nq * p.G + X::kCols - 1) / X::kCols);
             }
             sum += v[i];
         }
@@ -435,26 +447,27 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             before += v[i];
         }
         __syncthreads();
-        w.start = scan;
-        w.tiles = 0;
-        w.per = p.spe * p.H;
+        w.scan = scan;
+        w.mult = p.H;
     }
     w.step = (p.n_req + 30) / 31;
     int32_t* const probes = reinterpret_cast<int32_t*>(note + X::kStages * L::kUnits);
-    const int32_t probe = w.start[min(lane * w.step, p.n_req)];
+    const int32_t probe = base_of(p, w.scan, min(lane * w.step, p.n_req));
     probes[lane] = probe;
     __syncwarp();
     w.probes = probes;
-    const int32_t entries = __shfl_sync(0xffffffffu, probe, 31);          // a captured batch may use less than its capacity
-    w.all = (w.tiles == 0 ? entries : max(0, min(entries, p.total))) * w.per;
-    w.size = (int32_t)(((uint32_t)w.all + gridDim.x - 1u) / gridDim.x);   // (the host keeps all + grid below 2^31)
-    w.lo = min(w.all, (int32_t)blockIdx.x * w.size);
-    w.hi = w.lo + min(w.size, w.all - w.lo);
+    const int32_t all = __shfl_sync(0xffffffffu, probe, 31) * w.mult;     // (a captured batch may use less than its capacity)
+    w.size = (int32_t)(((uint32_t)all + gridDim.x - 1u) / gridDim.x);     // (the host keeps all + grid below 2^31)
+    w.lo = min(all, (int32_t)blockIdx.x * w.size);
+    w.hi = w.lo + min(w.size, all - w.lo);
     w.whole = max(kWhole, w.size / 8);
     int32_t begin = w.lo;
     if (begin < w.hi) {
         const Seg s = segment_at<X::kCols>(p, w, begin);
-        if (s.begin < begin && s.end - s.begin <= w.whole) begin = s.end;     // the thread block before takes all of it
+        if (s.begin < begin) {
+            if (s.end - s.begin <= w.whole) begin = s.end;                // the thread block before takes all of it
+            else if (begin <= s.begin + kLead) begin = s.begin;           // its first slice is here
+        }
     }
     Rec* const rec = reinterpret_cast<Rec*>(p.ws + (int64_t)2 * gridDim.x * X::kPart) + blockIdx.x;
     if (tid == 0) rec->parts = 0;
@@ -462,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     // ---- the warp's loads run ahead of its arithmetic, across items: a cursor of their own
     constexpr int kU = L::kUnits, kStep = kWarps * kU;
     Seg ps;
-    ps.hi = -1;
+    ps.to = -1;
     int32_t p_at = 0;                  // next slice to load of segment ps
     int32_t p_look = 32;               // lanes p_look .. p_look + kU - 1 know the slices to load next; 32: look again
     int32_t p_entries = 0;             // entries of the request that count
@@ -476,11 +489,10 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     bool p_done = false;
     int32_t p_next = begin;            // where the next segment begins
     uint32_t plain = 0;                // bit s: the step in stage s needs no masks
-    // what this lane has to know of slice `at` of segment ps
-    auto look_up = [&](int32_t at) {
+    // what this lane has to know of slice s of segment ps
+    auto look_up = [&](int32_t s) {
         my_flags = 0;
-        if (at >= ps.hi) return;
-        const int32_t s = at - ps.begin;
+        if (s >= ps.to) return;
         const int32_t e = s / p.spe, sub = (s - e * p.spe) * kRows;
         const int32_t pos_block = p.positions ? __ldg(p.positions + ps.first + e) : e;
         int32_t id = p.block_ids ? __ldg(p.block_ids + ps.first + e) : -1;
@@ -517,15 +529,15 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     };
     // start the loads of the warp's next step into stage s; every step completes its barrier, with or without bytes
     auto issue = [&](int s) {
-        if (p_at >= ps.hi) {
-            while (!p_done && p_at >= ps.hi) {
-                if (p_next >= w.hi) {
+        if (p_at >= ps.to) {
+            while (!p_done && p_at >= ps.to) {
+                if (p_next < w.hi) ps = segment_at<X::kCols>(p, w, p_next);
+                if (p_next >= w.hi || !begins_here(w, ps)) {
                     p_done = true;
                     break;
                 }
-                ps = segment_at<X::kCols>(p, w, p_next);
                 p_next = ps.hi;
-                p_at = ps.lo + warp * kU;
+                p_at = ps.from + warp * kU;
                 p_look = 32;
                 p_entries = p.counts ? min(ps.n, __ldg(p.counts + ps.r)) : ps.n;
                 if (p.ctx) {
@@ -605,6 +617,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
 #pragma unroll 1
     while (at < w.hi) {
         const Seg sg = segment_at<X::kCols>(p, w, at);
+        if (!begins_here(w, sg)) break;
         at = sg.hi;
         int q0, nq;
         queries_of(p, sg.r, q0, nq);
@@ -1050,7 +1063,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         };
         // ---------------------------------------------------------------------------- the warp's slices of this item
 #pragma unroll 1
-        for (int32_t s = sg.lo + warp * kU; s < sg.hi; s += kStep) {
+        for (int32_t s = sg.from + warp * kU; s < sg.to; s += kStep) {
             if (!dead && !mbar_wait(&full[stage], parity)) {
                 if (p.err && lane == 0) atomicExch(p.err, 1);
                 dead = true;
@@ -1151,16 +1164,6 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             }
         }
         __syncthreads();
-    }
-    // requests that list nothing have no slices: their rows are written here
-    for (int r = blockIdx.x; r < p.n_req; r += gridDim.x) {
-        if (__ldg(p.offsets + r + 1) > __ldg(p.offsets + r) && __ldg(p.offsets + r) < p.total) continue;
-        int q0, nq;
-        queries_of(p, r, q0, nq);
-        for (int64_t i = tid; i < (int64_t)nq * p.Hq * (D / 2); i += kThreads)
-            reinterpret_cast<uint32_t*>(p.out)[(int64_t)q0 * p.Hq * (D / 2) + i] = 0u;
-        if (p.lse)
-            for (int i = tid; i < nq * p.Hq; i += kThreads) p.lse[(int64_t)q0 * p.Hq + i] = -INFINITY;
     }
     // a wait that ran out leaves copies behind: give them one more bounded wait before the block's memory is reused
     if (dead) {
@@ -1280,17 +1283,14 @@ int32_t run(const Params& p, const Maps* maps, Plan* plan, cudaStream_t st)
         UCMX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, X::kSmem));
         if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_release);
     }
-    const int64_t all = (int64_t)p.total * p.spe * p.H * p.col_tiles;      // (attend_common has bounded it)
-    // a thread block per item, or one per kShare slices where that is more: further ones would only add partial results
-    constexpr int kShare = 4 * kWarps;
-    int64_t grid = (all + kShare - 1) / kShare;
-    if (grid < (int64_t)p.n_req * p.H * p.col_tiles) grid = (int64_t)p.n_req * p.H * p.col_tiles;
-    if (grid > all) grid = all;
+    // (attend_common has bounded it) a thread block per kLead units: an item of a few slices has one of its own
+    const int64_t all = ((int64_t)p.total * p.spe + (int64_t)p.n_req * kLead) * p.H * p.col_tiles;
+    int64_t grid = (all + kLead - 1) / kLead;
     if (grid > plan->ctas) grid = plan->ctas;
     if (grid < 1) grid = 1;
     kern<<<(unsigned)grid, kThreads, X::kSmem, st>>>(p, *maps);
     UCMX_LAUNCH_CHECK("attend_kernel");
-    if (grid == 1 || (int64_t)p.total * p.spe <= kWhole) return UCMX_OK;      // no item can be split
+    if (grid == 1 || (int64_t)p.total * p.spe + kLead <= kWhole) return UCMX_OK;      // no item can be split
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid - 1, X::kCols <= 8 ? 1 : X::kCols / 8);
     cfg.blockDim = dim3(256);
