@@ -558,6 +558,10 @@ class _on_device:
             self.guard.__exit__(*exc)
 
 
+# the current stream's handle without a Stream object around it (2 us less per call), where this torch has the call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _need_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
     """CUDA tensors, all of them on one device."""
     dev = first.device
@@ -594,8 +598,8 @@ def quant_write_tokens(cache: QuantKvCache, k: torch.Tensor, v: torch.Tensor, sl
         raise ValueError("slots must be contiguous int64")
     with _on_device(cache.data):
         strides = [x.stride(0) if n > 1 else g.n_kv_heads * g.head_dim for x in (k, v)]
-        st = N.lib.ucmx_quant_write_tokens(_ptr(k), _ptr(v), strides[0], strides[1], n, _ptr(slots), _ptr(cache.data), C.byref(g),
-                                           _stream(cache.data))
+        st = N.lib.ucmx_quant_write_tokens(k.data_ptr(), v.data_ptr(), strides[0], strides[1], n, slots.data_ptr(), cache.data.data_ptr(), C.byref(g),
+                                           _raw_stream(cache.data.device.index))
     N.check("ucmx_quant_write_tokens", st, 1 if n else 0)
 
 
@@ -608,9 +612,9 @@ def quant_write_blocks(cache: QuantKvCache, k_cache: torch.Tensor, v_cache: torc
     if out_slots is not None and out_slots.numel() != n:
         raise ValueError("one out_slots entry per block id")
     with _on_device(cache.data):
-        st = N.lib.ucmx_quant_write_blocks(_ptr(k_cache), C.byref(kv_geometry(k_cache)), _ptr(v_cache), C.byref(kv_geometry(v_cache)),
-                                           _ptr(ids), _ptr(_i32(out_slots, "out_slots")), n, _ptr(cache.data), C.byref(cache.geometry),
-                                           _stream(cache.data))
+        st = N.lib.ucmx_quant_write_blocks(k_cache.data_ptr(), C.byref(kv_geometry(k_cache)), v_cache.data_ptr(), C.byref(kv_geometry(v_cache)),
+                                           ids.data_ptr(), _ptr(_i32(out_slots, "out_slots")), n, cache.data.data_ptr(), C.byref(cache.geometry),
+                                           _raw_stream(cache.data.device.index))
     N.check("ucmx_quant_write_blocks", st, 1 if n else 0)
 
 
@@ -630,8 +634,8 @@ def quant_read_blocks(cache: QuantKvCache, block_ids: torch.Tensor, *, k_out: Op
         k_out, v_out = (torch.zeros((n, g.block_tokens, g.n_kv_heads, g.head_dim), dtype=torch.bfloat16, device=cache.data.device)
                         for _ in range(2))
     with _on_device(cache.data):
-        st = N.lib.ucmx_quant_read_blocks(_ptr(cache.data), C.byref(g), _ptr(ids), _ptr(_i32(out_slots, "out_slots")), n, _ptr(k_out),
-                                          C.byref(kv_geometry(k_out)), _ptr(v_out), C.byref(kv_geometry(v_out)), _stream(cache.data))
+        st = N.lib.ucmx_quant_read_blocks(cache.data.data_ptr(), C.byref(g), ids.data_ptr(), _ptr(_i32(out_slots, "out_slots")), n, k_out.data_ptr(),
+                                          C.byref(kv_geometry(k_out)), v_out.data_ptr(), C.byref(kv_geometry(v_out)), _raw_stream(cache.data.device.index))
     N.check("ucmx_quant_read_blocks", st, 1 if n else 0)
     return k_out, v_out
 
@@ -683,7 +687,7 @@ def _attend(name: str, fn, bits: int, n_kv_heads: int, head_dim: int, cache_args
     if q_offsets is None and (n_tok != n_req or max_q_tokens != 1):
         raise ValueError("without q_offsets there is one query token per request")
     if out is None:
-        out = torch.empty((n_tok, Hq, D), dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.dtype is not torch.bfloat16 or not out.is_contiguous() or tuple(out.shape) != (n_tok, Hq, D):
         raise ValueError("out must be contiguous bf16 of the query's shape")
     if lse is not None and (lse.dtype is not torch.float32 or not lse.is_contiguous() or tuple(lse.shape) != (n_tok, Hq)):
@@ -695,7 +699,7 @@ def _attend(name: str, fn, bits: int, n_kv_heads: int, head_dim: int, cache_args
     with _on_device(query):
         st = fn(query.data_ptr(), q_stride, Hq, q_off, n_tok, max_q_tokens, *cache_args, C.byref(lists),
                 D ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(),
-                workspace.nbytes, torch.cuda.current_stream(dev).cuda_stream)
+                workspace.nbytes, _raw_stream(dev.index))
     N.check(name, st, 2)
     return out
 
