@@ -1,6 +1,6 @@
 """One decode step of sparse-KV retrieval for a ragged batch, layer by layer:
 pool the newly filled blocks -> score every block of every request -> per-request top-k ->
-gather the selected K and V blocks into a contiguous working set.
+gather the selected K and V blocks into a contiguous working set, or attend to them where they are.
 
 This is the sequence the reference spreads over ESA's hooks (ucm/sparse/esa/esa.py:286-399: start_retrieval,
 wait_retrieval_and_start_load, block_repre_data, launch_transfer_task) with a CPU thread pool in the
@@ -24,7 +24,7 @@ class DecodeRetrievalEngine:
     def __init__(self, shape: KvShape, batch: RaggedBatch, device: torch.device, *, n_layers: Optional[int] = None,
                  with_kv_pool: bool = True, heads_local: Optional[int] = None, seed: int = 0,
                  score_reduce=None, peer_exchange=None, order: int = ops.ORDER_SCORE_DESC, delta: bool = False,
-                 overlap: bool = False):
+                 overlap: bool = False, attend: bool = False, cache_bits: int = 16):
         """heads_local: KV heads held by this rank under tensor parallelism (default: all).
         score_reduce: callable applied in place to the fp32 score vector between scoring and top-k
         (the tensor-parallel all-reduce); None on a single rank.
@@ -35,7 +35,12 @@ class DecodeRetrievalEngine:
         to the previous step's selection (what ESA does, ucm/sparse/esa/esa.py:313-338): top-k of block positions in
         ascending order -> resident-set remap -> block-to-block move of the misses.
         overlap: scoring and selection of layer l+1 run on a second stream while layer l's blocks move (they do not
-        depend on each other); the step is then bounded by the block moves alone."""
+        depend on each other); the step is then bounded by the block moves alone.
+        attend: each layer ends with the attention of its queries over the blocks just selected, written to
+        attn_out[layer].  It reads the blocks in the pool, in place of the gather; in the delta step it follows the
+        move and reads the resident working set.
+        cache_bits: 4 or 8 keeps a quantised copy of the pool beside it (quant_pool) and attends over that; blocks that
+        filled up since the last step are quantised when the step begins."""
         self.shape, self.batch, self.device = shape, batch, device
         self.L = n_layers if n_layers is not None else shape.n_layers
         self.H = heads_local if heads_local is not None else shape.n_kv_heads
@@ -101,6 +106,22 @@ class DecodeRetrievalEngine:
             self.moves = ops.MoveList(n, device)
             self.max_logical = int(batch.blocks_per_req.max())
             self.launches_per_step = self.L * 4 + 1
+        self.attend = attend
+        self.quant_pool: Optional[ops.QuantKvCache] = None
+        if not attend and cache_bits != 16:
+            raise ValueError("cache_bits says what the attention reads: it needs attend=True")
+        if attend:
+            if not with_kv_pool:
+                raise ValueError("the attention reads the K/V pool: it needs with_kv_pool=True")
+            if delta and cache_bits != 16:
+                raise ValueError("the delta step's working set is kept in bf16")
+            self.attn_out = torch.zeros((self.L, batch.n_req, self.Hq, self.D), dtype=torch.bfloat16, device=device)
+            self.attn_workspace = ops.attention_workspace(self.q_dev[0], self.H, bits=cache_bits)
+            self.launches_per_step += self.L * (2 if delta else 1)
+            if cache_bits != 16:
+                self.quant_pool = ops.QuantKvCache.alloc(batch.n_slots, self.T, self.H, self.D, cache_bits, device)
+                ops.quant_write_blocks(self.quant_pool, self.kv_pool[0], self.kv_pool[1], self.block_table, out_slots=self.block_table)
+                self.launches_per_step += 1
 
     # ---------------------------------------------------------------------------------- stages
     def make_queries(self) -> torch.Tensor:
@@ -120,6 +141,8 @@ class DecodeRetrievalEngine:
             self._pool_all = (ids, slots, self.rep_tables.view(self.L * ns, self.H, 1, self.D))
         ids, slots, table = self._pool_all
         ops.pool_blocks(self.kv_pool[0], ids, out_slots=slots, out_bf16=table)
+        if self.quant_pool is not None:
+            ops.quant_write_blocks(self.quant_pool, self.kv_pool[0], self.kv_pool[1], self.new_block_ids, out_slots=self.new_block_ids)
 
     def pool_layer(self, layer: int) -> None:
         ops.pool_blocks(self.kv_pool[0], self.new_block_ids, out_slots=self.new_block_ids,
@@ -159,6 +182,9 @@ class DecodeRetrievalEngine:
         if self.delta:
             self.remap_layer(layer)
             self.move_layer(layer)
+        if self.attend:
+            self.attend_layer(layer)
+        if self.delta or self.attend:
             return
         ops.gather_blocks([self.kv_pool[0], self.kv_pool[1]], self.sel_ids[layer], self.staging)
 
@@ -171,6 +197,18 @@ class DecodeRetrievalEngine:
 
     def move_layer(self, layer: int) -> None:
         ops.move_blocks([self.kv_pool[0], self.kv_pool[1]], self.moves, [self.staging[:, 0], self.staging[:, 1]])
+
+    def attend_layer(self, layer: int) -> torch.Tensor:
+        """Attention of the layer's queries over its selected blocks (every block of a selection is full, so their places
+        in the sequences do not matter)."""
+        args = dict(req_counts=self.sel_counts[layer], out=self.attn_out[layer], workspace=self.attn_workspace)
+        if self.delta:                             # the resident slots that serve the selection
+            shape = (self.batch.total_k, self.T, self.H, self.D)
+            k, v = (self.staging[:, i].view(torch.bfloat16).view(shape) for i in (0, 1))
+            return ops.block_attention(self.q_dev[layer], k, v, self.k_offsets, block_ids=self.remap_out[layer][0], **args)
+        if self.quant_pool is not None:
+            return ops.quant_block_attention(self.q_dev[layer], self.quant_pool, self.k_offsets, block_ids=self.sel_ids[layer], **args)
+        return ops.block_attention(self.q_dev[layer], self.kv_pool[0], self.kv_pool[1], self.k_offsets, block_ids=self.sel_ids[layer], **args)
 
     def drift_queries(self, rho: float = 0.98) -> None:
         """Next decode step's queries: a seeded random walk, q <- rho*q + sqrt(1-rho^2)*noise, so that consecutive
