@@ -370,7 +370,7 @@ struct Traits {
     static constexpr int kRingBytes = kWarps * kStages * L::kStage;
     static constexpr int kMergeBytes = kWarps * kMergeCols * kMergeLd * 4;
     static constexpr int kStatBytes = kWarps * kCols * 3 * 4;
-    static constexpr bool kTiled = NT == 4 || (D == 256 && NT == 2);      // the widest tile: requests may need several
+    static constexpr bool kTiled = NT >= 2;              // requests may need several tiles
     static constexpr int kScanBytes = kTiled ? (kMaxScan + 1) * 4 : 0;
     static constexpr int kQBytes = kQReg ? 0 : kKSteps * NT * 32 * 8;
     static constexpr int kBarStride = kStages * (8 + 8 * L::kUnits) + 128;    // a warp's barriers, a note (8) per slice, 32 probes
@@ -663,6 +663,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             if (FMT == 16) {
 #pragma unroll
                 for (int ks = 0; ks < X::kKSteps; ++ks) {
+                    if (!X::kQReg && (ks & 3) != warp) continue;
                     const uint32_t b0 = live ? __ldg(reinterpret_cast<const uint32_t*>(qp + ks * 16 + 2 * q4)) : 0u;
                     const uint32_t b1 = live ? __ldg(reinterpret_cast<const uint32_t*>(qp + ks * 16 + 8 + 2 * q4)) : 0u;
                     put(ks, b0, b1);
@@ -1205,6 +1206,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const 
         for (int v = 0; v < kV; ++v) acc[c][v] = 0.f;
     }
     if (warp < kJoinWarps) {
+#pragma unroll(kC == 4 ? 4 : 2)
         for (int i = warp; i < rec.parts; i += kJoinWarps) {
             const float* const part = part_of(i);
 #pragma unroll
@@ -1249,14 +1251,17 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const 
 
 // ---------------------------------------------------------------------------------------------------- host side
 
-// Columns of a tile for `cols` query rows of a KV head: the narrowest tile that takes them all, 32 (16 with 256 values a
-// head) and several tiles beyond that.  A tile reads K and V once; a narrower one costs fewer instructions per token.
-inline int tile_cols(int cols, int head_dim)
+// Columns of a tile for `cols` query rows of a KV head.  A tile reads K and V once and pays for its matrix instructions and
+// weights: a tile of 32 takes about 1.5 times one of 16 (24 requests of 6400 tokens, 128 values a head, 8 heads: 32 columns 138 us
+// in one tile, 202 us in two; 40 columns 241 us in two, 230 us in three).  Codes are decoded once per tile, but beside 128
+// accumulators there are no registers left for it: 16 is their widest (8 requests of 8192 tokens, 32 columns: 72 us against 94 us
+// with 32), as it is with 256 values a head.
+inline int tile_cols(int cols, int head_dim, int format)
 {
     if (cols <= 4) return 4;
     if (cols <= 8) return 8;
-    if (cols <= 16 || head_dim == 256) return 16;
-    return 32;
+    if (format != 16 || head_dim == 256) return 16;
+    return 2 * ((cols + 15) / 16) <= 3 * ((cols + 31) / 32) ? 16 : 32;
 }
 
 // what a launch needs for one shape (asked for without maps: nothing is launched)
@@ -1308,12 +1313,12 @@ int32_t run(const Params& p, const Maps* maps, Plan* plan, cudaStream_t st)
 template <int FMT, int D>
 int32_t run_cols(const Params& p, int cols, const Maps* maps, Plan* plan, cudaStream_t st)
 {
-    switch (tile_cols(cols, D)) {
+    switch (tile_cols(cols, D, FMT)) {
         case 4: return run<FMT, D, 1, true>(p, maps, plan, st);
         case 8: return run<FMT, D, 1, false>(p, maps, plan, st);
         case 16: return run<FMT, D, 2, false>(p, maps, plan, st);
         default:
-            if constexpr (D != 256) return run<FMT, D, 4, false>(p, maps, plan, st);
+            if constexpr (D != 256 && FMT == 16) return run<FMT, D, 4, false>(p, maps, plan, st);
             return UCMX_EUNSUPPORTED;
     }
 }
