@@ -598,11 +598,13 @@ int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_geometry* geo
  * head over that head's K and V:  out = sum_t softmax_t(scale * q . k_t) v_t.  fp32 inside, out is bf16 [n_q_tokens, n_q_heads,
  * head_dim], out_lse (NULL, or fp32 [n_q_tokens, n_q_heads]) the natural logarithm of the softmax's sum, for joining with
  * attention over other tokens.  A query that sees nothing gets zeros and -infinity.
- * Lists (all device pointers but the struct itself): entries [offsets[r], offsets[r+1]), offsets[0] = 0, ascending; `total` is
- *   the capacity of the entry arrays (what lies behind offsets[n_req] is not read, so a captured launch may be replayed with
- *   fewer entries); counts (or NULL) cuts a request's list short.
+ * Lists (all device pointers but the struct itself): entries [offsets[r], offsets[r+1]), ascending; `total` is the capacity of
+ *   the entry arrays: what lies outside [offsets[0], offsets[n_req]) is not read, so a captured launch may be replayed with fewer
+ *   entries.  Offsets that do not ascend are reported (code 3); the results of such a call are not defined.  counts (or NULL) cuts
+ *   a request's list short.
  *   block_ids[e] is the physical block, negative = skip the entry; with block_ids NULL the physical block is
- *   table[table_offsets[r] + positions[e]] (the request's row of a block table; table_offsets has n_req+1 entries).
+ *   table[table_offsets[r] + positions[e]] (the request's row of a block table; table_offsets has n_req+1 entries, table holds
+ *   table_size).
  *   positions[e] is the block's place in its sequence, negative = skip; with positions NULL the i-th entry stands at i.
  *   ctx_lens[r] (or NULL: every token of every listed block is seen) is the length of the sequence, the query tokens included:
  *   query token j of the request's n sees the tokens at places below ctx_lens[r] - (n-1-j).  What stands in tokens that a
@@ -625,6 +627,7 @@ typedef struct ucmx_block_lists {
     const int32_t* ctx_lens;
     int32_t n_req;
     int32_t total;
+    int32_t table_size;
 } ucmx_block_lists;
 size_t ucmx_attention_workspace_bytes(int32_t bits, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t max_q_tokens);
 int32_t ucmx_block_attention(const void* q, int64_t q_stride, int32_t n_q_heads, const int32_t* q_offsets, int32_t n_q_tokens,

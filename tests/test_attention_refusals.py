@@ -25,7 +25,7 @@ def qgeom(**kw):
 
 def lists(**kw):
     from ucmx import _native as N
-    a = dict(offsets=FAKE, counts=0, block_ids=FAKE, positions=0, table=0, table_offsets=0, ctx_lens=0, n_req=1, total=3)
+    a = dict(offsets=FAKE, counts=0, block_ids=FAKE, positions=0, table=0, table_offsets=0, ctx_lens=0, n_req=1, total=3, table_size=0)
     a.update(kw)
     return C.byref(N.BlockLists(*a.values()))
 
@@ -55,7 +55,7 @@ def test_attention_refusals(why):
             assert attend(kg=geom(**x), vg=geom(**x), q_stride=8 * d) == N.EUNSUPPORTED
     elif why == "lists":
         for kw in (dict(offsets=0), dict(block_ids=0), dict(block_ids=0, positions=FAKE), dict(block_ids=0, positions=FAKE, table=FAKE),
-                   dict(n_req=-1), dict(total=-1)):
+                   dict(n_req=-1), dict(total=-1), dict(table_size=-1)):
             assert attend(lists=lists(**kw)) == N.EPARAM, kw
     else:
         assert attend(**why) == N.EPARAM

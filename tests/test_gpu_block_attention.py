@@ -419,3 +419,45 @@ def test_offsets_beyond_32_bits():
     kd, vd = R.values(c.data[torch.tensor(used, device=DEV)].cpu(), 64, 4)
     out, _, tol, _ = R.attend(q.cpu(), kd, vd, [(range(1), [(i, i) for i in range(4)], None)], codes_err=8.0)
     R.check(got, out, tol)
+
+
+@pytest.mark.parametrize("fmt", [16, 8])
+def test_lists_inside_larger_arrays(fmt):
+    """Some of a batch's requests, by a piece of its offsets: entries, tables and offsets stay where they are."""
+    s = Setup(50, fmt, 2, 4, 128, 16, [4, 70, 5, 0, 40, 3]).tails()
+    w = s.want()
+    got = s.run(q=s.q[1:5].to(DEV), offsets=dev(s.off[1:6]), ctx_lens=dev(s.ctx[1:5]))
+    R.check(got, w[0][1:5], w[2][1:5])
+    t = Setup(51, fmt, 1, 8, 64, 32, [9, 30, 2], [2, 5, 3]).tails()      # with several tiles of columns
+    w = t.want()
+    qo = t.qoff[1:] - t.qoff[1]
+    got = t.run(q=t.q[2:].to(DEV), offsets=dev(t.off[1:]), ctx_lens=dev(t.ctx[1:]), q_offsets=dev(qo), max_q_tokens=5)
+    R.check(got, w[0][2:], w[2][2:])
+
+
+@pytest.mark.parametrize("nq", [1, 5])
+def test_offsets_that_do_not_ascend_are_reported(nq):
+    """They index nothing outside the lists, the call ends and says so, and the next one is fine."""
+    from ucmx import _native
+    s = Setup(52, 16, 2, 8, 64, 16, [6, 90, 4, 8], [nq] * 4).tails()
+    _native.device_error()
+    for off in ([0, 6, 3, 90, 40], [0, 108, 0, 108, 0], [50, 40, 30, 20, 10], [0, 2_000_000_000, -5, 7, 108], [0, 6, 200, 100, 108]):
+        s.run(offsets=dev(off))
+        torch.cuda.synchronize()
+    assert _native.device_error() == 3
+    s.check()
+
+
+def test_a_table_that_ends_early_is_reported():
+    from ucmx import _native
+    s = Setup(53, 4, 2, 4, 128, 16, [6, 5])
+    table = s.ids.copy()
+    place = np.asarray([0, 5, 2, 4, 1, 3, 0, 4, 2, 1, 3], np.int32)
+    s.positions = place
+    s.ids = np.asarray([table[p] for p in place[:6]] + [table[6 + p] if 6 + p < 9 else -1 for p in place[6:]], np.int32)
+    w = s.want()
+    _native.device_error()
+    got = s.run(block_ids=None, block_table=dev(table[:9]), table_offsets=dev(s.off))
+    torch.cuda.synchronize()
+    assert _native.device_error() == 3
+    R.check(got, w[0], w[2])

@@ -65,7 +65,7 @@ int32_t attend_common(Params& p, int bits, int32_t head_dim, const void* q, int6
                       const int32_t* q_offsets, int32_t n_q_tokens, int32_t max_q_tokens, const ucmx_block_lists* l, float scale,
                       void* out, float* out_lse, void* workspace, size_t workspace_bytes, ucmx_stream_t stream)
 {
-    if (!l || l->n_req < 0 || l->total < 0 || n_q_tokens < 0) return refuse("attention: negative sizes or no lists");
+    if (!l || l->n_req < 0 || l->total < 0 || l->table_size < 0 || n_q_tokens < 0) return refuse("attention: negative sizes or no lists");
     if (l->n_req == 0 || n_q_tokens == 0) return UCMX_OK;
     if (!q || !out || !l->offsets || !workspace) return refuse("attention: a pointer is missing");
     if (l->total > 0 && !l->block_ids && !(l->positions && l->table && l->table_offsets))
@@ -92,6 +92,7 @@ int32_t attend_common(Params& p, int bits, int32_t head_dim, const void* q, int6
     p.positions = l->positions;
     p.table = l->table;
     p.table_offsets = l->table_offsets;
+    p.table_size = l->table_size;
     p.ctx = l->ctx_lens;
     p.n_req = l->n_req;
     p.total = l->total;

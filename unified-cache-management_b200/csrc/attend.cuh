@@ -63,6 +63,7 @@ struct Params {
     const int32_t* positions;          // [total] or NULL: the i-th entry of a request stands at i
     const int32_t* table;
     const int32_t* table_offsets;      // [n_req+1]
+    int32_t table_size;
     const int32_t* ctx;                // [n_req] or NULL
     int32_t n_req, total;
     int32_t col_tiles, cols_per_tile;
@@ -99,12 +100,13 @@ constexpr int kLead = 16;              // an item's fixed cost in slices: querie
 constexpr int kWhole = 48;             // items up to this many units are not split (nor up to an eighth of a thread block's share)
 constexpr int kMaxScan = 1023;         // requests whose column tiles are counted exactly
 
-// How the units are shared out.  Request r begins at base(r) * mult: base(r) = offsets[r] * spe + r * kLead with mult = KV heads x
+// How the units are shared out.  Request r begins at (base(r) - base(0)) * mult: base(r) = offsets[r] * spe + r * kLead with mult = KV heads x
 // column tiles; or, where requests may need several tiles, base(r) = the sum of (slices + lead) x tiles of the requests before it,
 // built in shared memory, with mult = KV heads (the tiles of a request depend on its number of query tokens).
 struct Share {
     const int32_t* scan;               // nullptr: from the offsets
     int32_t mult, tiles;
+    int32_t zero;                      // base(0): the lists may begin anywhere in the entry arrays
     int32_t lo, hi;                    // this thread block's units
     int32_t size;                      // units of a thread block
     int32_t whole;
@@ -154,27 +156,38 @@ __device__ __forceinline__ void queries_of(const Params& p, int r, int& q0, int&
     }
 }
 
-// The item that holds unit `at` and the part of it that ends in this thread block; called by whole warps.
+// The item that holds unit `at` and the part of it that ends in this thread block; called by whole warps.  Offsets that do not
+// ascend make items that cannot be: they are passed over (n < 0) and reported.
 template <int COLS>
 __device__ __forceinline__ Seg segment_at(const Params& p, const Share& w, int32_t at)
 {
     Seg s;
     int32_t a, b, tiles = w.tiles;
-    s.r = request_of(p, w, at / w.mult, a, b);
+    s.r = request_of(p, w, at / w.mult + w.zero, a, b);
     if (w.scan) {
         int q0, nq;
         queries_of(p, s.r, q0, nq);
         tiles = max(1, (nq * p.G + COLS - 1) / COLS);
-        s.first = __ldg(p.offsets + s.r);
+        s.first = max(0, min(__ldg(p.offsets + s.r), p.total));
     } else {
         s.first = (a - s.r * kLead) / p.spe;
     }
     const int32_t item = w.scan ? (b - a) / tiles : b - a;       // units of one (KV head, column tile)
+    const int32_t start = (a - w.zero) * w.mult;
     s.n = (item - kLead) / p.spe;
-    const int32_t i = (at - a * w.mult) / item;
+    if (item < kLead || s.n > p.total - s.first || at < start || at - start >= item * (p.H * tiles)) {
+        if (p.err && threadIdx.x == 0) atomicExch(p.err, 3);
+        s.begin = s.lo = at;
+        s.end = s.hi = max(at + 1, w.hi);
+        s.from = s.to = 0;
+        s.h = s.ct = 0;
+        s.n = -1;
+        return s;
+    }
+    const int32_t i = (at - start) / item;
     s.h = i / tiles;
     s.ct = i - s.h * tiles;
-    s.begin = a * w.mult + i * item;
+    s.begin = start + i * item;
     s.end = s.begin + item;
     s.lo = at;
     s.hi = item <= w.whole || s.end < w.hi ? s.end : w.hi;
@@ -425,7 +438,9 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             if (r < p.n_req) {
                 int q0, nq;
                 queries_of(p, r, q0, nq);
-                v[i] = (base_of(p, nullptr, r + 1) - base_of(p, nullptr, r)) * ((nq * p.G + X::kCols - 1) / X::kCols);
+                const int32_t units = base_of(p, nullptr, r + 1) - base_of(p, nullptr, r);
+                if (units < kLead && p.err) atomicExch(p.err, 3);         // (offsets that do not ascend)
+                v[i] = max(kLead, units) * ((nq * p.G + X::kCols - 1) / X::kCols);
             }
             sum += v[i];
         }
@@ -456,7 +471,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     probes[lane] = probe;
     __syncwarp();
     w.probes = probes;
-    const int32_t all = __shfl_sync(0xffffffffu, probe, 31) * w.mult;     // (a captured batch may use less than its capacity)
+    w.zero = __shfl_sync(0xffffffffu, probe, 0);
+    const int32_t all = max(0, __shfl_sync(0xffffffffu, probe, 31) - w.zero) * w.mult;     // (a captured batch may use less than its capacity)
     w.size = (int32_t)(((uint32_t)all + gridDim.x - 1u) / gridDim.x);     // (the host keeps all + grid below 2^31)
     w.lo = min(all, (int32_t)blockIdx.x * w.size);
     w.hi = w.lo + min(w.size, all - w.lo);
@@ -498,8 +514,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         int32_t id = p.block_ids ? __ldg(p.block_ids + ps.first + e) : -1;
         if (e >= p_entries || pos_block < 0) return;
         if (!p.block_ids) {
-            const int32_t t0 = __ldg(p.table_offsets + ps.r), t1 = __ldg(p.table_offsets + ps.r + 1);
-            if (pos_block >= t1 - t0) {
+            const int32_t t0 = __ldg(p.table_offsets + ps.r), t1 = min(__ldg(p.table_offsets + ps.r + 1), p.table_size);
+            if (t0 < 0 || pos_block >= t1 - t0) {
                 if (p.err) atomicExch(p.err, 3);
                 return;
             }
@@ -621,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         at = sg.hi;
         int q0, nq;
         queries_of(p, sg.r, q0, nq);
-        const int cols = min(X::kCols, nq * p.G - sg.ct * X::kCols);      // may be <= 0: nothing to write
+        const int cols = sg.n < 0 ? 0 : min(X::kCols, nq * p.G - sg.ct * X::kCols);      // may be <= 0: nothing to write
         const int c0 = sg.ct * X::kCols;
         // first position that each of the thread's columns may not see
         int32_t limit[NT][2], limit_min = INT32_MAX;

@@ -59,7 +59,7 @@ class BlockLists(C.Structure):
     """ucmx_block_lists: which blocks each request's queries attend to."""
     _fields_ = [("offsets", C.c_void_p), ("counts", C.c_void_p), ("block_ids", C.c_void_p), ("positions", C.c_void_p),
                 ("table", C.c_void_p), ("table_offsets", C.c_void_p), ("ctx_lens", C.c_void_p), ("n_req", C.c_int32),
-                ("total", C.c_int32)]
+                ("total", C.c_int32), ("table_size", C.c_int32)]
 
 
 _vp, _i32, _i64, _f32, _sz = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_size_t

@@ -682,7 +682,7 @@ def _attend(name: str, fn, bits: int, n_kv_heads: int, head_dim: int, cache_args
     lists = N.BlockLists(_index(req_offsets, "req_offsets", dev), _index(req_counts, "req_counts", dev, n_req),
                          _index(block_ids, "block_ids", dev, total), _index(positions, "positions", dev, total),
                          _index(block_table, "block_table", dev), _index(table_offsets, "table_offsets", dev, n_req + 1),
-                         _index(ctx_lens, "ctx_lens", dev, n_req), n_req, total)
+                         _index(ctx_lens, "ctx_lens", dev, n_req), n_req, total, 0 if block_table is None else block_table.numel())
     q_off = _index(q_offsets, "q_offsets", dev, n_req + 1)
     if q_offsets is None and (n_tok != n_req or max_q_tokens != 1):
         raise ValueError("without q_offsets there is one query token per request")
