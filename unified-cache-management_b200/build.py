@@ -97,13 +97,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_python_front() -> str:
-    """gcc: the CPython module that fronts ucmx_retrieval_* (no CUDA, no link against libucmx.so)."""
+    """gcc: the CPython module in front of the calls made per layer and step (no CUDA, no link against libucmx.so)."""
     import numpy
     cc = os.environ.get("CC") or shutil.which("gcc") or shutil.which("cc")
     if not cc:
         raise RuntimeError("no C compiler found (set CC)")
     cmd = [cc, "-O2", "-fPIC", "-shared", "-Wall", "-o", PY_OUT, PY_SRC,
-           "-I", sysconfig.get_paths()["include"], "-I", numpy.get_include()]
+           "-I", sysconfig.get_paths()["include"], "-I", numpy.get_include(), "-I", INCLUDE]
     subprocess.run(cmd, check=True)
     return PY_OUT
 

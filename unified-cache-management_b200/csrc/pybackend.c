@@ -8,12 +8,18 @@
  * once (bind), so the C ABI stays the only boundary.  ucmx.retrieval.RetrievalWorkerBackend derives from the type
  * defined here, so the three methods are called without a Python frame in between.  Arrays that are not plain
  * C-contiguous float32 / int32 go to the subclass's _submit_converted, which converts and calls submit again; a status
- * other than success goes to the callable given to bind, which raises what the ctypes route raises. */
+ * other than success goes to the callable given to bind, which raises what the ctypes route raises.
+ *
+ * block_attention and quant_block_attention are the same for the two attention entries of the C ABI (ucmx/ops.py): all
+ * arguments as plain numbers, the structures are filled in here.  Through ctypes the structures and the call took 5 us, a
+ * quarter of a short decode step's call. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #define NPY_NO_DEPRECATED_API NPY_1_7_API_VERSION
 #include <numpy/arrayobject.h>
 #include <stdint.h>
+
+#include "ucmx.h"
 
 typedef int32_t (*submit_fn)(void*, const float*, int32_t, int32_t, int32_t, const int32_t*, int32_t, int32_t*);
 typedef int32_t (*wait_fn)(void*, int32_t);
@@ -26,8 +32,6 @@ static get_fn g_get;
 static shape_fn g_shape;
 static PyObject* g_on_error;   /* callable(function name, status): raises */
 static PyObject *g_key_indices, *g_key_scores;   /* the result dictionary's keys, made once */
-
-#define UCMX_ENOOBJ (-50005)
 
 static PyObject* raise_status(const char* fn, int32_t st)
 {
@@ -229,10 +233,107 @@ static PyObject* mod_bind(PyObject* self, PyObject* args)
     Py_RETURN_NONE;
 }
 
-static PyMethodDef mod_methods[] = {{"bind", mod_bind, METH_VARARGS, "bind(submit, wait, get_result, result_shape addresses, on_error)"},
+typedef int32_t (*attend_fn)(const void*, int64_t, int32_t, const int32_t*, int32_t, int32_t, const void*, const ucmx_kv_geometry*, const void*,
+                             const ucmx_kv_geometry*, const ucmx_block_lists*, float, void*, float*, void*, size_t, ucmx_stream_t);
+typedef int32_t (*quant_attend_fn)(const void*, int64_t, int32_t, const int32_t*, int32_t, int32_t, const void*, const ucmx_quant_geometry*,
+                                   const ucmx_block_lists*, float, void*, float*, void*, size_t, ucmx_stream_t);
+
+/* what both calls take behind the cache: ten numbers of the lists' addresses and sizes, then scale, out, lse, workspace, its
+ * bytes and the stream; before it: the entry's address, then q, its stride, heads, q_offsets, tokens, tokens per request */
+#define ATTEND_HEAD 7
+#define ATTEND_TAIL 16
+
+static int read_numbers(PyObject* const* args, Py_ssize_t n, Py_ssize_t skip, int64_t* v)
+{
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (i == skip) continue;
+        const unsigned long long u = PyLong_AsUnsignedLongLongMask(args[i]);
+        if (u == (unsigned long long)-1 && PyErr_Occurred()) return -1;
+        v[i] = (int64_t)u;
+    }
+    return 0;
+}
+
+static ucmx_block_lists lists_of(const int64_t* v)
+{
+    ucmx_block_lists l;
+    l.offsets = (const int32_t*)(uintptr_t)v[0];
+    l.counts = (const int32_t*)(uintptr_t)v[1];
+    l.block_ids = (const int32_t*)(uintptr_t)v[2];
+    l.positions = (const int32_t*)(uintptr_t)v[3];
+    l.table = (const int32_t*)(uintptr_t)v[4];
+    l.table_offsets = (const int32_t*)(uintptr_t)v[5];
+    l.ctx_lens = (const int32_t*)(uintptr_t)v[6];
+    l.n_req = (int32_t)v[7];
+    l.total = (int32_t)v[8];
+    l.table_size = (int32_t)v[9];
+    return l;
+}
+
+static ucmx_kv_geometry geometry_of(const int64_t* v)
+{
+    const ucmx_kv_geometry g = {v[0], v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4], (int32_t)v[5]};
+    return g;
+}
+
+/* block_attention(entry, q, q_stride, heads, q_offsets, tokens, max_q, k, six numbers of its geometry, v, six numbers, ten of the
+ * lists, scale, out, lse, workspace, bytes, stream) -> status */
+static PyObject* mod_block_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs)
+{
+    enum { kCache = 14, kN = ATTEND_HEAD + kCache + ATTEND_TAIL, kScale = kN - 6 };
+    int64_t v[kN];
+    (void)self;
+    if (nargs != kN) {
+        PyErr_SetString(PyExc_TypeError, "block_attention: wrong number of arguments");
+        return NULL;
+    }
+    const double scale = PyFloat_AsDouble(args[kScale]);
+    if ((scale == -1.0 && PyErr_Occurred()) || read_numbers(args, kN, kScale, v) < 0) return NULL;
+    const ucmx_kv_geometry kg = geometry_of(v + 8), vg = geometry_of(v + 15);
+    const ucmx_block_lists l = lists_of(v + ATTEND_HEAD + kCache);
+    const int64_t* t = v + kScale;
+    const attend_fn f = (attend_fn)(uintptr_t)v[0];
+    int32_t st;
+    Py_BEGIN_ALLOW_THREADS;       /* a launch waits where the stream's queue is full */
+    st = f((const void*)(uintptr_t)v[1], v[2], (int32_t)v[3], (const int32_t*)(uintptr_t)v[4], (int32_t)v[5], (int32_t)v[6],
+           (const void*)(uintptr_t)v[7], &kg, (const void*)(uintptr_t)v[14], &vg, &l, (float)scale, (void*)(uintptr_t)t[1],
+           (float*)(uintptr_t)t[2], (void*)(uintptr_t)t[3], (size_t)t[4], (ucmx_stream_t)(uintptr_t)t[5]);
+    Py_END_ALLOW_THREADS;
+    return PyLong_FromLong(st);
+}
+
+/* quant_block_attention(entry, q, q_stride, heads, q_offsets, tokens, max_q, cache, six numbers of its geometry, the rest as above) */
+static PyObject* mod_quant_block_attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs)
+{
+    enum { kCache = 7, kN = ATTEND_HEAD + kCache + ATTEND_TAIL, kScale = kN - 6 };
+    int64_t v[kN];
+    (void)self;
+    if (nargs != kN) {
+        PyErr_SetString(PyExc_TypeError, "quant_block_attention: wrong number of arguments");
+        return NULL;
+    }
+    const double scale = PyFloat_AsDouble(args[kScale]);
+    if ((scale == -1.0 && PyErr_Occurred()) || read_numbers(args, kN, kScale, v) < 0) return NULL;
+    const ucmx_quant_geometry g = {v[8], v[9], (int32_t)v[10], (int32_t)v[11], (int32_t)v[12], (int32_t)v[13]};
+    const ucmx_block_lists l = lists_of(v + ATTEND_HEAD + kCache);
+    const int64_t* t = v + kScale;
+    const quant_attend_fn f = (quant_attend_fn)(uintptr_t)v[0];
+    int32_t st;
+    Py_BEGIN_ALLOW_THREADS;
+    st = f((const void*)(uintptr_t)v[1], v[2], (int32_t)v[3], (const int32_t*)(uintptr_t)v[4], (int32_t)v[5], (int32_t)v[6],
+           (const void*)(uintptr_t)v[7], &g, &l, (float)scale, (void*)(uintptr_t)t[1], (float*)(uintptr_t)t[2],
+           (void*)(uintptr_t)t[3], (size_t)t[4], (ucmx_stream_t)(uintptr_t)t[5]);
+    Py_END_ALLOW_THREADS;
+    return PyLong_FromLong(st);
+}
+
+static PyMethodDef mod_methods[] = {{"block_attention", (PyCFunction)(void (*)(void))mod_block_attention, METH_FASTCALL, "ucmx_block_attention"},
+                                    {"quant_block_attention", (PyCFunction)(void (*)(void))mod_quant_block_attention, METH_FASTCALL,
+                                     "ucmx_quant_block_attention"},
+                                    {"bind", mod_bind, METH_VARARGS, "bind(submit, wait, get_result, result_shape addresses, on_error)"},
                                     {NULL, NULL, 0, NULL}};
 
-static struct PyModuleDef moddef = {PyModuleDef_HEAD_INIT, "_ucmx_fast", "CPython front of ucmx_retrieval_*", -1, mod_methods,
+static struct PyModuleDef moddef = {PyModuleDef_HEAD_INIT, "_ucmx_fast", "CPython front of the calls that are made per layer and step", -1, mod_methods,
                                     NULL, NULL, NULL, NULL};
 
 PyMODINIT_FUNC PyInit__ucmx_fast(void)

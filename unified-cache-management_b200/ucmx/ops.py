@@ -12,6 +12,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _native as N
+from .retrieval import _fast
 from ._native import (DT_BF16, DT_F32, DT_I32, ORDER_INDEX_ASC, ORDER_SCORE_DESC, POOL_MAX,  # noqa: F401
                       POOL_MEAN, POOL_MIN, POOL_SUM, WIN_EXCLUDE, WIN_FORCE, WIN_NONE)
 
@@ -45,15 +46,19 @@ def _i32(t: Optional[torch.Tensor], name: str) -> Optional[torch.Tensor]:
     return t
 
 
-def kv_geometry(k_cache: torch.Tensor) -> N.KvGeometry:
-    """Geometry of a paged cache tensor [num_blocks, block_tokens, n_kv_heads, head_dim] (bf16)."""
+def _kv_numbers(k_cache: torch.Tensor) -> tuple:
     if k_cache.dim() != 4 or k_cache.dtype != torch.bfloat16:
         raise ValueError("k_cache must be bf16 [num_blocks, block_tokens, n_kv_heads, head_dim]")
     nb, T, H, D = k_cache.shape
     sb, st, sh, sd = k_cache.stride()
     if sd != 1 or sh != D:
         raise ValueError("heads and head_dim of the paged cache must be contiguous")
-    return N.KvGeometry(sb, st, T, H, D, nb)
+    return sb, st, T, H, D, nb
+
+
+def kv_geometry(k_cache: torch.Tensor) -> N.KvGeometry:
+    """Geometry of a paged cache tensor [num_blocks, block_tokens, n_kv_heads, head_dim] (bf16)."""
+    return N.KvGeometry(*_kv_numbers(k_cache))
 
 
 def pool_blocks(k_cache: torch.Tensor, block_ids: torch.Tensor, *, mode: str = "mean",
@@ -521,7 +526,8 @@ class QuantKvCache:
         nb, H, groups, gb = data.shape
         if data.stride()[1:] != (groups * gb, gb, 1):
             raise ValueError("each block of the quantised cache must be contiguous")
-        self.geometry = N.QuantGeometry(nb, data.stride(0) if nb > 1 else H * groups * gb, groups * 16, H, head_dim, bits)
+        self.numbers = (nb, data.stride(0) if nb > 1 else H * groups * gb, groups * 16, H, head_dim, bits)
+        self.geometry = N.QuantGeometry(*self.numbers)
         if N.lib.ucmx_quant_block_bytes(C.byref(self.geometry)) != H * groups * gb:
             raise ValueError("bits must be 4 or 8, head_dim 64, 128 or 256, and the last dimension the bytes of a 16-token group")
         self.data = data
@@ -640,6 +646,8 @@ def quant_read_blocks(cache: QuantKvCache, block_ids: torch.Tensor, *, k_out: Op
     return k_out, v_out
 
 
+_BLOCK_ATTENTION, _QUANT_BLOCK_ATTENTION = (C.cast(f, C.c_void_p).value for f in
+                                            (N.lib.ucmx_block_attention, N.lib.ucmx_quant_block_attention))
 _workspace_bytes = {}     # (device, bits, query heads, KV heads, head_dim, query tokens) -> bytes
 
 
@@ -657,7 +665,7 @@ def attention_workspace(query: torch.Tensor, n_kv_heads: int, *, max_q_tokens: i
     return torch.empty(need, dtype=torch.uint8, device=query.device)
 
 
-def _attend(name: str, fn, bits: int, n_kv_heads: int, head_dim: int, cache_args, cache, query, req_offsets, block_ids, positions,
+def _attend(name: str, front, entry: int, bits: int, n_kv_heads: int, head_dim: int, cache_args, cache, query, req_offsets, block_ids, positions,
             block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out, lse, workspace):
     _need_device(query, cache, out, lse, workspace)
     dev = query.device
@@ -679,10 +687,10 @@ def _attend(name: str, fn, bits: int, n_kv_heads: int, head_dim: int, cache_args
     if block_ids is not None and (block_table is not None or table_offsets is not None):
         raise ValueError("give block_ids or block_table with table_offsets, not both")
     total = entries.numel()
-    lists = N.BlockLists(_index(req_offsets, "req_offsets", dev), _index(req_counts, "req_counts", dev, n_req),
-                         _index(block_ids, "block_ids", dev, total), _index(positions, "positions", dev, total),
-                         _index(block_table, "block_table", dev), _index(table_offsets, "table_offsets", dev, n_req + 1),
-                         _index(ctx_lens, "ctx_lens", dev, n_req), n_req, total, 0 if block_table is None else block_table.numel())
+    lists = (_index(req_offsets, "req_offsets", dev), _index(req_counts, "req_counts", dev, n_req),
+             _index(block_ids, "block_ids", dev, total), _index(positions, "positions", dev, total),
+             _index(block_table, "block_table", dev), _index(table_offsets, "table_offsets", dev, n_req + 1),
+             _index(ctx_lens, "ctx_lens", dev, n_req), n_req, total, 0 if block_table is None else block_table.numel())
     q_off = _index(q_offsets, "q_offsets", dev, n_req + 1)
     if q_offsets is None and (n_tok != n_req or max_q_tokens != 1):
         raise ValueError("without q_offsets there is one query token per request")
@@ -697,9 +705,9 @@ def _attend(name: str, fn, bits: int, n_kv_heads: int, head_dim: int, cache_args
     if workspace is None:
         workspace = attention_workspace(query, n_kv_heads, max_q_tokens=max_q_tokens, bits=bits)
     with _on_device(query):
-        st = fn(query.data_ptr(), q_stride, Hq, q_off, n_tok, max_q_tokens, *cache_args, C.byref(lists),
-                D ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(),
-                workspace.nbytes, _raw_stream(dev.index))
+        st = front(entry, query.data_ptr(), q_stride, Hq, q_off, n_tok, max_q_tokens, *cache_args, *lists,
+                   D ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(),
+                   workspace.nbytes, _raw_stream(dev.index))
     N.check(name, st, 2)
     return out
 
@@ -722,11 +730,11 @@ def block_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     sees n-1-j fewer.  Without it every token of every listed block is seen.
     q_offsets, max_q_tokens: each request's query tokens (one each without).  A query that sees nothing gives zeros.
     lse: fp32 [n_query_tokens, n_q_heads], receives the logarithm of the softmax's sum.  scale defaults to head_dim ** -0.5."""
-    kg, vg = kv_geometry(k_cache), kv_geometry(v_cache)
+    kg, vg = _kv_numbers(k_cache), _kv_numbers(v_cache)
     if v_cache.device != k_cache.device:
         raise ValueError("all tensors of a call must be on the same CUDA device")
-    args = (k_cache.data_ptr(), C.byref(kg), v_cache.data_ptr(), C.byref(vg))
-    return _attend("ucmx_block_attention", N.lib.ucmx_block_attention, 16, kg.n_kv_heads, kg.head_dim, args, k_cache, query, req_offsets, block_ids, positions,
+    args = (k_cache.data_ptr(), *kg, v_cache.data_ptr(), *vg)
+    return _attend("ucmx_block_attention", _fast.block_attention, _BLOCK_ATTENTION, 16, kg[3], kg[4], args, k_cache, query, req_offsets, block_ids, positions,
                    block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out, lse, workspace)
 
 
@@ -738,7 +746,7 @@ def quant_block_attention(query: torch.Tensor, cache: QuantKvCache, req_offsets:
                           out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
                           workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
     """block_attention over a quantised cache: the codes are read in place and never written out as bf16."""
-    g = cache.geometry
-    return _attend("ucmx_quant_block_attention", N.lib.ucmx_quant_block_attention, g.bits, g.n_kv_heads, g.head_dim,
-                   (cache.data.data_ptr(), C.byref(g)), cache.data, query, req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out,
+    g = cache.numbers
+    return _attend("ucmx_quant_block_attention", _fast.quant_block_attention, _QUANT_BLOCK_ATTENTION, g[5], g[3], g[4],
+                   (cache.data.data_ptr(), *g), cache.data, query, req_offsets, block_ids, positions, block_table, table_offsets, ctx_lens, req_counts, q_offsets, max_q_tokens, scale, out,
                    lse, workspace)
