@@ -4,7 +4,8 @@
 // scale), L = 15 or 255; the layout is described at ucmx_quant_geometry.  All three kernels are streams: a row of 128 values is
 // 256 bytes on the bf16 side and 68 (132) on the other, with one reduction over the lanes that hold it in between.
 //
-// Eight or sixteen values per lane, so that a row is 8 or 16 lanes and a warp holds two or four neighbouring tokens of one head.
+// Sixteen values per lane in pieces of eight (what 16 bytes hold), so that a row is 4, 8 or 16 lanes and a warp holds eight, four
+// or two neighbouring tokens of one head: what is done once per row is shared by that many.
 // V's layout puts the codes of tokens 2i and 2i+1 side by side in pairs of bytes: neighbouring rows of the warp exchange words, so
 // that V moves in 32-bit words like K (a token whose partner is not in the call stores 16-bit pieces).
 //
@@ -23,10 +24,11 @@ template <int BITS, int D>
 struct Q {
     static constexpr int kRowBytes = D * BITS / 8;
     static constexpr int kPanel = kRowBytes < 64 ? kRowBytes : 64;
-    static constexpr int kDims = D == 256 ? 16 : 8;      // values a lane holds
+    static constexpr int kPieces = 2;                    // pieces of 8 values a lane holds: lr, lr + kLanes
+    static constexpr int kDims = 8 * kPieces;
     static constexpr int kLanes = D / kDims;             // lanes of a row
     static constexpr int kTokens = 32 / kLanes;          // rows of a warp: neighbouring tokens of one head
-    static constexpr int kWords = kDims * BITS / 32;     // code words of a lane
+    static constexpr int kWords = BITS / 4;              // code words of a piece
     static constexpr int kGroup = 2 * kRows * kRowBytes + 2 * kRows * 4;
     static constexpr int kTop = (1 << BITS) - 1;
 };
@@ -94,27 +96,30 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b)
 }
 
 // Settles a code whose residual is half a step or more.  c: the code so far; v, lo: the value and the row's smallest.
-__device__ __noinline__ float settle(float c, float v, float lo, float half_scale)
+__device__ __forceinline__ float settle(float c, float v, float lo, float half_scale)
 {
     const float a = 0.5f * v, b = -0.5f * lo, hx = a + b;
     const float r = fmaf(-c, half_scale, hx);
-    if (fabsf(r) > 0.5f * half_scale) return r > 0.f ? c + 1.f : c - 1.f;
-    // a tie of the rounded difference: which side the exact one lies on (as far as fp64 would see it), else the even code
     const float bb = hx - a;
-    const float err = (a - (hx - bb)) + (b - bb);
-    const float unit = __uint_as_float(__float_as_uint(hx) & 0x7f800000u) * 1.1102230246251565e-16f;     // 2^-53 of hx's power of two
-    const float low = r > 0.f ? c : c - 1.f;
-    if (err > unit) return low + 1.f;
-    if (err < -unit) return low;
-    return (int)low & 1 ? low + 1.f : low;
+    const float err = (a - (hx - bb)) + (b - bb);        // what the difference was rounded by
+    const float to = r > 0.f ? 1.f : -1.f;
+    bool move = fabsf(r) > 0.5f * half_scale;
+    if (!move) {                                         // a tie of the rounded difference
+        move = __float_as_uint(c + kMagic) & 1u;         // of an exact one: the even code
+        if (err != 0.f) {                                // which side the exact difference lies on (as far as fp64 would see it)
+            const float unit = __uint_as_float(__float_as_uint(hx) & 0x7f800000u) * 1.1102230246251565e-16f;     // 2^-53 of hx's power of two
+            if (fabsf(err) > unit) move = (err > 0.f) == (r > 0.f);
+        }
+    }
+    return move ? c + to : c;
 }
 
-// byte offset of a lane's codes inside K's part of a group / of unit u (2 bytes of a row) inside V's part
+// byte offset of piece `pc` of a row (8 values) inside K's part of a group / of unit u (2 bytes of a row) inside V's part
 template <int BITS, int D>
-__device__ __forceinline__ int k_at(int t, int lr)
+__device__ __forceinline__ int k_at(int t, int pc)
 {
     using X = Q<BITS, D>;
-    const int b = lr * X::kWords * 4;
+    const int b = pc * X::kWords * 4;
     return (b / X::kPanel) * (kRows * X::kPanel) + t * X::kPanel + b % X::kPanel;
 }
 template <int BITS, int D>
@@ -145,7 +150,7 @@ __device__ __forceinline__ Piece piece_of(uint32_t item, uint32_t head_chunks)
 
 // HC heads of one token group per warp, their loads all in flight at once.
 template <int BITS, int D, bool BLOCKS, int HC>
-__global__ void __launch_bounds__(256, D == 256 ? 3 : 4) quant_write_kernel(const QuantParams p)
+__global__ void __launch_bounds__(256, 4) quant_write_kernel(const QuantParams p)
 {
     using X = Q<BITS, D>;
     const int lane = threadIdx.x & 31, lr = lane % X::kLanes, row = lane / X::kLanes;
@@ -179,13 +184,13 @@ __global__ void __launch_bounds__(256, D == 256 ? 3 : 4) quant_write_kernel(cons
         src += i * (x.kv ? p.v_token : p.k_token);
     }
     const bool live = block >= 0;
-    src += (int64_t)x.h * D + lr * X::kDims;
-    uint4 raw[HC][X::kDims / 8];
+    src += (int64_t)x.h * D + lr * 8;
+    uint4 raw[HC][X::kPieces];
 #pragma unroll
     for (int c = 0; c < HC; ++c)
 #pragma unroll
-        for (int i = 0; i < X::kDims / 8; ++i)
-            raw[c][i] = live && x.h + c < p.H ? ld_stream16(src + c * D + i * 8) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < X::kPieces; ++i)
+            raw[c][i] = live && x.h + c < p.H ? ld_stream16(src + c * D + i * X::kLanes * 8) : make_uint4(0, 0, 0, 0);
     // is the neighbouring row the other token of a pair?
     const int64_t place = live ? block * p.T + t : -2 - row;
     const int64_t other = __shfl_xor_sync(0xffffffffu, place, X::kLanes);
@@ -199,7 +204,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 3 : 4) quant_write_kernel(cons
     for (int c = 0; c < HC; ++c) {
         uint32_t hi2 = raw[c][0].x, lo2 = raw[c][0].x;
 #pragma unroll
-        for (int i = 0; i < X::kDims / 8; ++i) {
+        for (int i = 0; i < X::kPieces; ++i) {
             hi2 = max2(max2(max2(max2(hi2, raw[c][i].x), raw[c][i].y), raw[c][i].z), raw[c][i].w);
             lo2 = min2(min2(min2(min2(lo2, raw[c][i].x), raw[c][i].y), raw[c][i].z), raw[c][i].w);
         }
@@ -228,86 +233,76 @@ __global__ void __launch_bounds__(256, D == 256 ? 3 : 4) quant_write_kernel(cons
         const uint32_t sz = HC == 1 ? my_sz : __shfl_sync(0xffffffffu, my_sz, row * X::kLanes + c);
         const float inv = HC == 1 ? my_inv : __shfl_sync(0xffffffffu, my_inv, row * X::kLanes + c);
         const float scale = bf16lo(sz), half_scale = 0.5f * scale, lo = bf16hi(sz), half_lo = 0.5f * lo;
-        uint32_t q[X::kDims / 2];
+        const float half = 0.5f * half_scale, most = (float)X::kTop * half_scale;
+        uint8_t* const part = group + kRows * X::kRowBytes;
 #pragma unroll
-        for (int i = 0; i < X::kDims / 8; ++i) {
-            q[4 * i] = raw[c][i].x;
-            q[4 * i + 1] = raw[c][i].y;
-            q[4 * i + 2] = raw[c][i].z;
-            q[4 * i + 3] = raw[c][i].w;
-        }
-        // ---- codes, as floats
-        float f[X::kDims];
-        if (scale > 0.f) {                               // (not for a scale of 0, not for NaN)
-            const bool tiny = scale < 1e-30f;            // the reciprocal would leave the range: everything in fp64
-            const float most = (float)X::kTop * half_scale;
-            const float half = 0.5f * half_scale;
-            float worst = 0.f;
-            float e[X::kDims];
+        for (int pc = 0; pc < X::kPieces; ++pc) {
+            const uint32_t q[4] = {raw[c][pc].x, raw[c][pc].y, raw[c][pc].z, raw[c][pc].w};
+            auto value = [&](int i) { return i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]); };
+            // ---- codes, as floats
+            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (scale >= 1e-30f) {
+                float worst = 0.f, e[8];
 #pragma unroll
-            for (int i = 0; i < X::kDims; i += 2) {
-                F2 hx = fma2({bf16lo(q[i / 2]), bf16hi(q[i / 2])}, {0.5f, 0.5f}, {-half_lo, -half_lo});
-                if (BITS == 8) {                         // 255 steps of a scale that was rounded down may end beyond 255.5; 15 cannot
-                    hx.x = fminf(hx.x, most);
-                    hx.y = fminf(hx.y, most);
+                for (int i = 0; i < 8; i += 2) {
+                    F2 hx = fma2({value(i), value(i + 1)}, {0.5f, 0.5f}, {-half_lo, -half_lo});
+                    if (BITS == 8) {                     // 255 steps of a scale that was rounded down may end beyond 255.5; 15 cannot
+                        hx.x = fminf(hx.x, most);
+                        hx.y = fminf(hx.y, most);
+                    }
+                    const F2 d = add2(fma2(hx, {inv, inv}, {kMagic, kMagic}), {-kMagic, -kMagic});
+                    const F2 r = fma2(d, {-half_scale, -half_scale}, hx);
+                    f[i] = d.x;
+                    f[i + 1] = d.y;
+                    e[i] = fabsf(r.x);
+                    e[i + 1] = fabsf(r.y);
+                    worst = fmaxf(worst, fmaxf(e[i], e[i + 1]));
                 }
-                const F2 c = add2(fma2(hx, {inv, inv}, {kMagic, kMagic}), {-kMagic, -kMagic});
-                const F2 r = fma2(c, {-half_scale, -half_scale}, hx);
-                f[i] = c.x;
-                f[i + 1] = c.y;
-                e[i] = fabsf(r.x);
-                e[i + 1] = fabsf(r.y);
-                worst = fmaxf(worst, fmaxf(e[i], e[i + 1]));
-            }
-            if (tiny) {
+                if (worst >= half) {
 #pragma unroll
-                for (int i = 0; i < X::kDims; ++i) {
-                    const float v = i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]);
-                    f[i] = (float)fmin(rint(((double)v - (double)lo) / (double)scale), (double)X::kTop);
+                    for (int i = 0; i < 8; ++i)
+                        if (e[i] >= half) f[i] = settle(f[i], value(i), lo, half_scale);
                 }
-            } else if (worst >= half) {
+            } else if (scale > 0.f) {                    // the reciprocal would leave the range: in fp64.  (Neither: a scale of 0, or NaN)
 #pragma unroll
-                for (int i = 0; i < X::kDims; ++i)
-                    if (e[i] >= half) f[i] = settle(f[i], i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]), lo, half_scale);
+                for (int i = 0; i < 8; ++i)
+                    f[i] = (float)fmin(rint(((double)value(i) - (double)lo) / (double)scale), (double)X::kTop);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < X::kDims; ++i) f[i] = 0.f;
-        }
-        // ---- 16 bits at a time: the codes side by side in one float of 2^23
-        uint32_t w[X::kWords];
-        constexpr int kIn16 = 16 / BITS;
-#pragma unroll
-        for (int i = 0; i < X::kWords; ++i) {
-            uint32_t part[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float a = kMagic + f[(2 * i + j) * kIn16];
-#pragma unroll
-                for (int k = 1; k < kIn16; ++k) a = fmaf(f[(2 * i + j) * kIn16 + k], (float)(1 << (BITS * k)), a);
-                part[j] = __float_as_uint(a);
-            }
-            w[i] = __byte_perm(part[0], part[1], 0x5410);
-        }
-        if (x.kv == 0) {
-            if (live) {
-                uint8_t* const d = group + k_at<BITS, D>(tt, lr);
-                if (X::kWords == 1) *reinterpret_cast<uint32_t*>(d) = w[0];
-                if (X::kWords == 2) *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[X::kWords - 1]);
-                if (X::kWords == 4) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1 % X::kWords], w[2 % X::kWords], w[3 % X::kWords]);
-            }
-        } else {
-            uint8_t* const part = group + kRows * X::kRowBytes;
+            // ---- 16 bits at a time: the codes side by side in one float of 2^23
+            uint32_t w[X::kWords];
+            constexpr int kIn16 = 16 / BITS;
 #pragma unroll
             for (int i = 0; i < X::kWords; ++i) {
-                const uint32_t y = __shfl_xor_sync(0xffffffffu, w[i], X::kLanes);
-                const int u = (lr * X::kWords + i) * 2;
-                if (paired) {
-                    const uint32_t z = __byte_perm(w[i], y, (row & 1) ? 0x3276 : 0x5410);
-                    *reinterpret_cast<uint32_t*>(part + v_at<BITS, D>(tt & ~1, u + (row & 1))) = z;
-                } else if (live) {
-                    *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u)) = (uint16_t)w[i];
-                    *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u + 1)) = (uint16_t)(w[i] >> 16);
+                uint32_t half[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int at = (2 * i + j) * kIn16;
+                    float a = kMagic + f[at];
+#pragma unroll
+                    for (int k = 1; k < kIn16; ++k) a = fmaf(f[at + k], (float)(1 << (BITS * k)), a);
+                    half[j] = __float_as_uint(a);
+                }
+                w[i] = __byte_perm(half[0], half[1], 0x5410);
+            }
+            const int piece = pc * X::kLanes + lr;
+            if (x.kv == 0) {
+                if (live) {
+                    uint8_t* const d = group + k_at<BITS, D>(tt, piece);
+                    if (X::kWords == 1) *reinterpret_cast<uint32_t*>(d) = w[0];
+                    else *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[X::kWords - 1]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < X::kWords; ++i) {
+                    const uint32_t y = __shfl_xor_sync(0xffffffffu, w[i], X::kLanes);
+                    const int u = (piece * X::kWords + i) * 2;
+                    if (paired) {
+                        *reinterpret_cast<uint32_t*>(part + v_at<BITS, D>(tt & ~1, u + (row & 1))) =
+                            __byte_perm(w[i], y, (row & 1) ? 0x3276 : 0x5410);
+                    } else if (live) {
+                        *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u)) = (uint16_t)w[i];
+                        *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u + 1)) = (uint16_t)(w[i] >> 16);
+                    }
                 }
             }
         }
@@ -333,67 +328,60 @@ __global__ void __launch_bounds__(256) quant_read_kernel(const QuantParams p)
     const int group_step = (p.T / kRows) * X::kGroup;
     const uint8_t* const group = p.cache + (int64_t)id * p.block_stride + (int64_t)x.h * group_step + (t / kRows) * X::kGroup;
     const int tt = t % kRows;
-    uint32_t w[HC][X::kWords], sz[HC];
+    uint32_t w[HC][X::kPieces][X::kWords], sz[HC];
 #pragma unroll
     for (int c = 0; c < HC; ++c) {
         if (x.h + c >= p.H) break;
         const uint8_t* const g = group + c * group_step;
-        if (x.kv == 0) {
-            const uint8_t* const s = g + k_at<BITS, D>(tt, lr);
-            if (X::kWords == 1) w[c][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
-            if (X::kWords == 2) {
-                const uint2 y = __ldg(reinterpret_cast<const uint2*>(s));
-                w[c][0] = y.x;
-                w[c][X::kWords - 1] = y.y;
-            }
-            if (X::kWords == 4) {
-                const uint4 y = __ldg(reinterpret_cast<const uint4*>(s));
-                w[c][0] = y.x;
-                w[c][1 % X::kWords] = y.y;
-                w[c][2 % X::kWords] = y.z;
-                w[c][3 % X::kWords] = y.w;
-            }
-        } else {
 #pragma unroll
-            for (int j = 0; j < X::kWords; ++j)
-                w[c][j] = __ldg(reinterpret_cast<const uint32_t*>(g + kRows * X::kRowBytes +
-                                                                   v_at<BITS, D>(tt & ~1, (lr * X::kWords + j) * 2 + (row & 1))));
+        for (int pc = 0; pc < X::kPieces; ++pc) {
+            const int piece = pc * X::kLanes + lr;
+            if (x.kv == 0) {
+                const uint8_t* const s = g + k_at<BITS, D>(tt, piece);
+                if (X::kWords == 1) {
+                    w[c][pc][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+                } else {
+                    const uint2 y = __ldg(reinterpret_cast<const uint2*>(s));
+                    w[c][pc][0] = y.x;
+                    w[c][pc][X::kWords - 1] = y.y;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < X::kWords; ++j)
+                    w[c][pc][j] = __ldg(reinterpret_cast<const uint32_t*>(g + kRows * X::kRowBytes +
+                                                                           v_at<BITS, D>(tt & ~1, (piece * X::kWords + j) * 2 + (row & 1))));
+            }
         }
         sz[c] = __ldg(reinterpret_cast<const uint32_t*>(g + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4));
     }
     uint16_t* const dst = const_cast<uint16_t*>(x.kv ? p.v : p.k) + out * (x.kv ? p.v_block : p.k_block) +
-                          (int64_t)t * (x.kv ? p.v_token : p.k_token) + (int64_t)x.h * D + lr * X::kDims;
+                          (int64_t)t * (x.kv ? p.v_token : p.k_token) + (int64_t)x.h * D + lr * 8;
 #pragma unroll
     for (int c = 0; c < HC; ++c) {
         if (x.h + c >= p.H) break;
-        if (x.kv) {
+        const float scale = bf16lo(sz[c]), zero = bf16hi(sz[c]);
+#pragma unroll
+        for (int pc = 0; pc < X::kPieces; ++pc) {
+            float f[8];
 #pragma unroll
             for (int j = 0; j < X::kWords; ++j) {
-                const uint32_t y = __shfl_xor_sync(0xffffffffu, w[c][j], X::kLanes);
-                w[c][j] = (row & 1) ? __byte_perm(y, w[c][j], 0x7632) : __byte_perm(w[c][j], y, 0x5410);
-            }
-        }
-        const float scale = bf16lo(sz[c]), zero = bf16hi(sz[c]);
-        float f[X::kDims];
+                uint32_t u = w[c][pc][j];
+                if (x.kv) u = __byte_perm(u, __shfl_xor_sync(0xffffffffu, u, X::kLanes), (row & 1) ? 0x3276 : 0x5410);
+                const uint32_t even = BITS == 4 ? u & 0x0f0f0f0fu : u, odd = BITS == 4 ? (u >> 4) & 0x0f0f0f0fu : 0u;
 #pragma unroll
-        for (int j = 0; j < X::kWords; ++j) {
-            const uint32_t even = BITS == 4 ? w[c][j] & 0x0f0f0f0fu : w[c][j], odd = BITS == 4 ? (w[c][j] >> 4) & 0x0f0f0f0fu : 0u;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float a = __uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + k)) - kMagic;
-                if (BITS == 4) {
-                    const float b = __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + k)) - kMagic;
-                    f[(j * 8 + 2 * k) % X::kDims] = fmaf(a, scale, zero);
-                    f[(j * 8 + 2 * k + 1) % X::kDims] = fmaf(b, scale, zero);
-                } else {
-                    f[(j * 4 + k) % X::kDims] = fmaf(a, scale, zero);
+                for (int k = 0; k < 4; ++k) {
+                    const float a = __uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + k)) - kMagic;
+                    if (BITS == 4) {
+                        const float b = __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + k)) - kMagic;
+                        f[2 * k] = fmaf(a, scale, zero);
+                        f[2 * k + 1] = fmaf(b, scale, zero);
+                    } else {
+                        f[(j * 4 + k) % 8] = fmaf(a, scale, zero);
+                    }
                 }
             }
+            st_stream16(dst + c * D + pc * X::kLanes * 8, make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7])));
         }
-#pragma unroll
-        for (int j = 0; j < X::kDims / 8; ++j)
-            st_stream16(dst + c * D + j * 8, make_uint4(pack2(f[8 * j], f[8 * j + 1]), pack2(f[8 * j + 2], f[8 * j + 3]),
-                                                        pack2(f[8 * j + 4], f[8 * j + 5]), pack2(f[8 * j + 6], f[8 * j + 7])));
     }
 }
 
@@ -422,9 +410,9 @@ int32_t launch(QuantParams& p, Form form, cudaStream_t st)
 {
     using X = Q<BITS, D>;
     const int64_t groups = form == kTokensForm ? (p.n + X::kTokens - 1) / X::kTokens : p.n * (p.T / X::kTokens);
-    // Four rows of a lane in flight (two of the double-width ones) as soon as that still gives every SM its warps; with the few
+    // Two heads of a warp in flight as soon as that still gives every SM its warps; with the few
     // tokens of a decode step one row per lane, over as many warps as there are rows.
-    constexpr int kMany = D == 256 ? 2 : 4;
+    constexpr int kMany = 2;
     if (groups * 2 * ((p.H + kMany - 1) / kMany) >= (int64_t)sm_count() * 32) return launch_heads<BITS, D, kMany>(p, form, groups, st);
     return launch_heads<BITS, D, 1>(p, form, groups, st);
 }
