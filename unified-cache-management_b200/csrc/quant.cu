@@ -13,6 +13,10 @@
 // overflow for any finite row.  A reciprocal, a rounding to the integers by adding 2^23, and the residual x - code*scale, which is
 // exact in fp32: where it is half a step or more (ties, and quotients the reciprocal put on the wrong side) the code is settled by
 // it and by what the difference x - zero was rounded by.  A division per value, and fp64 for the ties, were the bound of this kernel.
+//
+// Measured on a B200 (8 heads of 128 values): 300 blocks of 128 tokens to 8 bits in 79 us (3.0 TB/s of both sides' bytes; floor
+// 36 us), back in 42 us (5.7 TB/s); 8144 tokens to 4 bits in 21 us, back in 11 us.  Writing is bound by instructions (90 per row
+// and lane, 60 % of the issue slots), reading by HBM.
 #include "common.cuh"
 
 namespace ucmx {
@@ -410,8 +414,8 @@ int32_t launch(QuantParams& p, Form form, cudaStream_t st)
 {
     using X = Q<BITS, D>;
     const int64_t groups = form == kTokensForm ? (p.n + X::kTokens - 1) / X::kTokens : p.n * (p.T / X::kTokens);
-    // Two heads of a warp in flight as soon as that still gives every SM its warps; with the few
-    // tokens of a decode step one row per lane, over as many warps as there are rows.
+    // Two heads of a warp in flight as soon as that still gives every SM its 32 warps; with the few tokens of a decode step one head
+    // each, over twice as many warps.
     constexpr int kMany = 2;
     if (groups * 2 * ((p.H + kMany - 1) / kMany) >= (int64_t)sm_count() * 32) return launch_heads<BITS, D, kMany>(p, form, groups, st);
     return launch_heads<BITS, D, 1>(p, form, groups, st);
