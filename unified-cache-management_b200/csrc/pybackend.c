@@ -10,9 +10,9 @@
  * C-contiguous float32 / int32 go to the subclass's _submit_converted, which converts and calls submit again; a status
  * other than success goes to the callable given to bind, which raises what the ctypes route raises.
  *
- * block_attention and quant_block_attention are the same for the two attention entries of the C ABI (ucmx/ops.py): all
- * arguments as plain numbers, the structures are filled in here.  Through ctypes the structures and the call took 5 us, a
- * quarter of a short decode step's call. */
+ * block_attention, quant_block_attention and quant_write_tokens are the same for what a decode step calls per layer over a
+ * cache (ucmx/ops.py): all arguments as plain numbers, the structures are filled in here.  Through ctypes the structures
+ * and an attention call took 5 us, a quarter of a short decode step's call. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #define NPY_NO_DEPRECATED_API NPY_1_7_API_VERSION
@@ -327,7 +327,32 @@ static PyObject* mod_quant_block_attention(PyObject* self, PyObject* const* args
     return PyLong_FromLong(st);
 }
 
-static PyMethodDef mod_methods[] = {{"block_attention", (PyCFunction)(void (*)(void))mod_block_attention, METH_FASTCALL, "ucmx_block_attention"},
+typedef int32_t (*quant_write_fn)(const void*, const void*, int64_t, int64_t, int64_t, const int64_t*, void*, const ucmx_quant_geometry*,
+                                  ucmx_stream_t);
+
+/* quant_write_tokens(entry, k, v, k_stride, v_stride, n, slots, cache, six numbers of its geometry, stream) -> status */
+static PyObject* mod_quant_write_tokens(PyObject* self, PyObject* const* args, Py_ssize_t nargs)
+{
+    enum { kN = 15 };
+    int64_t v[kN];
+    (void)self;
+    if (nargs != kN) {
+        PyErr_SetString(PyExc_TypeError, "quant_write_tokens: wrong number of arguments");
+        return NULL;
+    }
+    if (read_numbers(args, kN, -1, v) < 0) return NULL;
+    const ucmx_quant_geometry g = {v[8], v[9], (int32_t)v[10], (int32_t)v[11], (int32_t)v[12], (int32_t)v[13]};
+    int32_t st;
+    Py_BEGIN_ALLOW_THREADS;
+    st = ((quant_write_fn)(uintptr_t)v[0])((const void*)(uintptr_t)v[1], (const void*)(uintptr_t)v[2], v[3], v[4], v[5],
+                                           (const int64_t*)(uintptr_t)v[6], (void*)(uintptr_t)v[7], &g, (ucmx_stream_t)(uintptr_t)v[14]);
+    Py_END_ALLOW_THREADS;
+    return PyLong_FromLong(st);
+}
+
+static PyMethodDef mod_methods[] = {{"quant_write_tokens", (PyCFunction)(void (*)(void))mod_quant_write_tokens, METH_FASTCALL,
+                                     "ucmx_quant_write_tokens"},
+                                    {"block_attention", (PyCFunction)(void (*)(void))mod_block_attention, METH_FASTCALL, "ucmx_block_attention"},
                                     {"quant_block_attention", (PyCFunction)(void (*)(void))mod_quant_block_attention, METH_FASTCALL,
                                      "ucmx_quant_block_attention"},
                                     {"bind", mod_bind, METH_VARARGS, "bind(submit, wait, get_result, result_shape addresses, on_error)"},

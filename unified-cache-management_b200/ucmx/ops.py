@@ -547,6 +547,10 @@ class QuantKvCache:
         return int(N.lib.ucmx_quant_block_bytes(C.byref(self.geometry)))
 
 
+_BLOCK_ATTENTION, _QUANT_BLOCK_ATTENTION, _QUANT_WRITE_TOKENS = (
+    C.cast(f, C.c_void_p).value for f in (N.lib.ucmx_block_attention, N.lib.ucmx_quant_block_attention, N.lib.ucmx_quant_write_tokens))
+
+
 class _on_device:
     """Makes the device of `t` current for a launch where it is not (nothing at all in the usual case)."""
     __slots__ = ("index", "guard")
@@ -594,18 +598,21 @@ def _index(t: Optional[torch.Tensor], name: str, dev: torch.device, n: int = -1)
 def quant_write_tokens(cache: QuantKvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantise the K and V rows of new tokens into the cache: k, v bf16 [n, n_kv_heads, head_dim] (rows of a wider tensor are
     fine), slots int64 [n] = block * block_tokens + token, all different; a negative slot skips its token."""
-    _need_device(cache.data, k, v, slots)
-    g = cache.geometry
+    data = cache.data
+    _need_device(data, k, v, slots)
+    _, _, _, H, D, _ = cache.numbers
     n = slots.numel()
+    shape, strides = (n, H, D), []
     for x in (k, v):
-        if x.dtype != torch.bfloat16 or tuple(x.shape) != (n, g.n_kv_heads, g.head_dim) or x.stride()[1:] != (g.head_dim, 1):
+        step, sh, sd = x.stride() if x.dim() == 3 else (0, 0, 0)
+        if x.dtype is not torch.bfloat16 or x.shape != shape or sh != D or sd != 1:
             raise ValueError("k and v must be bf16 [n, n_kv_heads, head_dim] with contiguous heads")
-    if slots.dtype != torch.int64 or not slots.is_contiguous():
+        strides.append(step if n > 1 else H * D)
+    if slots.dtype is not torch.int64 or not slots.is_contiguous():
         raise ValueError("slots must be contiguous int64")
-    with _on_device(cache.data):
-        strides = [x.stride(0) if n > 1 else g.n_kv_heads * g.head_dim for x in (k, v)]
-        st = N.lib.ucmx_quant_write_tokens(k.data_ptr(), v.data_ptr(), strides[0], strides[1], n, slots.data_ptr(), cache.data.data_ptr(), C.byref(g),
-                                           _raw_stream(cache.data.device.index))
+    with _on_device(data):
+        st = _fast.quant_write_tokens(_QUANT_WRITE_TOKENS, k.data_ptr(), v.data_ptr(), strides[0], strides[1], n, slots.data_ptr(),
+                                      data.data_ptr(), *cache.numbers, _raw_stream(data.device.index))
     N.check("ucmx_quant_write_tokens", st, 1 if n else 0)
 
 
@@ -646,8 +653,6 @@ def quant_read_blocks(cache: QuantKvCache, block_ids: torch.Tensor, *, k_out: Op
     return k_out, v_out
 
 
-_BLOCK_ATTENTION, _QUANT_BLOCK_ATTENTION = (C.cast(f, C.c_void_p).value for f in
-                                            (N.lib.ucmx_block_attention, N.lib.ucmx_quant_block_attention))
 _workspace_bytes = {}     # (device, bits, query heads, KV heads, head_dim, query tokens) -> bytes
 
 
