@@ -14,8 +14,8 @@
 // exact in fp32: where it is half a step or more (ties, and quotients the reciprocal put on the wrong side) the code is settled by
 // it and by what the difference x - zero was rounded by.  A division per value, and fp64 for the ties, were the bound of this kernel.
 //
-// Measured on a B200 (8 heads of 128 values): 300 blocks of 128 tokens to 8 bits in 79 us (3.0 TB/s of both sides' bytes; floor
-// 36 us), back in 42 us (5.7 TB/s); 8144 tokens to 4 bits in 21 us, back in 11 us.  Writing is bound by instructions (90 per row
+// Measured on a B200 (8 heads of 128 values): 300 blocks of 128 tokens to 8 bits in 67 us (3.6 TB/s of both sides' bytes; floor
+// 36 us), back in 41 us (5.8 TB/s); 8144 tokens to 4 bits in 19 us, back in 11 us.  Writing is bound by instructions (74 per row
 // and lane, 60 % of the issue slots), reading by HBM.
 #include "common.cuh"
 
@@ -52,7 +52,8 @@ struct QuantParams {
     int32_t T, H;
     int64_t n;                         // tokens or blocks
     uint32_t items;                    // pieces of work, one per warp
-    uint32_t head_chunks;              // pieces that the heads are cut into
+    uint32_t head_chunks;              // pieces that the heads are cut into,
+    int32_t heads_per;                 // of this many heads
     int32_t* err;
 };
 
@@ -141,18 +142,17 @@ struct Piece {
     uint32_t tg;
     int32_t kv, h;
 };
-template <int HC>
-__device__ __forceinline__ Piece piece_of(uint32_t item, uint32_t head_chunks)
+__device__ __forceinline__ Piece piece_of(uint32_t item, const QuantParams& p)
 {
     Piece x;
-    const uint32_t a = item / head_chunks;
-    x.h = (int32_t)(item - a * head_chunks) * HC;
+    const uint32_t a = item / p.head_chunks;
+    x.h = (int32_t)(item - a * p.head_chunks) * p.heads_per;
     x.kv = (int32_t)(a & 1);
     x.tg = a >> 1;
     return x;
 }
 
-// HC heads of one token group per warp, their loads all in flight at once.
+// heads_per heads of one token group per warp, HC at a time with their loads in flight at once.
 template <int BITS, int D, bool BLOCKS, int HC>
 __global__ void __launch_bounds__(256, 4) quant_write_kernel(const QuantParams p)
 {
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(256, 4) quant_write_kernel(const QuantParams p
     const int lane = threadIdx.x & 31, lr = lane % X::kLanes, row = lane / X::kLanes;
     const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (item >= p.items) return;
-    const Piece x = piece_of<HC>(item, p.head_chunks);
+    const Piece x = piece_of(item, p);
     // ---- where the rows come from and where they go
     const uint16_t* src = x.kv ? p.v : p.k;
     int64_t block = -1;
@@ -189,12 +189,7 @@ __global__ void __launch_bounds__(256, 4) quant_write_kernel(const QuantParams p
     }
     const bool live = block >= 0;
     src += (int64_t)x.h * D + lr * 8;
-    uint4 raw[HC][X::kPieces];
-#pragma unroll
-    for (int c = 0; c < HC; ++c)
-#pragma unroll
-        for (int i = 0; i < X::kPieces; ++i)
-            raw[c][i] = live && x.h + c < p.H ? ld_stream16(src + c * D + i * X::kLanes * 8) : make_uint4(0, 0, 0, 0);
+    const int head_end = min(p.H, x.h + p.heads_per);
     // is the neighbouring row the other token of a pair?
     const int64_t place = live ? block * p.T + t : -2 - row;
     const int64_t other = __shfl_xor_sync(0xffffffffu, place, X::kLanes);
@@ -202,116 +197,125 @@ __global__ void __launch_bounds__(256, 4) quant_write_kernel(const QuantParams p
     const int tt = t % kRows;
     const int group_step = (p.T / kRows) * X::kGroup;
     uint8_t* group = p.cache + block * p.block_stride + (int64_t)x.h * group_step + (t / kRows) * X::kGroup;
-    // ---- each row's range: (max x, max -x) in one register
-    uint32_t range[HC];
+#pragma unroll 1
+    for (int h = x.h; h < head_end; h += HC, src += HC * D) {
+        uint4 raw[HC][X::kPieces];
 #pragma unroll
-    for (int c = 0; c < HC; ++c) {
-        uint32_t hi2 = raw[c][0].x, lo2 = raw[c][0].x;
+        for (int c = 0; c < HC; ++c)
 #pragma unroll
-        for (int i = 0; i < X::kPieces; ++i) {
-            hi2 = max2(max2(max2(max2(hi2, raw[c][i].x), raw[c][i].y), raw[c][i].z), raw[c][i].w);
-            lo2 = min2(min2(min2(min2(lo2, raw[c][i].x), raw[c][i].y), raw[c][i].z), raw[c][i].w);
+            for (int i = 0; i < X::kPieces; ++i)
+                raw[c][i] = live && h + c < head_end ? ld_stream16(src + c * D + i * X::kLanes * 8) : make_uint4(0, 0, 0, 0);
+        // ---- each row's range: (max x, max -x) in one register
+        uint32_t range[HC];
+#pragma unroll
+        for (int c = 0; c < HC; ++c) {
+            uint32_t hi2 = raw[c][0].x, lo2 = raw[c][0].x;
+#pragma unroll
+            for (int i = 0; i < X::kPieces; ++i) {
+                hi2 = max2(max2(max2(max2(hi2, raw[c][i].x), raw[c][i].y), raw[c][i].z), raw[c][i].w);
+                lo2 = min2(min2(min2(min2(lo2, raw[c][i].x), raw[c][i].y), raw[c][i].z), raw[c][i].w);
+            }
+            lo2 ^= 0x80008000u;
+            range[c] = max2(__byte_perm(hi2, lo2, 0x5410), __byte_perm(hi2, lo2, 0x7632));
+#pragma unroll
+            for (int o = 1; o < X::kLanes; o <<= 1) range[c] = max2(range[c], __shfl_xor_sync(0xffffffffu, range[c], o));
         }
-        lo2 ^= 0x80008000u;
-        range[c] = max2(__byte_perm(hi2, lo2, 0x5410), __byte_perm(hi2, lo2, 0x7632));
+        // ---- scale and zero: lane lr works them out for head lr % HC, the others fetch them
+        uint32_t my_sz;
+        float my_inv;
+        {
+            uint32_t r = range[0];
 #pragma unroll
-        for (int o = 1; o < X::kLanes; o <<= 1) range[c] = max2(range[c], __shfl_xor_sync(0xffffffffu, range[c], o));
-    }
-    // ---- scale and zero: lane lr works them out for head lr % HC, the others fetch them
-    uint32_t my_sz;
-    float my_inv;
-    {
-        uint32_t r = range[0];
+            for (int c = 1; c < HC; ++c)
+                if (lr % HC == c) r = range[c];
+            const float hi = bf16lo(r), lo = -bf16hi(r);
+            const bool bad = !((hi - hi) + (lo - lo) == 0.f);
+            my_sz = f32_to_bf16_bits(fmaf(0.5f, hi, -0.5f * lo) / (0.5f * (float)X::kTop)) | (__float_as_uint(lo) & 0xffff0000u);
+            if (bad) my_sz = 0x7fc07fc0u;
+            my_inv = __fdividef(1.f, 0.5f * bf16lo(my_sz));
+        }
 #pragma unroll
-        for (int c = 1; c < HC; ++c)
-            if (lr % HC == c) r = range[c];
-        const float hi = bf16lo(r), lo = -bf16hi(r);
-        const bool bad = !((hi - hi) + (lo - lo) == 0.f);
-        my_sz = f32_to_bf16_bits(fmaf(0.5f, hi, -0.5f * lo) / (0.5f * (float)X::kTop)) | (__float_as_uint(lo) & 0xffff0000u);
-        if (bad) my_sz = 0x7fc07fc0u;
-        my_inv = __fdividef(1.f, 0.5f * bf16lo(my_sz));
-    }
+        for (int c = 0; c < HC; ++c, group += group_step) {
+            if (h + c >= head_end) break;
+            const uint32_t sz = HC == 1 ? my_sz : __shfl_sync(0xffffffffu, my_sz, row * X::kLanes + c);
+            const float inv = HC == 1 ? my_inv : __shfl_sync(0xffffffffu, my_inv, row * X::kLanes + c);
+            const float scale = bf16lo(sz), half_scale = 0.5f * scale, lo = bf16hi(sz), half_lo = 0.5f * lo;
+            const float half = 0.5f * half_scale, most = (float)X::kTop * half_scale;
+            uint8_t* const part = group + kRows * X::kRowBytes;
 #pragma unroll
-    for (int c = 0; c < HC; ++c, group += group_step) {
-        if (x.h + c >= p.H) break;
-        const uint32_t sz = HC == 1 ? my_sz : __shfl_sync(0xffffffffu, my_sz, row * X::kLanes + c);
-        const float inv = HC == 1 ? my_inv : __shfl_sync(0xffffffffu, my_inv, row * X::kLanes + c);
-        const float scale = bf16lo(sz), half_scale = 0.5f * scale, lo = bf16hi(sz), half_lo = 0.5f * lo;
-        const float half = 0.5f * half_scale, most = (float)X::kTop * half_scale;
-        uint8_t* const part = group + kRows * X::kRowBytes;
+            for (int pc = 0; pc < X::kPieces; ++pc) {
+                const uint32_t q[4] = {raw[c][pc].x, raw[c][pc].y, raw[c][pc].z, raw[c][pc].w};
+                auto value = [&](int i) { return i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]); };
+                // ---- codes, as floats
+                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (scale >= 1e-30f) {
+                    float worst = 0.f, e[8];
 #pragma unroll
-        for (int pc = 0; pc < X::kPieces; ++pc) {
-            const uint32_t q[4] = {raw[c][pc].x, raw[c][pc].y, raw[c][pc].z, raw[c][pc].w};
-            auto value = [&](int i) { return i & 1 ? bf16hi(q[i / 2]) : bf16lo(q[i / 2]); };
-            // ---- codes, as floats
-            float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (scale >= 1e-30f) {
-                float worst = 0.f, e[8];
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    F2 hx = fma2({value(i), value(i + 1)}, {0.5f, 0.5f}, {-half_lo, -half_lo});
-                    if (BITS == 8) {                     // 255 steps of a scale that was rounded down may end beyond 255.5; 15 cannot
-                        hx.x = fminf(hx.x, most);
-                        hx.y = fminf(hx.y, most);
+                    for (int i = 0; i < 8; i += 2) {
+                        F2 hx = fma2({value(i), value(i + 1)}, {0.5f, 0.5f}, {-half_lo, -half_lo});
+                        if (BITS == 8) {                     // 255 steps of a scale that was rounded down may end beyond 255.5; 15 cannot
+                            hx.x = fminf(hx.x, most);
+                            hx.y = fminf(hx.y, most);
+                        }
+                        const F2 d = add2(fma2(hx, {inv, inv}, {kMagic, kMagic}), {-kMagic, -kMagic});
+                        const F2 r = fma2(d, {-half_scale, -half_scale}, hx);
+                        f[i] = d.x;
+                        f[i + 1] = d.y;
+                        e[i] = fabsf(r.x);
+                        e[i + 1] = fabsf(r.y);
+                        worst = fmaxf(worst, fmaxf(e[i], e[i + 1]));
                     }
-                    const F2 d = add2(fma2(hx, {inv, inv}, {kMagic, kMagic}), {-kMagic, -kMagic});
-                    const F2 r = fma2(d, {-half_scale, -half_scale}, hx);
-                    f[i] = d.x;
-                    f[i + 1] = d.y;
-                    e[i] = fabsf(r.x);
-                    e[i + 1] = fabsf(r.y);
-                    worst = fmaxf(worst, fmaxf(e[i], e[i + 1]));
-                }
-                if (worst >= half) {
+                    if (worst >= half) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (e[i] >= half) f[i] = settle(f[i], value(i), lo, half_scale);
+                    }
+                } else if (scale > 0.f) {                    // the reciprocal would leave the range: in fp64.  (Neither: a scale of 0, or NaN)
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (e[i] >= half) f[i] = settle(f[i], value(i), lo, half_scale);
+                        f[i] = (float)fmin(rint(((double)value(i) - (double)lo) / (double)scale), (double)X::kTop);
                 }
-            } else if (scale > 0.f) {                    // the reciprocal would leave the range: in fp64.  (Neither: a scale of 0, or NaN)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    f[i] = (float)fmin(rint(((double)value(i) - (double)lo) / (double)scale), (double)X::kTop);
-            }
-            // ---- 16 bits at a time: the codes side by side in one float of 2^23
-            uint32_t w[X::kWords];
-            constexpr int kIn16 = 16 / BITS;
-#pragma unroll
-            for (int i = 0; i < X::kWords; ++i) {
-                uint32_t half[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int at = (2 * i + j) * kIn16;
-                    float a = kMagic + f[at];
-#pragma unroll
-                    for (int k = 1; k < kIn16; ++k) a = fmaf(f[at + k], (float)(1 << (BITS * k)), a);
-                    half[j] = __float_as_uint(a);
-                }
-                w[i] = __byte_perm(half[0], half[1], 0x5410);
-            }
-            const int piece = pc * X::kLanes + lr;
-            if (x.kv == 0) {
-                if (live) {
-                    uint8_t* const d = group + k_at<BITS, D>(tt, piece);
-                    if (X::kWords == 1) *reinterpret_cast<uint32_t*>(d) = w[0];
-                    else *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[X::kWords - 1]);
-                }
-            } else {
+                // ---- 16 bits at a time: the codes side by side in one float of 2^23
+                uint32_t w[X::kWords];
+                constexpr int kIn16 = 16 / BITS;
 #pragma unroll
                 for (int i = 0; i < X::kWords; ++i) {
-                    const uint32_t y = __shfl_xor_sync(0xffffffffu, w[i], X::kLanes);
-                    const int u = (piece * X::kWords + i) * 2;
-                    if (paired) {
-                        *reinterpret_cast<uint32_t*>(part + v_at<BITS, D>(tt & ~1, u + (row & 1))) =
-                            __byte_perm(w[i], y, (row & 1) ? 0x3276 : 0x5410);
-                    } else if (live) {
-                        *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u)) = (uint16_t)w[i];
-                        *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u + 1)) = (uint16_t)(w[i] >> 16);
+                    uint32_t half[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int at = (2 * i + j) * kIn16;
+                        float a = kMagic + f[at];
+#pragma unroll
+                        for (int k = 1; k < kIn16; ++k) a = fmaf(f[at + k], (float)(1 << (BITS * k)), a);
+                        half[j] = __float_as_uint(a);
+                    }
+                    w[i] = __byte_perm(half[0], half[1], 0x5410);
+                }
+                const int piece = pc * X::kLanes + lr;
+                if (x.kv == 0) {
+                    if (live) {
+                        uint8_t* const d = group + k_at<BITS, D>(tt, piece);
+                        if (X::kWords == 1) *reinterpret_cast<uint32_t*>(d) = w[0];
+                        else *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[X::kWords - 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < X::kWords; ++i) {
+                        const uint32_t y = __shfl_xor_sync(0xffffffffu, w[i], X::kLanes);
+                        const int u = (piece * X::kWords + i) * 2;
+                        if (paired) {
+                            *reinterpret_cast<uint32_t*>(part + v_at<BITS, D>(tt & ~1, u + (row & 1))) =
+                                __byte_perm(w[i], y, (row & 1) ? 0x3276 : 0x5410);
+                        } else if (live) {
+                            *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u)) = (uint16_t)w[i];
+                            *reinterpret_cast<uint16_t*>(part + v_at<BITS, D>(tt, u + 1)) = (uint16_t)(w[i] >> 16);
+                        }
                     }
                 }
             }
+            if (live && lr == 0)
+                *reinterpret_cast<uint32_t*>(group + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4) = sz;
         }
-        if (live && lr == 0)
-            *reinterpret_cast<uint32_t*>(group + 2 * kRows * X::kRowBytes + x.kv * (kRows * 4) + tt * 4) = sz;
     }
 }
 
@@ -322,7 +326,7 @@ __global__ void __launch_bounds__(256) quant_read_kernel(const QuantParams p)
     const int lane = threadIdx.x & 31, lr = lane % X::kLanes, row = lane / X::kLanes;
     const uint32_t item = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (item >= p.items) return;
-    const Piece x = piece_of<HC>(item, p.head_chunks);
+    const Piece x = piece_of(item, p);
     const uint32_t per_block = (uint32_t)p.T / X::kTokens;
     const uint32_t i = x.tg / per_block;
     const int t = (int)(x.tg - i * per_block) * X::kTokens + row;
@@ -392,9 +396,10 @@ __global__ void __launch_bounds__(256) quant_read_kernel(const QuantParams p)
 enum Form { kTokensForm, kBlocksForm, kReadForm };
 
 template <int BITS, int D, int HC>
-int32_t launch_heads(QuantParams& p, Form form, int64_t groups, cudaStream_t st)
+int32_t launch_heads(QuantParams& p, Form form, int64_t groups, int chunks, cudaStream_t st)
 {
-    p.head_chunks = (uint32_t)((p.H + HC - 1) / HC);
+    p.heads_per = ((p.H + chunks - 1) / chunks + HC - 1) / HC * HC;
+    p.head_chunks = (uint32_t)((p.H + p.heads_per - 1) / p.heads_per);
     const int64_t items = groups * 2 * p.head_chunks;
     if (items > INT32_MAX) return UCMX_EUNSUPPORTED;     // (more rows than any memory holds)
     p.items = (uint32_t)items;
@@ -415,10 +420,14 @@ int32_t launch(QuantParams& p, Form form, cudaStream_t st)
     using X = Q<BITS, D>;
     const int64_t groups = form == kTokensForm ? (p.n + X::kTokens - 1) / X::kTokens : p.n * (p.T / X::kTokens);
     // Two heads of a warp in flight as soon as that still gives every SM its 32 warps; with the few tokens of a decode step one head
-    // each, over twice as many warps.
-    constexpr int kMany = 2;
-    if (groups * 2 * ((p.H + kMany - 1) / kMany) >= (int64_t)sm_count() * 32) return launch_heads<BITS, D, kMany>(p, form, groups, st);
-    return launch_heads<BITS, D, 1>(p, form, groups, st);
+    // each, over twice as many warps.  Writing, a warp goes on through its tokens' heads (finding its place costs as much as two thirds
+    // of a head) as long as that leaves two rounds of warps; reading, which HBM bounds, it does not.
+    const int64_t full = (int64_t)sm_count() * 32;
+    const int pairs = (p.H + 1) / 2;
+    if (groups * 2 * pairs < full) return launch_heads<BITS, D, 1>(p, form, groups, p.H, st);
+    int64_t chunks = form == kReadForm ? pairs : (2 * full + groups * 2 - 1) / (groups * 2);
+    if (chunks > pairs) chunks = pairs;
+    return launch_heads<BITS, D, 2>(p, form, groups, (int)chunks, st);
 }
 
 int32_t dispatch(QuantParams& p, const ucmx_quant_geometry* g, Form form, cudaStream_t st)
