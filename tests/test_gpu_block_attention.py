@@ -461,3 +461,14 @@ def test_a_table_that_ends_early_is_reported():
     torch.cuda.synchronize()
     assert _native.device_error() == 3
     R.check(got, w[0], w[2])
+
+
+@pytest.mark.parametrize("fmt", [16, 4])
+def test_several_tiles_of_columns(fmt):
+    """More requests than are counted one by one; tiles of 32; tiles that are cut over many thread blocks."""
+    rng = np.random.default_rng(60)
+    n = 1100
+    Setup(61, fmt, 1, 8, 64, 16, [int(x) for x in rng.integers(0, 3, n)], [int(x) for x in rng.integers(1, 7, n)]).tails().check()
+    Setup(62, fmt, 2, 8, 128, 16, [300, 5, 120], [4, 8, 1]).tails().check()
+    Setup(63, fmt, 1, 8, 256, 16, [400, 3], [5, 2]).tails().check()
+    Setup(64, fmt, 2, 16, 64, 16, [250, 9], [3, 4]).spread().tails().check()

@@ -188,3 +188,30 @@ def test_write_then_attend_then_move():
     R.check(a, out, tol)
     out, _, tol, _ = R.attend(q, kd, vd, [(range(1), blocks, ctx)], codes_err=err)
     R.check(b, out, tol)
+
+
+@pytest.mark.parametrize("bits,D", FORMS)
+@pytest.mark.parametrize("H", [1, 7])
+def test_many_rows_at_once(bits, D, H):
+    """Enough rows that a warp goes through several heads, of an odd number; blocks and tokens, and the way back."""
+    from ucmx import _native, ops
+    n, T = (160, 64) if H == 7 else (640, 64)
+    k, v = rows(41, n, T, H, D), rows(42, n, T, H, D, scale=3.0)
+    kd, vd = k.to(DEV), v.to(DEV)
+    c = ops.QuantKvCache.alloc(n, T, H, D, bits, DEV)
+    order = np.random.default_rng(5).permutation(n)
+    ops.quant_write_blocks(c, kd, vd, dev(order), out_slots=dev(order))
+    want = R.pack(k, v, bits)
+    assert torch.equal(c.data.cpu(), want)
+    t = ops.QuantKvCache.alloc(n, T, H, D, bits, DEV)
+    slots = torch.arange(n * T, device=DEV)
+    slots[5::1000] = -1
+    ops.quant_write_tokens(t, kd.view(-1, H, D), vd.view(-1, H, D), slots)
+    ops.quant_write_tokens(t, kd.view(-1, H, D)[5::1000], vd.view(-1, H, D)[5::1000], torch.arange(n * T, device=DEV)[5::1000].contiguous())
+    assert torch.equal(t.data.cpu(), want)
+    kb, vb = ops.quant_read_blocks(c, dev(order))
+    torch.cuda.synchronize()
+    assert _native.device_error() == 0
+    for got, x in ((kb, k), (vb, v)):
+        codes, scale, zero = R.to_codes(x[order], bits)
+        assert torch.equal(got.cpu(), (codes.double() * scale + zero).float().to(torch.bfloat16))
