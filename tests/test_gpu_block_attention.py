@@ -472,3 +472,19 @@ def test_several_tiles_of_columns(fmt):
     Setup(62, fmt, 2, 8, 128, 16, [300, 5, 120], [4, 8, 1]).tails().check()
     Setup(63, fmt, 1, 8, 256, 16, [400, 3], [5, 2]).tails().check()
     Setup(64, fmt, 2, 16, 64, 16, [250, 9], [3, 4]).spread().tails().check()
+
+
+@pytest.mark.parametrize("fmt", [8, 4])
+@pytest.mark.parametrize("T,H", [(16, 1), (16, 2), (32, 1)])
+def test_blocks_that_follow_one_another_in_memory(fmt, T, H):
+    """Neighbouring blocks in every place of a list: two slices are copied at once only where they are the ones wanted."""
+    for seed in range(6):
+        s = Setup(70 + seed, fmt, H, 4, 64, T, [40, 17], pool=200)
+        rng = np.random.default_rng(seed)
+        ids = rng.permutation(200)[:57]
+        for i in rng.permutation(50)[:30]:
+            ids[i + rng.integers(1, 8)] = (ids[i] + 1) % 200               # follows the block a few places before it
+        if seed == 0:
+            ids = np.arange(57)
+        s.ids = ids.astype(np.int32)
+        s.check()

@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     int32_t p_end = 0;                 // first position that no column of the tile sees
     int32_t p_all = 0;                 // first position that some column of the tile does not see
     // this lane's slice: where it lies (bf16: block and first token, codes: byte address), its first position, and
-    // bits 0..4 tokens to load, bit 5 every column sees all 16, bit 6 the next lane's slice follows it in memory
+    // bits 0..4 tokens to load, bit 5 every column sees all 16, bit 6 (first of a step) the step's other slice follows in memory
     int32_t my_id = 0, my_sub = 0, my_pos = 0;
     const uint8_t* my_src = nullptr;
     uint32_t my_flags = 0;
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             if (kU == 2) {
                 const unsigned long long next = __shfl_down_sync(0xffffffffu, (unsigned long long)my_src, 1);
                 const uint32_t other = __shfl_down_sync(0xffffffffu, my_flags, 1);
-                if ((my_flags & 31u) && (other & 31u) && next == (unsigned long long)my_src + L::kGroup) my_flags |= 64u;
+                if (lane % kU == 0 && (my_flags & 31u) && (other & 31u) && next == (unsigned long long)my_src + L::kGroup) my_flags |= 64u;
             }
         }
         const int from = p_look + lane % kU;
