@@ -47,7 +47,7 @@ def test_attention_refusals(why):
     from ucmx import _native as N
     if why == "geom":
         for kw in (dict(block_tokens=0), dict(n_kv_heads=0), dict(reserved=0), dict(token_stride=128), dict(token_stride=260),
-                   dict(block_stride=4), dict(block_stride=-4096)):
+                   dict(block_stride=4), dict(block_stride=-4096), dict(block_stride=0)):
             assert attend(kg=geom(**kw)) == N.EPARAM, kw
         assert attend(vg=geom(block_tokens=32)) == N.EPARAM
         for d in (32, 96, 120, 192, 512):

@@ -151,6 +151,8 @@ extern "C" int32_t ucmx_block_attention(const void* q, int64_t q_stride, int32_t
     if (kg->token_stride < E || vg->token_stride < E || kg->token_stride % 8 || vg->token_stride % 8 || kg->block_stride % 8 || vg->block_stride % 8 ||
         kg->block_stride < 0 || vg->block_stride < 0)
         return refuse("block_attention: strides must be multiples of 8 elements and hold a token's heads");
+    if ((kg->block_stride == 0 && kg->reserved > 1) || (vg->block_stride == 0 && vg->reserved > 1))
+        return refuse("block_attention: all blocks of the cache lie in one place");
     if (lists->n_req > 0 && lists->total > 0 && n_q_tokens > 0 && (!k_cache || !v_cache)) return refuse("block_attention: no cache");
     Params p = {};
     p.k = (const uint8_t*)k_cache;
