@@ -106,7 +106,6 @@ int32_t attend_common(Params& p, int bits, int32_t head_dim, const void* q, int6
     const int32_t rc = run_any(bits, p, head_dim, cols, nullptr, &plan, nullptr);
     if (rc != UCMX_OK) return refuse("attention: head_dim must be 64, 128 or 256", rc);
     if (workspace_bytes < plan_bytes(plan)) return refuse("attention: workspace too small");
-    p.cols_per_tile = plan.cols;
     p.col_tiles = (cols + plan.cols - 1) / plan.cols;
     // the slices of all requests, heads and tiles, and a lead for each of them, are numbered in 32 bits
     const int64_t units = (int64_t)p.total * p.spe + (int64_t)p.n_req * kLead;

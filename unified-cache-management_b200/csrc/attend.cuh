@@ -77,7 +77,7 @@ struct Params {
     int32_t table_size;
     const int32_t* ctx;                // [n_req] or NULL
     int32_t n_req, total;
-    int32_t col_tiles, cols_per_tile;
+    int32_t col_tiles;
     float scale_log2;
     uint16_t* out;                     // [n_q_tokens, Hq, D]
     float* lse;                        // [n_q_tokens, Hq] or NULL
@@ -403,7 +403,7 @@ struct Traits {
     static constexpr int kPart = kCols * (D + 2);        // floats of a partial result: m, l, then the rows
     // thread blocks per SM: what shared memory holds (228 KB, 1 KB of it per block), and the registers of the accumulators
     static constexpr int kBySmem = 233472 / (kSmem + 1024);
-    static constexpr int kByRegs = D * NT <= 128 ? 4 : 2;
+    static constexpr int kByRegs = D * NT > 128 ? 2 : NT == 1 ? 4 : 3;
     static constexpr int kOcc = kBySmem < 1 ? 1 : kBySmem < kByRegs ? kBySmem : kByRegs;
 };
 
