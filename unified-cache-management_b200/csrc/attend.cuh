@@ -397,7 +397,7 @@ struct Traits {
     static constexpr bool kTiled = NT >= 2;              // requests may need several tiles
     static constexpr int kScanBytes = kTiled ? (kMaxScan + 1) * 4 : 0;
     static constexpr int kQBytes = kQReg ? 0 : kKSteps * NT * 32 * 8;
-    static constexpr int kBarStride = kStages * (8 + 8 * L::kUnits) + 128;    // a warp's barriers, a note (8) per slice, 32 probes
+    static constexpr int kBarStride = kStages * (8 + 8 * L::kUnits) + 128 + 48;   // a warp's barriers, a note (8) per slice, 32 probes, a Seg
     static constexpr int kBarBytes = kWarps * kBarStride;
     static constexpr int kSmem = 1024 + kRingBytes + kMergeBytes + kStatBytes + kQBytes + kScanBytes + kBarBytes;   // (1024: alignment)
     static constexpr int kPart = kCols * (D + 2);        // floats of a partial result: m, l, then the rows
@@ -489,12 +489,20 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     w.hi = w.lo + min(w.size, all - w.lo);
     w.whole = max(kWhole, w.size / 8);
     int32_t begin = w.lo;
+    Seg* const head = reinterpret_cast<Seg*>(probes + 32);                // the first segment, for the loads and for the arithmetic
+    static_assert(sizeof(Seg) <= 48, "a Seg has 48 bytes of shared memory");
     if (begin < w.hi) {
-        const Seg s = segment_at<X::kCols>(p, w, begin);
+        Seg s = segment_at<X::kCols>(p, w, begin);
         if (s.begin < begin) {
-            if (s.end - s.begin <= w.whole) begin = s.end;                // the thread block before takes all of it
-            else if (begin <= s.begin + kLead) begin = s.begin;           // its first slice is here
+            if (s.end - s.begin <= w.whole) {                             // the thread block before takes all of it
+                begin = s.end;
+                if (begin < w.hi) s = segment_at<X::kCols>(p, w, begin);
+            } else if (begin <= s.begin + kLead) {                        // its first slice is here
+                begin = s.lo = s.begin;
+            }
         }
+        if (lane == 0) *head = s;
+        __syncwarp();
     }
     Rec* const rec = reinterpret_cast<Rec*>(p.ws + (int64_t)2 * gridDim.x * X::kPart) + blockIdx.x;
     if (tid == 0) rec->parts = 0;
@@ -504,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     Seg ps;
     ps.to = -1;
     int32_t p_at = 0;                  // next slice to load of segment ps
-    int32_t p_look = 32;               // lanes p_look .. p_look + kU - 1 know the slices to load next; 32: look again
+    int32_t p_look = 33;               // lanes p_look .. p_look + kU - 1 know the slices to load next; 32: look again, 33: at another segment
     int32_t p_entries = 0;             // entries of the request that count
     int32_t p_end = 0;                 // first position that no column of the tile sees
     int32_t p_all = 0;                 // first position that some column of the tile does not see
@@ -516,14 +524,25 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     bool p_done = false;
     int32_t p_next = begin;            // where the next segment begins
     uint32_t plain = 0;                // bit s: the step in stage s needs no masks
-    // what this lane has to know of slice s of segment ps
-    auto look_up = [&](int32_t s) {
-        my_flags = 0;
-        if (s >= ps.to) return;
+    // what this lane has to know of slice s of segment ps; `fresh`: and all of them of the segment (after the list's entries have
+    // been asked for: these are trips to memory that need not wait for one another)
+    auto look_up = [&](int32_t s, bool fresh) {
         const int32_t e = s / p.spe, sub = (s - e * p.spe) * kRows;
-        const int32_t pos_block = p.positions ? __ldg(p.positions + ps.first + e) : e;
-        int32_t id = p.block_ids ? __ldg(p.block_ids + ps.first + e) : -1;
-        if (e >= p_entries || pos_block < 0) return;
+        const bool mine = s < ps.to;
+        const int32_t pos_block = mine && p.positions ? __ldg(p.positions + ps.first + e) : e;
+        int32_t id = mine && p.block_ids ? __ldg(p.block_ids + ps.first + e) : -1;
+        if (fresh) {
+            p_entries = p.counts ? min(ps.n, __ldg(p.counts + ps.r)) : ps.n;
+            if (p.ctx) {
+                int q0, nq;
+                queries_of(p, ps.r, q0, nq);
+                const int32_t ctx = __ldg(p.ctx + ps.r) - (nq - 1);
+                p_end = ctx + min(nq - 1, (ps.ct * X::kCols + X::kCols - 1) / p.G);
+                p_all = ctx + ps.ct * X::kCols / p.G;
+            }
+        }
+        my_flags = 0;
+        if (!mine || e >= p_entries || pos_block < 0) return;
         if (!p.block_ids) {
             const int32_t t0 = __ldg(p.table_offsets + ps.r), t1 = min(__ldg(p.table_offsets + ps.r + 1), p.table_size);
             if (t0 < 0 || pos_block >= t1 - t0) {
@@ -558,27 +577,19 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     auto issue = [&](int s) {
         if (p_at >= ps.to) {
             while (!p_done && p_at >= ps.to) {
-                if (p_next < w.hi) ps = segment_at<X::kCols>(p, w, p_next);
+                if (p_next < w.hi) ps = p_next == begin ? *head : segment_at<X::kCols>(p, w, p_next);
                 if (p_next >= w.hi || !begins_here(w, ps)) {
                     p_done = true;
                     break;
                 }
                 p_next = ps.hi;
                 p_at = ps.from + warp * kU;
-                p_look = 32;
-                p_entries = p.counts ? min(ps.n, __ldg(p.counts + ps.r)) : ps.n;
-                if (p.ctx) {
-                    int q0, nq;
-                    queries_of(p, ps.r, q0, nq);
-                    const int32_t ctx = __ldg(p.ctx + ps.r) - (nq - 1);
-                    p_end = ctx + min(nq - 1, (ps.ct * X::kCols + X::kCols - 1) / p.G);
-                    p_all = ctx + ps.ct * X::kCols / p.G;
-                }
+                p_look = 33;
             }
             if (p_done) return;
         }
         if (p_look >= 32) {
-            look_up(p_at + (lane / kU) * kStep + lane % kU);
+            look_up(p_at + (lane / kU) * kStep + lane % kU, p_look > 32);
             p_look = 0;
             if (kU == 2) {
                 const unsigned long long next = __shfl_down_sync(0xffffffffu, (unsigned long long)my_src, 1);
@@ -643,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     int32_t at = begin;
 #pragma unroll 1
     while (at < w.hi) {
-        const Seg sg = segment_at<X::kCols>(p, w, at);
+        const Seg sg = at == begin ? *head : segment_at<X::kCols>(p, w, at);
         if (!begins_here(w, sg)) break;
         at = sg.hi;
         int q0, nq;
