@@ -616,7 +616,9 @@ int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_geometry* geo
  * n_q_heads a multiple of the cache's heads; head_dim 64, 128 or 256; any block_tokens (bf16 cache).  An infinity in a V row that
  *   is seen makes that dimension infinite or NaN.
  * workspace: ucmx_attention_workspace_bytes(...) bytes (bits: 16 for the bf16 cache), 16-byte aligned, any contents; it depends
- *   on neither the lists nor the batch.  Launches that may overlap need workspaces of their own.  Two kernels per call. */
+ *   on neither the lists nor the batch.  Launches that may overlap need workspaces of their own.  Two kernels per call (one where no list
+ *   can be long enough to be split), placed with programmatic stream serialization: both wait for the end of the kernel ahead of
+ *   them before they read anything, and let the next one begin only then, so stream order is what it always was. */
 typedef struct ucmx_block_lists {
     const int32_t* offsets;
     const int32_t* counts;

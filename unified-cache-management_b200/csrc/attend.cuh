@@ -33,7 +33,7 @@
 //   bf16, 64 requests, 16..52 blocks of 128 tokens: 166 us, 6.2 TB/s, 0.95 of a copy's rate: HBM.  One request of 130 944 tokens:
 //   95 us, 5.6 TB/s (7 us of it the joining of 37 parts).  8 bits, the first batch: 96 us, 5.5 TB/s: HBM, and eight warps per SM.
 //   4 bits, 32 requests of 120..500 blocks of 64 tokens: 140 us, 4.2 TB/s: the integer pipe (codes to bf16: 326 instructions per
-//   slice, 147 of them on a pipe of half rate; 58 % of the issue slots).  Shortest call, 40 slices: 7 us.
+//   slice, 147 of them on a pipe of half rate; 58 % of the issue slots).  Shortest call, 40 slices: 6 us.
 #pragma once
 
 #include <cuda.h>
@@ -432,6 +432,9 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     }
     __syncwarp();
 
+    // This kernel may be placed on the SMs while the one ahead of it ends; it reads nothing before that, and lets the next one begin
+    // only then (what a kernel that may begin early relies on is that everything ahead of this one is over).
+    early_start_wait();
     early_start_allow();
 
     // ---- this thread block's share
@@ -1331,18 +1334,22 @@ int32_t run(const Params& p, const Maps* maps, Plan* plan, cudaStream_t st)
     int64_t grid = (all + kLead - 1) / kLead;
     if (grid > plan->ctas) grid = plan->ctas;
     if (grid < 1) grid = 1;
-    kern<<<(unsigned)grid, kThreads, X::kSmem, st>>>(p, *maps);
-    UCMX_LAUNCH_CHECK("attend_kernel");
-    if (grid == 1 || (int64_t)p.total * p.spe + kLead <= kWhole) return UCMX_OK;      // no item can be split
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid - 1, X::kCols <= 8 ? 1 : X::kCols / 8);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = X::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    UCMX_CUDA(cudaLaunchKernelEx(&cfg, kern, p, *maps));
+    UCMX_LAUNCH_CHECK("attend_kernel");
+    if (grid == 1 || (int64_t)p.total * p.spe + kLead <= kWhole) return UCMX_OK;      // no item can be split
+    cfg.gridDim = dim3((unsigned)grid - 1, X::kCols <= 8 ? 1 : X::kCols / 8);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
     UCMX_CUDA(cudaLaunchKernelEx(&cfg, attend_join_kernel<D, X::kCols>, p, (int)grid));
     UCMX_LAUNCH_CHECK("attend_join_kernel");
     return UCMX_OK;
