@@ -12,7 +12,7 @@
 // codes, which have to pass through registers anyway.)
 //
 // Split.  The unit is a slice: up to 16 consecutive tokens of one listed block.  All slices of all (request, KV head,
-// column tile) items are laid end to end, each item behind a lead of kLead units (what beginning and ending an item costs;
+// column tile) items are laid end to end, each item behind a lead of 16 or 24 units (what beginning and ending an item costs;
 // without it 190 requests of 1 to 40 blocks took 38 us, with it 17), and cut into equal parts, one per thread block, whatever
 // the lengths of the requests are.  A short item stays with the thread block that it begins in; a longer one that crosses
 // cuts leaves partial results (running maximum, sum, unnormalised output) in the workspace, which a second small kernel joins
@@ -107,11 +107,18 @@ struct Seg {
     int32_t n;                         // entries of the request's list
 };
 
-constexpr int kLead = 16;              // an item's fixed cost in slices: queries in, four warps' results joined, result out
-constexpr int kWhole = 48;             // items up to this many units are not split (nor up to an eighth of a thread block's share)
+// An item's fixed cost in slices: queries in, four warps' results joined, result out.  Tiles of 16 and 32 columns have more to join
+// (24 requests of 8..40 columns: 46 us with 16, 41 with 24, 42 with 32; one column tile of 8, 4 bits, 3 requests: 13 us with 16, 14 with 24).
+constexpr int lead_of(bool tiled) { return tiled ? 24 : 16; }
+constexpr int kLeadMost = lead_of(true);
 constexpr int kMaxScan = 1023;         // requests whose column tiles are counted exactly
+// Items up to this many units, for shares of `size` units, are not split.  Where the shares are small a thread block has an item or two
+// whatever is done, and whole ones need no joining, up to 32 slices (119 requests of 6 to 18 slices: 10 us, 14 where
+// the longer of them were split; beyond 32 slices the warps' own share of an item grows: 3 requests over 4 bits 13 -> 16 us).  Where the shares are larger a whole item makes one that
+// much longer than the others (the 24 requests above: 41 us, 46 with 56 units).
+__host__ __device__ constexpr int whole_of(int size, int lead) { return size < 64 ? 32 + lead : size / 8 > 32 ? size / 8 : 32; }
 
-// How the units are shared out.  Request r begins at (base(r) - base(0)) * mult: base(r) = offsets[r] * spe + r * kLead with mult = KV heads x
+// How the units are shared out.  Request r begins at (base(r) - base(0)) * mult: base(r) = offsets[r] * spe + r * lead with mult = KV heads x
 // column tiles; or, where requests may need several tiles, base(r) = the sum of (slices + lead) x tiles of the requests before it,
 // built in shared memory, with mult = KV heads (the tiles of a request depend on its number of query tokens).
 struct Share {
@@ -125,12 +132,14 @@ struct Share {
     const int32_t* probes;             // 32 of them in shared memory
 };
 
+template <int LEAD>
 __device__ __forceinline__ int32_t base_of(const Params& p, const int32_t* scan, int32_t r)
 {
-    return scan ? scan[r] : max(0, min(__ldg(p.offsets + r), p.total)) * p.spe + r * kLead;
+    return scan ? scan[r] : max(0, min(__ldg(p.offsets + r), p.total)) * p.spe + r * LEAD;
 }
 
 // The last r with base(r) <= e, and base(r), base(r+1); 31 intervals a step, the first of them at hand.
+template <int LEAD>
 __device__ __forceinline__ int request_of(const Params& p, const Share& w, int32_t e, int32_t& first, int32_t& next)
 {
     const int lane = threadIdx.x & 31;
@@ -147,7 +156,7 @@ __device__ __forceinline__ int request_of(const Params& p, const Share& w, int32
         lo += adv;
         n = min(step, n - adv);
         step = (n + 30) / 31;
-        v = base_of(p, w.scan, lo + min(lane * step, n));
+        v = base_of<LEAD>(p, w.scan, lo + min(lane * step, n));
     }
 }
 
@@ -169,24 +178,24 @@ __device__ __forceinline__ void queries_of(const Params& p, int r, int& q0, int&
 
 // The item that holds unit `at` and the part of it that ends in this thread block; called by whole warps.  Offsets that do not
 // ascend make items that cannot be: they are passed over (n < 0) and reported.
-template <int COLS>
+template <int COLS, int LEAD>
 __device__ __forceinline__ Seg segment_at(const Params& p, const Share& w, int32_t at)
 {
     Seg s;
     int32_t a, b, tiles = w.tiles;
-    s.r = request_of(p, w, at / w.mult + w.zero, a, b);
+    s.r = request_of<LEAD>(p, w, at / w.mult + w.zero, a, b);
     if (w.scan) {
         int q0, nq;
         queries_of(p, s.r, q0, nq);
         tiles = max(1, (nq * p.G + COLS - 1) / COLS);
         s.first = max(0, min(__ldg(p.offsets + s.r), p.total));
     } else {
-        s.first = (a - s.r * kLead) / p.spe;
+        s.first = (a - s.r * LEAD) / p.spe;
     }
     const int32_t item = w.scan ? (b - a) / tiles : b - a;       // units of one (KV head, column tile)
     const int32_t start = (a - w.zero) * w.mult;
-    s.n = (item - kLead) / p.spe;
-    if (item < kLead || s.n > p.total - s.first || at < start || at - start >= item * (p.H * tiles)) {
+    s.n = (item - LEAD) / p.spe;
+    if (item < LEAD || s.n > p.total - s.first || at < start || at - start >= item * (p.H * tiles)) {
         if (p.err && threadIdx.x == 0) atomicExch(p.err, 3);
         s.begin = s.lo = at;
         s.end = s.hi = max(at + 1, w.hi);
@@ -202,14 +211,15 @@ __device__ __forceinline__ Seg segment_at(const Params& p, const Share& w, int32
     s.end = s.begin + item;
     s.lo = at;
     s.hi = item <= w.whole || s.end < w.hi ? s.end : w.hi;
-    s.from = max(0, at - s.begin - kLead);
-    s.to = s.hi - s.begin - kLead;
+    s.from = max(0, at - s.begin - LEAD);
+    s.to = s.hi - s.begin - LEAD;
     return s;
 }
 
 // Does the part that begins with the item belong to this thread block?  A split item's first part goes to the one that holds its
 // first slice.
-__device__ __forceinline__ bool begins_here(const Share& w, const Seg& s) { return s.end - s.begin <= w.whole || s.begin + kLead < w.hi; }
+template <int LEAD>
+__device__ __forceinline__ bool begins_here(const Share& w, const Seg& s) { return s.end - s.begin <= w.whole || s.begin + LEAD < w.hi; }
 
 // 2^x for a weight: x is at most kMaxSlack, and what is below 2^-126 of the largest weight is nothing
 __device__ __forceinline__ float exp2_fast(float x)
@@ -395,6 +405,7 @@ struct Traits {
     static constexpr int kMergeBytes = kWarps * kMergeCols * kMergeLd * 4;
     static constexpr int kStatBytes = kWarps * kCols * 3 * 4;
     static constexpr bool kTiled = NT >= 2;              // requests may need several tiles
+    static constexpr int kLead = lead_of(kTiled);
     static constexpr int kScanBytes = kTiled ? (kMaxScan + 1) * 4 : 0;
     static constexpr int kQBytes = kQReg ? 0 : kKSteps * NT * 32 * 8;
     static constexpr int kBarStride = kStages * (8 + 8 * L::kUnits) + 128 + 48;   // a warp's barriers, a note (8) per slice, 32 probes, a Seg
@@ -452,9 +463,9 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             if (r < p.n_req) {
                 int q0, nq;
                 queries_of(p, r, q0, nq);
-                const int32_t units = base_of(p, nullptr, r + 1) - base_of(p, nullptr, r);
-                if (units < kLead && p.err) atomicExch(p.err, 3);         // (offsets that do not ascend)
-                v[i] = max(kLead, units) * ((nq * p.G + X::kCols - 1) / X::kCols);
+                const int32_t units = base_of<X::kLead>(p, nullptr, r + 1) - base_of<X::kLead>(p, nullptr, r);
+                if (units < X::kLead && p.err) atomicExch(p.err, 3);         // (offsets that do not ascend)
+                v[i] = max(X::kLead, units) * ((nq * p.G + X::kCols - 1) / X::kCols);
             }
             sum += v[i];
         }
@@ -481,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     }
     w.step = (p.n_req + 30) / 31;
     int32_t* const probes = reinterpret_cast<int32_t*>(note + X::kStages * L::kUnits);
-    const int32_t probe = base_of(p, w.scan, min(lane * w.step, p.n_req));
+    const int32_t probe = base_of<X::kLead>(p, w.scan, min(lane * w.step, p.n_req));
     probes[lane] = probe;
     __syncwarp();
     w.probes = probes;
@@ -490,17 +501,17 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     w.size = (int32_t)(((uint32_t)all + gridDim.x - 1u) / gridDim.x);     // (the host keeps all + grid below 2^31)
     w.lo = min(all, (int32_t)blockIdx.x * w.size);
     w.hi = w.lo + min(w.size, all - w.lo);
-    w.whole = max(kWhole, w.size / 8);
+    w.whole = whole_of(w.size, X::kLead);
     int32_t begin = w.lo;
     Seg* const head = reinterpret_cast<Seg*>(probes + 32);                // the first segment, for the loads and for the arithmetic
     static_assert(sizeof(Seg) <= 48, "a Seg has 48 bytes of shared memory");
     if (begin < w.hi) {
-        Seg s = segment_at<X::kCols>(p, w, begin);
+        Seg s = segment_at<X::kCols, X::kLead>(p, w, begin);
         if (s.begin < begin) {
             if (s.end - s.begin <= w.whole) {                             // the thread block before takes all of it
                 begin = s.end;
-                if (begin < w.hi) s = segment_at<X::kCols>(p, w, begin);
-            } else if (begin <= s.begin + kLead) {                        // its first slice is here
+                if (begin < w.hi) s = segment_at<X::kCols, X::kLead>(p, w, begin);
+            } else if (begin <= s.begin + X::kLead) {                        // its first slice is here
                 begin = s.lo = s.begin;
             }
         }
@@ -580,8 +591,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     auto issue = [&](int s) {
         if (p_at >= ps.to) {
             while (!p_done && p_at >= ps.to) {
-                if (p_next < w.hi) ps = p_next == begin ? *head : segment_at<X::kCols>(p, w, p_next);
-                if (p_next >= w.hi || !begins_here(w, ps)) {
+                if (p_next < w.hi) ps = p_next == begin ? *head : segment_at<X::kCols, X::kLead>(p, w, p_next);
+                if (p_next >= w.hi || !begins_here<X::kLead>(w, ps)) {
                     p_done = true;
                     break;
                 }
@@ -657,8 +668,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     int32_t at = begin;
 #pragma unroll 1
     while (at < w.hi) {
-        const Seg sg = at == begin ? *head : segment_at<X::kCols>(p, w, at);
-        if (!begins_here(w, sg)) break;
+        const Seg sg = at == begin ? *head : segment_at<X::kCols, X::kLead>(p, w, at);
+        if (!begins_here<X::kLead>(w, sg)) break;
         at = sg.hi;
         int q0, nq;
         queries_of(p, sg.r, q0, nq);
@@ -1329,9 +1340,9 @@ int32_t run(const Params& p, const Maps* maps, Plan* plan, cudaStream_t st)
         UCMX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, X::kSmem));
         if (dev < 64) set.fetch_or(1ull << dev, std::memory_order_release);
     }
-    // (attend_common has bounded it) a thread block per kLead units: an item of a few slices has one of its own
-    const int64_t all = ((int64_t)p.total * p.spe + (int64_t)p.n_req * kLead) * p.H * p.col_tiles;
-    int64_t grid = (all + kLead - 1) / kLead;
+    // (attend_common has bounded it) a thread block per lead: an item of a few slices has one of its own
+    const int64_t all = ((int64_t)p.total * p.spe + (int64_t)p.n_req * X::kLead) * p.H * p.col_tiles;
+    int64_t grid = (all + X::kLead - 1) / X::kLead;
     if (grid > plan->ctas) grid = plan->ctas;
     if (grid < 1) grid = 1;
     cudaLaunchConfig_t cfg = {};
@@ -1346,7 +1357,9 @@ int32_t run(const Params& p, const Maps* maps, Plan* plan, cudaStream_t st)
     cfg.numAttrs = 1;
     UCMX_CUDA(cudaLaunchKernelEx(&cfg, kern, p, *maps));
     UCMX_LAUNCH_CHECK("attend_kernel");
-    if (grid == 1 || (int64_t)p.total * p.spe + kLead <= kWhole) return UCMX_OK;      // no item can be split
+    // no item can be split?  (A captured batch may use less than its capacity: then the shares are smaller, never larger.)
+    const int64_t size = (all + grid - 1) / grid;
+    if (grid == 1 || (int64_t)p.total * p.spe + X::kLead <= whole_of((int)(size < 64 ? size : 64), X::kLead)) return UCMX_OK;
     cfg.gridDim = dim3((unsigned)grid - 1, X::kCols <= 8 ? 1 : X::kCols / 8);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
