@@ -30,9 +30,9 @@
 // share one instruction (columns 4..7 repeat 0..3), otherwise they are two.
 //
 // Measured on a B200 (128 values a head, 32 query heads on 8; device times of a call, both kernels; bytes of the listed K and V):
-//   bf16, 64 requests, 16..52 blocks of 128 tokens: 166 us, 6.2 TB/s, 0.95 of a copy's rate: HBM.  One request of 130 944 tokens:
-//   95 us, 5.6 TB/s (7 us of it the joining of 37 parts).  8 bits, the first batch: 96 us, 5.5 TB/s: HBM, and eight warps per SM.
-//   4 bits, 32 requests of 120..500 blocks of 64 tokens: 140 us, 4.2 TB/s: the integer pipe (codes to bf16: 326 instructions per
+//   bf16, 64 requests, 16..52 blocks of 128 tokens: 162 us, 6.3 TB/s, 0.97 of a copy's rate: HBM.  One request of 130 944 tokens:
+//   91 us, 5.9 TB/s.  8 bits, the first batch: 92 us, 5.8 TB/s: HBM, and eight warps per SM.
+//   4 bits, 32 requests of 120..500 blocks of 64 tokens: 139 us, 4.3 TB/s: the integer pipe (codes to bf16: 326 instructions per
 //   slice, 147 of them on a pipe of half rate; 58 % of the issue slots).  Shortest call, 40 slices: 6 us.
 #pragma once
 
@@ -108,7 +108,7 @@ struct Seg {
 };
 
 // An item's fixed cost in slices: queries in, four warps' results joined, result out.  Tiles of 16 and 32 columns have more to join
-// (24 requests of 8..40 columns: 46 us with 16, 41 with 24, 42 with 32; one column tile of 8, 4 bits, 3 requests: 13 us with 16, 14 with 24).
+// (24 requests of 8..40 columns: 46 us with 16, 41 with 24, 42 with 32, joining kernel of then; one column tile of 8, 4 bits, 3 requests: 13 us with 16, 14 with 24).
 constexpr int lead_of(bool tiled) { return tiled ? 24 : 16; }
 constexpr int kLeadMost = lead_of(true);
 constexpr int kMaxScan = 1023;         // requests whose column tiles are counted exactly
@@ -1226,77 +1226,158 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
 }
 
 // Joins the partial results of the item that begins in thread block blockIdx.x and ends in a later one, eight columns per
-// blockIdx.y.  Part 0 is that block's trailing result, the others are leading ones.
+// blockIdx.y.  Part 0 is that block's trailing result, the others are leading ones.  Latency is all there is to it, and as many
+// thread blocks as can be at once: a few parts are joined column by column, one warp each; many of them by all warps together, two
+// columns at a time.  (All warps over every item, eight columns in registers: 44 requests with 32 columns spent 21 us here, 6 so;
+// 6 requests of 6 650..29 600 tokens, 256 values a head, 25 parts: 12 us.)
 template <int D, int COLS>
-__global__ void __launch_bounds__(256) attend_join_kernel(const Params p, const int n_blocks)
+__global__ void __launch_bounds__(256, 4) attend_join_kernel(const Params p, const int n_blocks)
 {
     constexpr int kC = COLS < 8 ? COLS : 8;
-    constexpr int kJoinWarps = D == 256 ? 4 : 8;
+    constexpr int kJoinWarps = 8;
     constexpr int kPart = COLS * (D + 2);
-    constexpr int kV = D / 32;                        // values of a row per lane
-    __shared__ float buf[kJoinWarps][kC][D];
-    __shared__ float sums[kJoinWarps][kC];
+    constexpr int kW = D < 128 ? 2 : 4;               // values of one load
+    constexpr int kV = D / 32 / kW;                   // loads of a row per lane
+    struct __align__(4 * kW) Vec {
+        float x[kW];
+    };
+    __shared__ Vec buf[kJoinWarps][2][D / kW];
+    __shared__ float sums[2];
     early_start_wait();
     const Rec rec = reinterpret_cast<const Rec*>(p.ws + (int64_t)2 * n_blocks * kPart)[blockIdx.x];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int y0 = blockIdx.y * 8;
     if (rec.parts == 0 || y0 >= rec.cols) return;
 
-    const float* const first = p.ws + (int64_t)(2 * blockIdx.x + 1) * kPart;
-    const float* const rest = p.ws + (int64_t)2 * blockIdx.x * kPart;
+    const float* const first = p.ws + (int64_t)(2 * blockIdx.x + 1) * kPart + y0;
+    const float* const rest = p.ws + (int64_t)2 * blockIdx.x * kPart + y0;
     auto part_of = [&](int i) { return i == 0 ? first : rest + (int64_t)2 * i * kPart; };
-    float top[kC], sum[kC], acc[kC][kV];
+    auto row_of = [&](Vec (&x)[kV], int i, int c) {
+        const Vec* const s = reinterpret_cast<const Vec*>(part_of(i) + 2 * COLS + y0 * (D - 1) + c * D);
 #pragma unroll
-    for (int c = 0; c < kC; ++c) {
-        float x = -INFINITY;
-        for (int i = lane; i < rec.parts; i += 32) x = fmaxf(x, part_of(i)[y0 + c]);
+        for (int v = 0; v < kV; ++v) x[v] = s[v * 32 + lane];
+    };
+    auto add = [&](float (&acc)[kV][kW], const Vec (&x)[kV], float w) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-        top[c] = x;
-        sum[c] = 0.f;
+        for (int v = 0; v < kV; ++v)
 #pragma unroll
-        for (int v = 0; v < kV; ++v) acc[c][v] = 0.f;
+            for (int k = 0; k < kW; ++k) acc[v][k] = fmaf(w, x[v].x[k], acc[v][k]);
+    };
+    auto over_lanes = [](float x, auto op) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, o));
+        return x;
+    };
+    auto most = [](float x, float y) { return fmaxf(x, y); };
+    auto plus = [](float x, float y) { return x + y; };
+    auto put = [&](int cl, const float (&acc)[kV][kW], float top, float l) {       // one column's result, by a warp
+        const int c = rec.c0 + y0 + cl, j = c / p.G;
+        const int64_t row = (int64_t)(rec.q0 + j) * p.Hq + rec.h * p.G + (c - j * p.G);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) {
+            uint32_t y[kW / 2];
+#pragma unroll
+            for (int k = 0; k < kW / 2; ++k) y[k] = l == 0.f ? 0u : pack_bf16(acc[v][2 * k] * inv, acc[v][2 * k + 1] * inv);
+            uint32_t* const to = reinterpret_cast<uint32_t*>(p.out + row * D) + (v * 32 + lane) * (kW / 2);
+            if constexpr (kW == 4) *reinterpret_cast<uint2*>(to) = make_uint2(y[0], y[1]);
+            else *to = y[0];
+        }
+        if (lane == 0 && p.lse) p.lse[row] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+    };
+    const int cols = min(kC, rec.cols - y0);
+    if (rec.parts <= 8) {
+        if (warp >= cols) return;
+        const bool mine = lane < rec.parts;
+        const float* const s = part_of(mine ? lane : 0) + warp;
+        Vec x[2][kV];
+        row_of(x[0], 0, warp);
+        if (rec.parts > 1) row_of(x[1], 1, warp);
+        const float m = mine ? s[0] : -INFINITY, l0 = mine ? s[COLS] : 0.f;
+        const float top = over_lanes(m, most);
+        const float f = exp2_fast(m - (top == -INFINITY ? 0.f : top));
+        const float l = over_lanes(f * l0, plus);
+        float acc[kV][kW] = {};
+        add(acc, x[0], __shfl_sync(0xffffffffu, f, 0));
+        if (rec.parts > 1) add(acc, x[1], __shfl_sync(0xffffffffu, f, 1));
+#pragma unroll 2
+        for (int i = 2; i < rec.parts; ++i) {
+            row_of(x[0], i, warp);
+            add(acc, x[0], __shfl_sync(0xffffffffu, f, i));
+        }
+        put(warp, acc, top, l);
+        return;
     }
-    if (warp < kJoinWarps) {
-#pragma unroll(kC == 4 ? 4 : 2)
-        for (int i = warp; i < rec.parts; i += kJoinWarps) {
-            const float* const part = part_of(i);
+    float top[kC];
 #pragma unroll
-            for (int c = 0; c < kC; ++c) {
-                const float f = exp2_fast(part[y0 + c] - (top[c] == -INFINITY ? 0.f : top[c]));
-                sum[c] += f * part[COLS + y0 + c];
+    for (int c = 0; c < kC; ++c) top[c] = -INFINITY;
+    for (int i = lane; i < rec.parts; i += 32) {
+        const float4* const s = reinterpret_cast<const float4*>(part_of(i));
 #pragma unroll
-                for (int v = 0; v < kV; ++v) acc[c][v] += f * part[2 * COLS + (y0 + c) * D + v * 32 + lane];
+        for (int c = 0; c < kC; c += 4) {
+            const float4 x = s[c / 4];
+            top[c] = fmaxf(top[c], x.x);
+            top[c + 1] = fmaxf(top[c + 1], x.y);
+            top[c + 2] = fmaxf(top[c + 2], x.z);
+            top[c + 3] = fmaxf(top[c + 3], x.w);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < kC; ++c) top[c] = over_lanes(top[c], most);
+#pragma unroll
+    for (int c0 = 0; c0 < kC; c0 += 2) {
+        if (c0 >= cols) break;
+        if (c0) __syncthreads();
+        float acc[2][kV][kW] = {}, sum[2] = {};
+        const float off[2] = {top[c0] == -INFINITY ? 0.f : top[c0], top[c0 + 1] == -INFINITY ? 0.f : top[c0 + 1]};
+#pragma unroll 1
+        for (int from = 0; from < rec.parts; from += 32) {        // 32 parts at a time, their factors in the lanes
+            float f[2] = {0.f, 0.f};
+            if (from + lane < rec.parts) {
+                const float* const s = part_of(from + lane) + c0;
+                const float2 m = *reinterpret_cast<const float2*>(s), l = *reinterpret_cast<const float2*>(s + COLS);
+                f[0] = exp2_fast(m.x - off[0]);
+                f[1] = exp2_fast(m.y - off[1]);
+                sum[0] = fmaf(f[0], l.x, sum[0]);
+                sum[1] = fmaf(f[1], l.y, sum[1]);
+            }
+            const int end = min(32, rec.parts - from);
+#pragma unroll
+            for (int k = 0; k < 32 / kJoinWarps; ++k) {
+                const int j = warp + k * kJoinWarps;
+                if (j >= end) break;
+                Vec x[2][kV];
+                row_of(x[0], from + j, c0);
+                row_of(x[1], from + j, c0 + 1);
+                add(acc[0], x[0], __shfl_sync(0xffffffffu, f[0], j));
+                add(acc[1], x[1], __shfl_sync(0xffffffffu, f[1], j));
             }
         }
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-            if (lane == 0) sums[warp][c] = sum[c];
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int v = 0; v < kV; ++v) buf[warp][c][v * 32 + lane] = acc[c][v];
+            for (int v = 0; v < kV; ++v) {
+                Vec x;
+#pragma unroll
+                for (int k = 0; k < kW; ++k) x.x[k] = acc[e][v][k];
+                buf[warp][e][v * 32 + lane] = x;
+            }
+            if (warp == 0) {
+                sum[e] = over_lanes(sum[e], plus);
+                if (lane == 0) sums[e] = sum[e];
+            }
         }
-    }
-    __syncthreads();
-    for (int i = tid; i < kC * (D / 2); i += 256) {
-        const int cl = i / (D / 2), d = (i - cl * (D / 2)) * 2, cc = y0 + cl;
-        if (cc >= rec.cols) continue;
-        float l = 0.f, x = 0.f, y = 0.f;
+        __syncthreads();
+        if (warp < 2 && c0 + warp < cols) {
+            float all[kV][kW] = {};
 #pragma unroll
-        for (int k = 0; k < kJoinWarps; ++k) {
-            l += sums[k][cl];
-            x += buf[k][cl][d];
-            y += buf[k][cl][d + 1];
-        }
-        const int c = rec.c0 + cc, j = c / p.G;
-        const int64_t row = (int64_t)(rec.q0 + j) * p.Hq + rec.h * p.G + (c - j * p.G);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        reinterpret_cast<uint32_t*>(p.out)[row * (D / 2) + d / 2] = l == 0.f ? 0u : pack_bf16(x * inv, y * inv);
-        if (d == 0 && p.lse) {
-            float t = -INFINITY;
+            for (int k = 0; k < kJoinWarps; ++k) {
+                Vec x[kV];
 #pragma unroll
-            for (int k = 0; k < kC; ++k)
-                if (k == cl) t = top[k];
-            p.lse[row] = l == 0.f ? -INFINITY : (t + log2f(l)) * kLn2;
+                for (int v = 0; v < kV; ++v) x[v] = buf[k][warp][v * 32 + lane];
+                add(all, x, 1.f);
+            }
+            put(c0 + warp, all, top[c0 + (warp ? 1 : 0)], sums[warp]);
         }
     }
 }
