@@ -108,14 +108,14 @@ struct Seg {
 };
 
 // An item's fixed cost in slices: queries in, four warps' results joined, result out.  Tiles of 16 and 32 columns have more to join
-// (24 requests of 8..40 columns: 46 us with 16, 41 with 24, 42 with 32, joining kernel of then; one column tile of 8, 4 bits, 3 requests: 13 us with 16, 14 with 24).
+// (24 requests of 8..40 columns: 43 us with 16, 38 with 24, 39 with 32; one column tile of 8, 4 bits, 3 requests: 13 us with 16, 14 with 24).
 constexpr int lead_of(bool tiled) { return tiled ? 24 : 16; }
 constexpr int kLeadMost = lead_of(true);
 constexpr int kMaxScan = 1023;         // requests whose column tiles are counted exactly
 // Items up to this many units, for shares of `size` units, are not split.  Where the shares are small a thread block has an item or two
 // whatever is done, and whole ones need no joining, up to 32 slices (119 requests of 6 to 18 slices: 10 us, 14 where
 // the longer of them were split; beyond 32 slices the warps' own share of an item grows: 3 requests over 4 bits 13 -> 16 us).  Where the shares are larger a whole item makes one that
-// much longer than the others (the 24 requests above: 41 us, 46 with 56 units).
+// much longer than the others (the 24 requests above, with the joining kernel of then: 41 us, 46 with 56 units).
 __host__ __device__ constexpr int whole_of(int size, int lead) { return size < 64 ? 32 + lead : size / 8 > 32 ? size / 8 : 32; }
 
 // How the units are shared out.  Request r begins at (base(r) - base(0)) * mult: base(r) = offsets[r] * spe + r * lead with mult = KV heads x
@@ -399,7 +399,7 @@ struct Traits {
     static constexpr int kMTiles = D / 16;
     static constexpr bool kQReg = kKSteps * NT <= 16;    // query fragments in registers (else in shared memory)
     static constexpr int kMergeLd = D + 4;
-    static constexpr int kMergeCols = D <= 128 && NT > 1 ? 8 : 4;         // columns joined at a time
+    static constexpr int kMergeCols = NT == 1 ? 4 : D == 256 ? 4 : D == 128 && NT == 4 ? 8 : 16;   // columns joined at a time: what there is room for
     static constexpr int kMergeSteps = kCols / kMergeCols;
     static constexpr int kRingBytes = kWarps * kStages * L::kStage;
     static constexpr int kMergeBytes = kWarps * kMergeCols * kMergeLd * 4;
@@ -1161,7 +1161,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             if (step) __syncthreads();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                if (nt != step * X::kMergeCols / 8) continue;
+                if (nt * 8 / X::kMergeCols > step || (nt * 8 + 7) / X::kMergeCols < step) continue;
 #pragma unroll
                 for (int mt = 0; mt < X::kMTiles; ++mt)
 #pragma unroll
@@ -1172,8 +1172,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                         const int d = FMT == 16 ? mt * 16 + g + row * 8
                                                 : (mt / (L::kPanelDims / 16)) * L::kPanelDims + g * (L::kPanelDims / 8) +
                                                       (mt % (L::kPanelDims / 16)) * 2 + row;
-                        if (X::kMergeCols == 8 || (q4 >> 1) == (step & 1))
-                            merge[(warp * X::kMergeCols + (2 * q4 + (i & 1)) % X::kMergeCols) * X::kMergeLd + d] = x;
+                        if ((nt * 8 + 2 * q4) / X::kMergeCols == step)
+                            merge[(warp * X::kMergeCols + (nt * 8 + 2 * q4 + (i & 1)) % X::kMergeCols) * X::kMergeLd + d] = x;
                     }
             }
             __syncthreads();
