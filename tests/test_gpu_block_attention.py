@@ -488,3 +488,15 @@ def test_blocks_that_follow_one_another_in_memory(fmt, T, H):
             ids = np.arange(57)
         s.ids = ids.astype(np.int32)
         s.check()
+
+
+@pytest.mark.parametrize("fmt", [16, 4])
+@pytest.mark.parametrize("G,D", [(1, 64), (3, 128), (7, 128), (2, 256), (13, 64), (16, 128), (20, 256), (33, 64)])
+def test_parts_by_the_hundred_are_joined(fmt, G, D):
+    """One KV head and one long request: more parts than a warp has lanes, in each width of tile; contexts that leave the later parts
+    empty, or all of them; a shorter request whose few parts are joined another way."""
+    s = Setup(70, fmt, 1, G, D, 16, [1500, 90]).tails()
+    s.check()
+    for ctx in ([700 * 16 + 5, 41], [3, 0], [0, 90 * 16]):
+        s.ctx = np.asarray(ctx, np.int32)
+        s.check()
