@@ -123,3 +123,9 @@ def test_the_plain_form_packs_what_it_unpacks():
             for (codes, scale, zero), x in zip(R.held(data, D, bits), (k, v)):
                 c, s, z = R.to_codes(x, bits)
                 assert torch.equal(codes, c) and torch.equal(scale, s) and torch.equal(zero, z)
+
+
+def test_reading_back_into_blocks_that_lie_in_one_place():
+    from ucmx import _native as N
+    for kg, vg in ((geom(block_stride=0), geom()), (geom(), geom(block_stride=0))):
+        assert N.lib.ucmx_quant_read_blocks(FAKE, qgeom(), FAKE, None, 1, FAKE, kg, FAKE, vg, None) == N.EPARAM

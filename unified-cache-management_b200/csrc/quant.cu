@@ -555,6 +555,8 @@ extern "C" int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_ge
     QuantParams p = {};
     if (rc == UCMX_OK) rc = check_pair(p, k_cache, kg, v_cache, vg, g);
     if (rc != UCMX_OK) return rc;
+    if ((kg->block_stride == 0 && kg->reserved > 1) || (vg->block_stride == 0 && vg->reserved > 1))
+        return refuse("quant_read_blocks: all blocks of the output lie in one place");
     if (!block_ids) return refuse("quant_read_blocks: no block ids");
     p.ids = block_ids;
     p.out_slots = out_slots;
