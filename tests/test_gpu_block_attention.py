@@ -500,3 +500,11 @@ def test_parts_by_the_hundred_are_joined(fmt, G, D):
     for ctx in ([700 * 16 + 5, 41], [3, 0], [0, 90 * 16]):
         s.ctx = np.asarray(ctx, np.int32)
         s.check()
+
+
+@pytest.mark.parametrize("fmt", [16, 4])
+def test_a_workspace_whose_bytes_are_not_its_own_is_refused(fmt):
+    s = Setup(71, fmt, 1, 2, 64, 16, [2])
+    with pytest.raises(ValueError):
+        s.run(workspace=torch.zeros(1, dtype=torch.uint8, device=DEV).expand(1 << 26))
+    s.check()

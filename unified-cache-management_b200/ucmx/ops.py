@@ -709,6 +709,8 @@ def _attend(name: str, front, entry: int, bits: int, n_kv_heads: int, head_dim: 
         return out
     if workspace is None:
         workspace = attention_workspace(query, n_kv_heads, max_q_tokens=max_q_tokens, bits=bits)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     with _on_device(query):
         st = front(entry, query.data_ptr(), q_stride, Hq, q_off, n_tok, max_q_tokens, *cache_args, *lists,
                    D ** -0.5 if scale is None else scale, out.data_ptr(), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(),
