@@ -33,12 +33,13 @@ class DecodeRetrievalEngine:
         order: order of the selected ids (best first, or ascending block position).
         delta: keep a resident working set per layer and request and move only the blocks that are new with respect
         to the previous step's selection (what ESA does, ucm/sparse/esa/esa.py:313-338): top-k of block positions in
-        ascending order -> resident-set remap -> block-to-block move of the misses.
+        ascending order -> resident-set remap -> block-to-block move of the misses.  Without attend nothing reads the
+        blocks that were moved, and all layers move into the same slots: what such a step shows is its time.
         overlap: scoring and selection of layer l+1 run on a second stream while layer l's blocks move (they do not
         depend on each other); the step is then bounded by the block moves alone.
         attend: each layer ends with the attention of its queries over the blocks just selected, written to
         attn_out[layer].  It reads the blocks in the pool, in place of the gather; in the delta step it follows the
-        move and reads the resident working set.
+        move and reads the layer's resident working set (one per layer: n_layers x the selected blocks' bytes).
         cache_bits: 4 or 8 keeps a quantised copy of the pool beside it (quant_pool) and attends over that; blocks that
         filled up since the last step are quantised when the step begins."""
         self.shape, self.batch, self.device = shape, batch, device
@@ -78,7 +79,10 @@ class DecodeRetrievalEngine:
                     e = min(s + chunk, batch.n_slots)
                     self.kv_pool[p, s:e].copy_(torch.randn((e - s, self.T, self.H, self.D), generator=g, device=device)
                                                .to(torch.bfloat16))
-            self.staging = torch.empty((batch.total_k, 2, self.T * E * 2), dtype=torch.uint8, device=device)
+            # where selected blocks go.  An attention over the delta step's working set reads what earlier steps of the same layer
+            # left there, so each layer has one of its own then; what only times the moves shares one among the layers.
+            sets = (self.L,) if attend and delta else ()
+            self.staging = torch.empty((*sets, batch.total_k, 2, self.T * E * 2), dtype=torch.uint8, device=device)
         self.qbar = torch.empty((batch.n_req, E), dtype=torch.float32, device=device)
         self.scores = torch.empty((batch.total,), dtype=torch.float32, device=device)
         self.sel_ids = torch.full((self.L, batch.total_k), -1, **i32)
@@ -96,7 +100,7 @@ class DecodeRetrievalEngine:
         if delta:
             if not with_kv_pool:
                 raise ValueError("the delta step moves blocks: it needs the K/V pool")
-            # resident working set: request r owns slots [k_offsets[r], k_offsets[r+1]) of `staging` in every layer
+            # resident working set: request r owns slots [k_offsets[r], k_offsets[r+1]) of working_set(layer) in every layer
             n = batch.total_k
             self.slot_phys = torch.arange(n, **i32)
             self.slot_logical = torch.full((self.L, n), -1, **i32)
@@ -195,8 +199,13 @@ class DecodeRetrievalEngine:
                            sel_counts=self.sel_counts[layer], src_map=self.block_table, src_map_offsets=self.offsets,
                            moves=self.moves, out=self.remap_out[layer])
 
+    def working_set(self, layer: int) -> torch.Tensor:
+        """The slots [total_k, 2, bytes of a block] that serve the layer's selection in the delta step."""
+        return self.staging[layer] if self.attend else self.staging
+
     def move_layer(self, layer: int) -> None:
-        ops.move_blocks([self.kv_pool[0], self.kv_pool[1]], self.moves, [self.staging[:, 0], self.staging[:, 1]])
+        slots = self.working_set(layer)
+        ops.move_blocks([self.kv_pool[0], self.kv_pool[1]], self.moves, [slots[:, 0], slots[:, 1]])
 
     def attend_layer(self, layer: int) -> torch.Tensor:
         """Attention of the layer's queries over its selected blocks (every block of a selection is full, so their places
@@ -204,7 +213,7 @@ class DecodeRetrievalEngine:
         args = dict(req_counts=self.sel_counts[layer], out=self.attn_out[layer], workspace=self.attn_workspace)
         if self.delta:                             # the resident slots that serve the selection
             shape = (self.batch.total_k, self.T, self.H, self.D)
-            k, v = (self.staging[:, i].view(torch.bfloat16).view(shape) for i in (0, 1))
+            k, v = (self.working_set(layer)[:, i].view(torch.bfloat16).view(shape) for i in (0, 1))
             return ops.block_attention(self.q_dev[layer], k, v, self.k_offsets, block_ids=self.remap_out[layer][0], **args)
         if self.quant_pool is not None:
             return ops.quant_block_attention(self.q_dev[layer], self.quant_pool, self.k_offsets, block_ids=self.sel_ids[layer], **args)
