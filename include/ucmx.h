@@ -284,7 +284,9 @@ int32_t ucmx_topk_ragged_peer_sum(const ucmx_peer_exchange* exchange /* host */,
  * of the s-th HBM block the request owns (ascending; a negative id marks a slot that does not
  * exist, which lets requests with different numbers of blocks share one slot stride), slot_logical[s]
  * the logical block it holds (-1 = none), slot_free[s] != 0 marks slots the previous round left on
- * the free list.
+ * the free list (a block that was selected a round ago may still be read then).  slot_free NULL: every slot
+ * that is not a hit now may be taken, for a caller whose readers of the previous round are done; a request with
+ * as many slots as it selects blocks is then always served.
  * Selection, per request (entries [sel_offsets[r], sel_offsets[r+1]), of which only the first
  * sel_counts[r] are used when sel_counts is given; a negative count leaves the request's state and
  * outputs untouched): ascending logical block ids (negative = skip).

@@ -26,3 +26,52 @@ def test_every_layer_keeps_a_working_set_of_its_own():
     assert eng.loads_of_last_step() == 0
     a, b = (set(eng.sel_ids[l].tolist()) for l in (0, 1))
     assert a != b                                   # (the layers do select different blocks)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(overlap=True)])
+def test_newly_selected_blocks_are_all_loaded(kw):
+    """Queries that drift: some of each selection is resident, the rest is moved, and none of it is left out."""
+    eng = make(n_layers=3, **kw)
+    eng.make_queries()
+    eng.step()
+    check(eng)
+    for _ in range(4):
+        eng.drift_queries(0.7)
+        eng.step()
+        check(eng)
+        assert 0 < eng.loads_of_last_step() < eng.L * eng.batch.total_k
+        for l in range(eng.L):
+            n = eng.sel_counts[l].tolist()
+            off = eng.k_offsets.tolist()
+            served = torch.cat([eng.remap_out[l][0][off[r]:off[r] + n[r]] for r in range(eng.batch.n_req)])
+            assert bool((served >= 0).all())
+    eng.capture()
+    for _ in range(3):
+        eng.drift_queries(0.7)
+        eng.step()
+        check(eng)
+
+
+def test_remap_without_a_deferred_free_list():
+    """slot_free None: with as many slots as selected blocks every block is served in every round, hits stay, slots are distinct."""
+    import numpy as np
+    from ucmx import ops
+    rng = np.random.default_rng(7)
+    n_logical, ks = [300, 64, 9], [40, 64, 3]
+    off = np.concatenate([[0], np.cumsum(ks)]).astype(np.int32)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(DEV)  # noqa: E731
+    logical, phys = t(np.full(107, -1)), t(np.arange(107))
+    resident = {}
+    for _ in range(5):
+        sel = np.concatenate([np.sort(rng.choice(n, k, replace=False)) for n, k in zip(n_logical, ks)]).astype(np.int32)
+        table, ll, lp, lc = ops.remap_resident(logical, None, phys, t(off), t(sel), t(off), max_logical=300, max_slots=64)
+        table, lc = table.cpu().numpy(), lc.cpu().numpy()
+        new = {}
+        for r in range(3):
+            a, b = off[r], off[r + 1]
+            assert sorted(table[a:b]) == list(range(a, b))                   # every slot of the request serves one block
+            assert lc[r] == sum((r, int(x)) not in resident for x in sel[a:b])
+            for x, s in zip(sel[a:b], table[a:b]):
+                assert resident.get((r, int(x)), s) == s
+                new[r, int(x)] = s
+        resident = new

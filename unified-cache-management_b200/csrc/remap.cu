@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kRemapThreads) remap_resident_kernel(RemapPara
         n_sel = min(n_sel, c);
     }
     int32_t* slot_logical = p.slot_logical + s0;
-    uint8_t* slot_free = p.slot_free + s0;
+    uint8_t* slot_free = p.slot_free ? p.slot_free + s0 : nullptr;
     const int32_t* slot_phys = p.slot_phys + s0;
     const int32_t* sel = p.sel + j0;
     int32_t* table = p.table + j0;
@@ -116,11 +116,11 @@ __global__ void __launch_bounds__(kRemapThreads) remap_resident_kernel(RemapPara
     }
     __syncthreads();
 
-    // free list of this round: listed free by the previous round and not hit now, in slot order
+    // free list of this round: listed free by the previous round (where that is kept) and not hit now, in slot order
     int n_free = 0;
     for (int c0 = 0; c0 < n_slots; c0 += kRemapThreads) {
         const int s = c0 + tid;
-        const bool f = s < n_slots && slot_free[s] != 0 && hit[s] == 0 && __ldg(slot_phys + s) >= 0;
+        const bool f = s < n_slots && (!slot_free || slot_free[s] != 0) && hit[s] == 0 && __ldg(slot_phys + s) >= 0;
         int tot;
         const int pos = n_free + excl_scan(f, s_warp, tot);
         if (f) free_list[pos] = s;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kRemapThreads) remap_resident_kernel(RemapPara
         n_miss += tot;
     }
     __syncthreads();
-    for (int s = tid; s < n_slots; s += kRemapThreads) slot_free[s] = (hit[s] || __ldg(slot_phys + s) < 0) ? 0 : 1;
+    for (int s = tid; slot_free && s < n_slots; s += kRemapThreads) slot_free[s] = (hit[s] || __ldg(slot_phys + s) < 0) ? 0 : 1;
     // the rest of this request's room in the load lists is marked empty, so that a block mover can take the lists
     // of all requests as one array and skip what is not a load
     const int n_load = min(n_miss, n_free);
@@ -182,7 +182,7 @@ extern "C" int32_t ucmx_remap_resident(int32_t* slot_logical, uint8_t* slot_free
     using namespace ucmx;
     if (n_req < 0 || max_logical < 1 || max_slots < 0) return UCMX_EPARAM;
     if (n_req == 0) return UCMX_OK;
-    if (!slot_logical || !slot_free || !slot_phys || !slot_offsets || !sel || !sel_offsets || !table || !load_logical ||
+    if (!slot_logical || !slot_phys || !slot_offsets || !sel || !sel_offsets || !table || !load_logical ||
         !load_phys || !load_counts)
         return UCMX_EPARAM;
     ucmx_remap_moves mv{};

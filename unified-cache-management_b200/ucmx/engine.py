@@ -194,7 +194,10 @@ class DecodeRetrievalEngine:
 
     def remap_layer(self, layer: int) -> None:
         """Which resident slot serves each selected block, and the (pool block -> resident slot) list of the misses."""
-        ops.remap_resident(self.slot_logical[layer], self.slot_free[layer], self.slot_phys, self.k_offsets,
+        # a slot per selected block: where an attention reads all of them, the misses take what the last step's selection left
+        # (its attention is over: the moves follow it on this stream)
+        free = None if self.attend else self.slot_free[layer]
+        ops.remap_resident(self.slot_logical[layer], free, self.slot_phys, self.k_offsets,
                            self.sel_ids[layer], self.k_offsets, max_logical=self.max_logical, max_slots=self.out_stride,
                            sel_counts=self.sel_counts[layer], src_map=self.block_table, src_map_offsets=self.offsets,
                            moves=self.moves, out=self.remap_out[layer])

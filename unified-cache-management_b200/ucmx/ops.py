@@ -406,21 +406,22 @@ class MoveList:
         self.capacity = capacity
 
 
-def remap_resident(slot_logical: torch.Tensor, slot_free: torch.Tensor, slot_phys: torch.Tensor,
+def remap_resident(slot_logical: torch.Tensor, slot_free: Optional[torch.Tensor], slot_phys: torch.Tensor,
                    slot_offsets: torch.Tensor, sel: torch.Tensor, sel_offsets: torch.Tensor, *, max_logical: int,
                    max_slots: int, sel_counts: Optional[torch.Tensor] = None, src_map: Optional[torch.Tensor] = None,
                    src_map_offsets: Optional[torch.Tensor] = None, moves: Optional[MoveList] = None,
                    out: Optional[tuple] = None):
     """One round of the resident-set remap for every request (state tensors are updated in place).
 
-    slot_logical int32, slot_free uint8, slot_phys int32: flat per-request state (CSR by slot_offsets);
+    slot_logical int32, slot_free uint8, slot_phys int32: flat per-request state (CSR by slot_offsets); slot_free None:
+    every slot that is not a hit may be taken now (nothing reads the previous round's blocks any more);
     sel: ascending selected logical blocks (CSR by sel_offsets).  Returns (table, load_logical, load_phys,
     load_counts): table[j] = physical block serving sel[j]; the load lists are packed like sel, unused entries -1.
     With `moves` (and src_map, optionally src_map_offsets) the loads of all requests are also appended to that list
     as (src_map[src_map_offsets[r] + logical block] -> HBM block), ready for move_blocks.
     out: the result tensors of an earlier call, to be reused."""
     _need_cuda(slot_logical, slot_free, slot_phys, slot_offsets, sel, sel_offsets, sel_counts, src_map, src_map_offsets)
-    if slot_free.dtype != torch.uint8 or not slot_free.is_contiguous():
+    if slot_free is not None and (slot_free.dtype != torch.uint8 or not slot_free.is_contiguous()):
         raise ValueError("slot_free must be contiguous uint8")
     n_req = slot_offsets.numel() - 1
     dev = sel.device
