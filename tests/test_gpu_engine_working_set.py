@@ -17,13 +17,18 @@ def make(ratio=0.2, n_layers=2, **kw):
 
 
 def test_every_layer_keeps_a_working_set_of_its_own():
-    """The same queries again: every block is resident, nothing moves, and each layer reads its own blocks."""
+    """The same queries again: every block is resident, none but the newest ones may move, and each layer reads its own blocks."""
     eng = make()
     eng.make_queries()
     for _ in range(3):
         eng.step()
         check(eng)
-    assert eng.loads_of_last_step() == 0
+    newest = set(eng.new_block_ids.tolist())
+    table, boff, off = eng.block_table.tolist(), eng.offsets.tolist(), eng.k_offsets.tolist()
+    for l in range(eng.L):
+        for r in range(eng.batch.n_req):
+            moved = eng.remap_out[l][1][off[r]:off[r + 1]].tolist()
+            assert all(table[boff[r] + x] in newest for x in moved if x >= 0)
     a, b = (set(eng.sel_ids[l].tolist()) for l in (0, 1))
     assert a != b                                   # (the layers do select different blocks)
 
@@ -50,6 +55,28 @@ def test_newly_selected_blocks_are_all_loaded(kw):
         eng.drift_queries(0.7)
         eng.step()
         check(eng)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(overlap=True)])
+def test_a_block_that_filled_up_is_moved_again(kw):
+    """Every block is selected and resident; the newest one of each request changes in the pool between the steps."""
+    eng = make(ratio=1.0, **kw)
+    eng.make_queries()
+    eng.step()
+    check(eng)
+    new = eng.new_block_ids.long()
+
+    def refill():
+        eng.kv_pool[:, new] = torch.randn(eng.kv_pool[:, new].shape, device=DEV, generator=eng.gen).to(torch.bfloat16)
+
+    refill()
+    eng.step()
+    check(eng)
+    assert eng.loads_of_last_step() == eng.L * eng.batch.n_req      # the newest blocks and no others
+    eng.capture()
+    refill()
+    eng.step()
+    check(eng)
 
 
 def test_remap_without_a_deferred_free_list():

@@ -39,7 +39,8 @@ class DecodeRetrievalEngine:
         depend on each other); the step is then bounded by the block moves alone.
         attend: each layer ends with the attention of its queries over the blocks just selected, written to
         attn_out[layer].  It reads the blocks in the pool, in place of the gather; in the delta step it follows the
-        move and reads the layer's resident working set (one per layer: n_layers x the selected blocks' bytes).
+        move and reads the layer's resident working set (one per layer: n_layers x the selected blocks' bytes), whose
+        copies of the blocks that filled up since the last step are given up when the step begins.
         cache_bits: 4 or 8 keeps a quantised copy of the pool beside it (quant_pool) and attends over that; blocks that
         filled up since the last step are quantised when the step begins."""
         self.shape, self.batch, self.device = shape, batch, device
@@ -109,6 +110,8 @@ class DecodeRetrievalEngine:
                                torch.zeros((batch.n_req,), **i32)) for _ in range(self.L)]
             self.moves = ops.MoveList(n, device)
             self.max_logical = int(batch.blocks_per_req.max())
+            # the newest block of the request that each slot belongs to, by its position
+            self._newest = torch.repeat_interleave(torch.from_numpy(batch.blocks_per_req - 1), torch.from_numpy(batch.k_per_req).long()).to(device)
             self.launches_per_step = self.L * 4 + 1
         self.attend = attend
         self.quant_pool: Optional[ops.QuantKvCache] = None
@@ -147,6 +150,8 @@ class DecodeRetrievalEngine:
         ops.pool_blocks(self.kv_pool[0], ids, out_slots=slots, out_bf16=table)
         if self.quant_pool is not None:
             ops.quant_write_blocks(self.quant_pool, self.kv_pool[0], self.kv_pool[1], self.new_block_ids, out_slots=self.new_block_ids)
+        if self.delta and self.attend:             # what a working set holds of these blocks is out of date: not resident any more
+            self.slot_logical.masked_fill_(self.slot_logical == self._newest, -1)
 
     def pool_layer(self, layer: int) -> None:
         ops.pool_blocks(self.kv_pool[0], self.new_block_ids, out_slots=self.new_block_ids,
