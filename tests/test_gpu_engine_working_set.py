@@ -79,6 +79,36 @@ def test_a_block_that_filled_up_is_moved_again(kw):
     check(eng)
 
 
+@pytest.mark.parametrize("kw", [dict(cache_bits=4), dict(delta=True)])
+def test_representatives_of_the_whole_pool_renew_what_the_attention_reads(kw):
+    """prefill_pool_all says that the pool holds new blocks: the quantised copy and the working sets hold them then, too."""
+    from test_gpu_engine_attention import make as make_any
+    eng = make_any(**kw)
+    eng.make_queries()
+    eng.step()
+    check(eng, kw.get("cache_bits", 16))
+    eng.kv_pool.copy_(torch.randn(eng.kv_pool.shape, device=DEV, generator=eng.gen).to(torch.bfloat16))
+    for l in range(eng.L):
+        eng.prefill_pool_all(l)
+    eng.step()
+    check(eng, kw.get("cache_bits", 16))
+
+
+@pytest.mark.parametrize("kw", [dict(cache_bits=8), dict(delta=True)])
+def test_pooling_a_layer_renews_what_its_attention_reads(kw):
+    """pool_layer, in place of the pooling that a step begins with, says the same of the newest blocks."""
+    from test_gpu_engine_attention import make as make_any
+    eng = make_any(**kw)
+    eng.make_queries()
+    eng.step()
+    new = eng.new_block_ids.long()
+    eng.kv_pool[:, new] = torch.randn(eng.kv_pool[:, new].shape, device=DEV, generator=eng.gen).to(torch.bfloat16)
+    for l in range(eng.L):
+        eng.pool_layer(l)
+        eng.layer_step(l)
+    check(eng, kw.get("cache_bits", 16))
+
+
 def test_remap_without_a_deferred_free_list():
     """slot_free None: with as many slots as selected blocks every block is served in every round, hits stay, slots are distinct."""
     import numpy as np

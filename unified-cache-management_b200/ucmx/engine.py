@@ -127,7 +127,7 @@ class DecodeRetrievalEngine:
             self.launches_per_step += self.L * (2 if delta else 1)
             if cache_bits != 16:
                 self.quant_pool = ops.QuantKvCache.alloc(batch.n_slots, self.T, self.H, self.D, cache_bits, device)
-                ops.quant_write_blocks(self.quant_pool, self.kv_pool[0], self.kv_pool[1], self.block_table, out_slots=self.block_table)
+                self._quantise(self.block_table)
                 self.launches_per_step += 1
 
     # ---------------------------------------------------------------------------------- stages
@@ -148,18 +148,30 @@ class DecodeRetrievalEngine:
             self._pool_all = (ids, slots, self.rep_tables.view(self.L * ns, self.H, 1, self.D))
         ids, slots, table = self._pool_all
         ops.pool_blocks(self.kv_pool[0], ids, out_slots=slots, out_bf16=table)
-        if self.quant_pool is not None:
-            ops.quant_write_blocks(self.quant_pool, self.kv_pool[0], self.kv_pool[1], self.new_block_ids, out_slots=self.new_block_ids)
+        self._quantise(self.new_block_ids)
         if self.delta and self.attend:             # what a working set holds of these blocks is out of date: not resident any more
             self.slot_logical.masked_fill_(self.slot_logical == self._newest, -1)
 
+    def _quantise(self, ids: torch.Tensor) -> None:
+        """The quantised copies of these pool blocks, where there are any."""
+        if self.quant_pool is not None:
+            ops.quant_write_blocks(self.quant_pool, self.kv_pool[0], self.kv_pool[1], ids, out_slots=ids)
+
     def pool_layer(self, layer: int) -> None:
+        """Representatives of the blocks that filled up since the last step, for one layer."""
         ops.pool_blocks(self.kv_pool[0], self.new_block_ids, out_slots=self.new_block_ids,
                         out_bf16=self.rep_tables[layer])
+        self._quantise(self.new_block_ids)
+        if self.delta and self.attend:
+            self.slot_logical[layer].masked_fill_(self.slot_logical[layer] == self._newest, -1)
 
     def prefill_pool_all(self, layer: int) -> None:
-        """Representatives of every block of the pool (what the last prefill chunk does)."""
+        """Representatives of every block of the pool (what the last prefill chunk does).  What an attention reads of the pool follows:
+        the quantised copy is written anew, and no block is resident in the layer's working set."""
         ops.pool_blocks(self.kv_pool[0], self.block_table, out_slots=self.block_table, out_bf16=self.rep_tables[layer])
+        self._quantise(self.block_table)
+        if self.delta and self.attend:
+            self.slot_logical[layer].fill_(-1)
 
     def score_layer(self, layer: int, early: bool = False) -> None:
         """early: the kernel ahead in the stream writes none of the scoring inputs (it is the previous layer's top-k or
