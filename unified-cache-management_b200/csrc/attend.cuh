@@ -91,11 +91,12 @@ struct Maps {
 };
 
 // What a thread block tells the joining kernel about the item that begins in its range and goes on behind it.
-struct __align__(32) Rec {
+struct __align__(16) Rec {
     int32_t parts;                     // 0: there is none
     int32_t q0, c0, cols, h;
     int32_t pad[3];
 };
+static_assert(alignof(Rec) <= 16 && sizeof(Rec) == 32, "records lie in a workspace that starts on 16 bytes, and no more is asked of it");
 
 // One item's part inside a thread block's range, in units (leads included).
 struct Seg {
