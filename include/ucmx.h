@@ -602,8 +602,8 @@ int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_geometry* geo
  * attention over other tokens.  A query that sees nothing gets zeros and -infinity.
  * Lists (all device pointers but the struct itself): entries [offsets[r], offsets[r+1]), ascending; `total` is the capacity of
  *   the entry arrays: what lies outside [offsets[0], offsets[n_req]) is not read, so a captured launch may be replayed with fewer
- *   entries.  Offsets that do not ascend are reported (code 3); the results of such a call are not defined.  counts (or NULL) cuts
- *   a request's list short.
+ *   entries.  Offsets that do not ascend, or that lie outside [0, total], are reported (code 3); the results of such a call are
+ *   not defined, but nothing outside the lists, the workspace and out is touched.  counts (or NULL) cuts a request's list short.
  *   block_ids[e] is the physical block, negative = skip the entry; with block_ids NULL the physical block is
  *   table[table_offsets[r] + positions[e]] (the request's row of a block table; table_offsets has n_req+1 entries, table holds
  *   table_size).

@@ -22,3 +22,23 @@ def test_a_workspace_that_starts_on_16_bytes_and_no_more(fmt, H, G, D, T, counts
     out, _, tol, _ = s.want()
     R.check(s.run(workspace=ws), out, tol)
     assert bool((room[:16] == 255).all()) and bool((room[16 + need:] == 255).all())      # nothing beside it is written
+
+
+@pytest.mark.parametrize("fmt,nq", [(16, 1), (16, 5), (4, 1), (8, 3)])
+def test_every_call_with_offsets_that_lists_cannot_have_says_so(fmt, nq):
+    """Each of them by itself; nothing beside the workspace and out is written, and the next call is fine."""
+    from ucmx import _native, ops
+    s = Setup(91, fmt, 2, 8, 64, 16, [6, 90, 4, 8], [nq] * 4).tails()
+    need = ops.attention_workspace(s.q.to(DEV), 2, max_q_tokens=nq, bits=fmt).numel()
+    room = torch.full((need + (1 << 20),), 255, dtype=torch.uint8, device=DEV)
+    _native.device_error()
+    for off in ([0, 108, 1, 108, 108], [0, 1, 108, 1, 1], [0, 6, 3, 90, 40], [0, 108, 0, 108, 0], [50, 40, 30, 20, 10], [0, 2_000_000_000, -5, 7, 108],
+                [0, 6, 200, 100, 108], [0, 6, 96, 100, 109], [-1, 6, 96, 100, 108], [108, 0, 0, 0, 0]):
+        s.run(offsets=torch.tensor(off, dtype=torch.int32, device=DEV), workspace=room[:need])
+        torch.cuda.synchronize()
+        assert _native.device_error() == 3, off
+        assert bool((room[need:] == 255).all())
+    s.run(offsets=torch.tensor([3, 9, 9, 60, 108], dtype=torch.int32, device=DEV), workspace=room[:need])
+    torch.cuda.synchronize()
+    assert _native.device_error() == 0
+    s.check()

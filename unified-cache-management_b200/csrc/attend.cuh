@@ -42,6 +42,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "split.cuh"
 
 namespace ucmx {
 namespace attend {
@@ -98,45 +99,10 @@ struct __align__(16) Rec {
 };
 static_assert(alignof(Rec) <= 16 && sizeof(Rec) == 32, "records lie in a workspace that starts on 16 bytes, and no more is asked of it");
 
-// One item's part inside a thread block's range, in units (leads included).
-struct Seg {
-    int32_t begin, end;                // of the whole item
-    int32_t lo, hi;                    // the part of it
-    int32_t from, to;                  // that part's slices, counted from the item's first
-    int32_t r, h, ct;
-    int32_t first;                     // offsets[r]
-    int32_t n;                         // entries of the request's list
-};
-
-// An item's fixed cost in slices: queries in, four warps' results joined, result out.  Tiles of 16 and 32 columns have more to join
-// (24 requests of 8..40 columns: 43 us with 16, 38 with 24, 39 with 32; one column tile of 8, 4 bits, 3 requests: 13 us with 16, 14 with 24).
-constexpr int lead_of(bool tiled) { return tiled ? 24 : 16; }
-constexpr int kLeadMost = lead_of(true);
-constexpr int kMaxScan = 1023;         // requests whose column tiles are counted exactly
-// Items up to this many units, for shares of `size` units, are not split.  Where the shares are small a thread block has an item or two
-// whatever is done, and whole ones need no joining, up to 32 slices (119 requests of 6 to 18 slices: 10 us, 14 where
-// the longer of them were split; beyond 32 slices the warps' own share of an item grows: 3 requests over 4 bits 13 -> 16 us).  Where the shares are larger a whole item makes one that
-// much longer than the others (the 24 requests above, with the joining kernel of then: 41 us, 46 with 56 units).
-__host__ __device__ constexpr int whole_of(int size, int lead) { return size < 64 ? 32 + lead : size / 8 > 32 ? size / 8 : 32; }
-
-// How the units are shared out.  Request r begins at (base(r) - base(0)) * mult: base(r) = offsets[r] * spe + r * lead with mult = KV heads x
-// column tiles; or, where requests may need several tiles, base(r) = the sum of (slices + lead) x tiles of the requests before it,
-// built in shared memory, with mult = KV heads (the tiles of a request depend on its number of query tokens).
-struct Share {
-    const int32_t* scan;               // nullptr: from the offsets
-    int32_t mult, tiles;
-    int32_t zero;                      // base(0): the lists may begin anywhere in the entry arrays
-    int32_t lo, hi;                    // this thread block's units
-    int32_t size;                      // units of a thread block
-    int32_t whole;
-    int32_t step;                      // the first level of the search: every step-th base,
-    const int32_t* probes;             // 32 of them in shared memory
-};
-
 template <int LEAD>
 __device__ __forceinline__ int32_t base_of(const Params& p, const int32_t* scan, int32_t r)
 {
-    return scan ? scan[r] : max(0, min(__ldg(p.offsets + r), p.total)) * p.spe + r * LEAD;
+    return scan ? scan[r] : inside(__ldg(p.offsets + r), p.total) * p.spe + r * LEAD;
 }
 
 // The last r with base(r) <= e, and base(r), base(r+1); 31 intervals a step, the first of them at hand.
@@ -177,8 +143,8 @@ __device__ __forceinline__ void queries_of(const Params& p, int r, int& q0, int&
     }
 }
 
-// The item that holds unit `at` and the part of it that ends in this thread block; called by whole warps.  Offsets that do not
-// ascend make items that cannot be: they are passed over (n < 0) and reported.
+// The item that holds unit `at` and the part of it that ends in this thread block; called by whole warps.  Items that cannot be are passed
+// over (n < 0) and reported.
 template <int COLS, int LEAD>
 __device__ __forceinline__ Seg segment_at(const Params& p, const Share& w, int32_t at)
 {
@@ -189,38 +155,13 @@ __device__ __forceinline__ Seg segment_at(const Params& p, const Share& w, int32
         int q0, nq;
         queries_of(p, s.r, q0, nq);
         tiles = max(1, (nq * p.G + COLS - 1) / COLS);
-        s.first = max(0, min(__ldg(p.offsets + s.r), p.total));
+        s.first = inside(__ldg(p.offsets + s.r), p.total);
     } else {
         s.first = (a - s.r * LEAD) / p.spe;
     }
-    const int32_t item = w.scan ? (b - a) / tiles : b - a;       // units of one (KV head, column tile)
-    const int32_t start = (a - w.zero) * w.mult;
-    s.n = (item - LEAD) / p.spe;
-    if (item < LEAD || s.n > p.total - s.first || at < start || at - start >= item * (p.H * tiles)) {
-        if (p.err && threadIdx.x == 0) atomicExch(p.err, 3);
-        s.begin = s.lo = at;
-        s.end = s.hi = max(at + 1, w.hi);
-        s.from = s.to = 0;
-        s.h = s.ct = 0;
-        s.n = -1;
-        return s;
-    }
-    const int32_t i = (at - start) / item;
-    s.h = i / tiles;
-    s.ct = i - s.h * tiles;
-    s.begin = start + i * item;
-    s.end = s.begin + item;
-    s.lo = at;
-    s.hi = item <= w.whole || s.end < w.hi ? s.end : w.hi;
-    s.from = max(0, at - s.begin - LEAD);
-    s.to = s.hi - s.begin - LEAD;
+    if (!place(s, w, a, b, tiles, p.H, p.spe, p.total, LEAD, at) && p.err && threadIdx.x == 0) atomicExch(p.err, 3);
     return s;
 }
-
-// Does the part that begins with the item belong to this thread block?  A split item's first part goes to the one that holds its
-// first slice.
-template <int LEAD>
-__device__ __forceinline__ bool begins_here(const Share& w, const Seg& s) { return s.end - s.begin <= w.whole || s.begin + LEAD < w.hi; }
 
 // 2^x for a weight: x is at most kMaxSlack, and what is below 2^-126 of the largest weight is nothing
 __device__ __forceinline__ float exp2_fast(float x)
@@ -457,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     w.mult = p.H * p.col_tiles;
     if (X::kTiled && p.col_tiles > 1 && p.n_req <= kMaxScan) {
         constexpr int kEach = (kMaxScan + kThreads) / kThreads;
+        const int32_t most = most_units(p.H);
         int32_t v[kEach], sum = 0;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
@@ -466,27 +408,26 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                 int q0, nq;
                 queries_of(p, r, q0, nq);
                 const int32_t units = base_of<X::kLead>(p, nullptr, r + 1) - base_of<X::kLead>(p, nullptr, r);
-                if (units < X::kLead && p.err) atomicExch(p.err, 3);         // (offsets that do not ascend)
                 v[i] = max(X::kLead, units) * ((nq * p.G + X::kCols - 1) / X::kCols);
             }
-            sum += v[i];
+            sum = add_units(sum, v[i], most);
         }
-        int32_t before = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int32_t y = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += y;
+            const int32_t y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum = add_units(sum, y, most);
         }
         int32_t* const warp_sum = reinterpret_cast<int32_t*>(stat);
-        if (lane == 31) warp_sum[warp] = before;
+        if (lane == 31) warp_sum[warp] = sum;
+        int32_t before = __shfl_up_sync(0xffffffffu, sum, 1);
+        if (lane == 0) before = 0;
         __syncthreads();
-        before -= sum;
-        for (int i = 0; i < warp; ++i) before += warp_sum[i];
+        for (int i = 0; i < warp; ++i) before = add_units(before, warp_sum[i], most);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             const int r = tid * kEach + i;
             if (r <= p.n_req) scan[r] = before;
-            before += v[i];
+            before = add_units(before, v[i], most);
         }
         __syncthreads();
         w.scan = scan;
@@ -498,25 +439,16 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     probes[lane] = probe;
     __syncwarp();
     w.probes = probes;
-    w.zero = __shfl_sync(0xffffffffu, probe, 0);
-    const int32_t all = max(0, __shfl_sync(0xffffffffu, probe, 31) - w.zero) * w.mult;     // (a captured batch may use less than its capacity)
-    w.size = (int32_t)(((uint32_t)all + gridDim.x - 1u) / gridDim.x);     // (the host keeps all + grid below 2^31)
-    w.lo = min(all, (int32_t)blockIdx.x * w.size);
-    w.hi = w.lo + min(w.size, all - w.lo);
-    w.whole = whole_of(w.size, X::kLead);
+    share_out(w, __shfl_sync(0xffffffffu, probe, 0), __shfl_sync(0xffffffffu, probe, 31), blockIdx.x, gridDim.x, X::kLead);
+    // the offsets of all requests, shared out among the thread blocks: what no list can have is reported, whether or not it is met below
+    for (int r = blockIdx.x * kThreads + tid; r < p.n_req; r += gridDim.x * kThreads)
+        if (bad_offsets(__ldg(p.offsets + r), __ldg(p.offsets + r + 1), p.total) && p.err) atomicExch(p.err, 3);
     int32_t begin = w.lo;
     Seg* const head = reinterpret_cast<Seg*>(probes + 32);                // the first segment, for the loads and for the arithmetic
     static_assert(sizeof(Seg) <= 48, "a Seg has 48 bytes of shared memory");
     if (begin < w.hi) {
         Seg s = segment_at<X::kCols, X::kLead>(p, w, begin);
-        if (s.begin < begin) {
-            if (s.end - s.begin <= w.whole) {                             // the thread block before takes all of it
-                begin = s.end;
-                if (begin < w.hi) s = segment_at<X::kCols, X::kLead>(p, w, begin);
-            } else if (begin <= s.begin + X::kLead) {                        // its first slice is here
-                begin = s.lo = s.begin;
-            }
-        }
+        if (passes_over(w, s, begin, X::kLead) && begin < w.hi) s = segment_at<X::kCols, X::kLead>(p, w, begin);
         if (lane == 0) *head = s;
         __syncwarp();
     }
@@ -604,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         if (p_at >= ps.to) {
             while (!p_done && p_at >= ps.to) {
                 if (p_next < w.hi) ps = p_next == begin ? *head : segment_at<X::kCols, X::kLead>(p, w, p_next);
-                if (p_next >= w.hi || !begins_here<X::kLead>(w, ps)) {
+                if (p_next >= w.hi || !begins_here(w, ps, X::kLead)) {
                     p_done = true;
                     break;
                 }
@@ -681,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
 #pragma unroll 1
     while (at < w.hi) {
         const Seg sg = at == begin ? *head : segment_at<X::kCols, X::kLead>(p, w, at);
-        if (!begins_here<X::kLead>(w, sg)) break;
+        if (!begins_here(w, sg, X::kLead)) break;
         at = sg.hi;
         int q0, nq;
         queries_of(p, sg.r, q0, nq);
@@ -1166,7 +1098,7 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             }
         const bool whole = sg.lo == sg.begin && sg.hi == sg.end;
         if (tid == 0 && sg.lo == sg.begin && sg.hi < sg.end)
-            *rec = Rec{(sg.end - 1) / w.size - (int32_t)blockIdx.x + 1, q0, c0, cols, sg.h, {0, 0, 0}};
+            *rec = Rec{parts_of(w, sg, blockIdx.x, gridDim.x), q0, c0, cols, sg.h, {0, 0, 0}};
         float* const part = p.ws + (int64_t)(2 * blockIdx.x + (sg.lo == sg.begin ? 1 : 0)) * X::kPart;
 #pragma unroll
         for (int step = 0; step < X::kMergeSteps; ++step) {
