@@ -393,7 +393,15 @@ __global__ void __launch_bounds__(256) quant_read_kernel(const QuantParams p)
     }
 }
 
+int32_t refuse(const char* why, int32_t code = UCMX_EPARAM)
+{
+    set_last_text(why);
+    return code;
+}
+
 enum Form { kTokensForm, kBlocksForm, kReadForm };
+
+constexpr char kTooMany[] = "quantised cache: more rows than one call takes";
 
 template <int BITS, int D, int HC>
 int32_t launch_heads(QuantParams& p, Form form, int64_t groups, int chunks, cudaStream_t st)
@@ -401,7 +409,7 @@ int32_t launch_heads(QuantParams& p, Form form, int64_t groups, int chunks, cuda
     p.heads_per = ((p.H + chunks - 1) / chunks + HC - 1) / HC * HC;
     p.head_chunks = (uint32_t)((p.H + p.heads_per - 1) / p.heads_per);
     const int64_t items = groups * 2 * p.head_chunks;
-    if (items > INT32_MAX) return UCMX_EUNSUPPORTED;     // (more rows than any memory holds)
+    if (items > INT32_MAX) return refuse(kTooMany, UCMX_EUNSUPPORTED);
     p.items = (uint32_t)items;
     const unsigned grid = (unsigned)((items + 7) / 8);
     if (form == kTokensForm)
@@ -418,7 +426,8 @@ template <int BITS, int D>
 int32_t launch(QuantParams& p, Form form, cudaStream_t st)
 {
     using X = Q<BITS, D>;
-    const int64_t groups = form == kTokensForm ? (p.n + X::kTokens - 1) / X::kTokens : p.n * (p.T / X::kTokens);
+    const int64_t groups = form == kTokensForm ? p.n / X::kTokens + (p.n % X::kTokens != 0) : p.n * (p.T / X::kTokens);
+    if (groups > INT32_MAX) return refuse(kTooMany, UCMX_EUNSUPPORTED);  // (what follows is counted in 64 bits)
     // Two heads of a warp in flight as soon as that still gives every SM its 32 warps; with the few tokens of a decode step one head
     // each, over twice as many warps.  Writing, a warp goes on through its tokens' heads (finding its place costs as much as two thirds
     // of a head) as long as that leaves two rounds of warps; reading, which HBM bounds, it does not.
@@ -442,12 +451,6 @@ int32_t dispatch(QuantParams& p, const ucmx_quant_geometry* g, Form form, cudaSt
         case 1128: return launch<8, 128>(p, form, st);
         default: return launch<8, 256>(p, form, st);
     }
-}
-
-int32_t refuse(const char* why, int32_t code = UCMX_EPARAM)
-{
-    set_last_text(why);
-    return code;
 }
 
 int32_t check_cache(const void* cache, const ucmx_quant_geometry* g)
