@@ -129,3 +129,30 @@ def test_reading_back_into_blocks_that_lie_in_one_place():
     from ucmx import _native as N
     for kg, vg in ((geom(block_stride=0), geom()), (geom(), geom(block_stride=0))):
         assert N.lib.ucmx_quant_read_blocks(FAKE, qgeom(), FAKE, None, 1, FAKE, kg, FAKE, vg, None) == N.EPARAM
+
+
+@pytest.mark.parametrize("quant", [False, True])
+def test_numbers_beyond_32_bits_are_refused_by_the_python_front(quant):
+    """Cut to 32 bits they would be other sizes: 2^32 + 1 query tokens per request one, 2^32 entries none."""
+    from ucmx import ops
+    from ucmx.retrieval import _fast
+    cache = (FAKE, 4, 2 * 2176, 16, 2, 128, 4) if quant else (FAKE, 4096, 256, 16, 2, 128, 4) * 2
+    call = _fast.quant_block_attention if quant else _fast.block_attention
+    entry = ops._QUANT_BLOCK_ATTENTION if quant else ops._BLOCK_ATTENTION
+    head = [FAKE, 1024, 8, 0, 1, 1]                                        # q, stride, heads, q_offsets, tokens, tokens per request
+    lists = [FAKE, 0, FAKE, 0, 0, 0, 0, 1, 3, 0]
+    tail = [1.0, FAKE, 0, FAKE, 64, 0]                                     # (a workspace of 64 bytes: never launched)
+    assert call(entry, *head, *cache, *lists, *tail) < 0                   # EPARAM: the workspace is too small
+    for which, at in ((head, 2), (head, 4), (head, 5), (lists, 7), (lists, 8), (lists, 9)):
+        keep = which[at]
+        which[at] = keep + 2 ** 32
+        with pytest.raises(ValueError):
+            call(entry, *head, *cache, *lists, *tail)
+        which[at] = keep
+    for at in range(3, 7):
+        c = list(cache)
+        c[at] += 2 ** 32
+        with pytest.raises(ValueError):
+            call(entry, *head, *c, *lists, *tail)
+    with pytest.raises(ValueError):
+        _fast.quant_write_tokens(ops._QUANT_WRITE_TOKENS, FAKE, FAKE, 256, 256, 0, FAKE, FAKE, 4, 4352, 16, 2 + 2 ** 32, 128, 4, 0)

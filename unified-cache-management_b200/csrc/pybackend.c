@@ -254,6 +254,18 @@ static int read_numbers(PyObject* const* args, Py_ssize_t n, Py_ssize_t skip, in
     return 0;
 }
 
+/* are v[0..n) numbers that the structures and the entries hold in 32 bits? */
+static int need_int32(const int64_t* v, int n)
+{
+    for (int i = 0; i < n; ++i) {
+        if (v[i] != (int32_t)v[i]) {
+            PyErr_Format(PyExc_ValueError, "%lld is more than the 32 bits that this number has in a call", (long long)v[i]);
+            return -1;
+        }
+    }
+    return 0;
+}
+
 static ucmx_block_lists lists_of(const int64_t* v)
 {
     ucmx_block_lists l;
@@ -289,6 +301,9 @@ static PyObject* mod_block_attention(PyObject* self, PyObject* const* args, Py_s
     }
     const double scale = PyFloat_AsDouble(args[kScale]);
     if ((scale == -1.0 && PyErr_Occurred()) || read_numbers(args, kN, kScale, v) < 0) return NULL;
+    if (need_int32(v + 3, 1) < 0 || need_int32(v + 5, 2) < 0 || need_int32(v + 10, 4) < 0 || need_int32(v + 17, 4) < 0 ||
+        need_int32(v + ATTEND_HEAD + kCache + 7, 3) < 0)
+        return NULL;
     const ucmx_kv_geometry kg = geometry_of(v + 8), vg = geometry_of(v + 15);
     const ucmx_block_lists l = lists_of(v + ATTEND_HEAD + kCache);
     const int64_t* t = v + kScale;
@@ -314,6 +329,8 @@ static PyObject* mod_quant_block_attention(PyObject* self, PyObject* const* args
     }
     const double scale = PyFloat_AsDouble(args[kScale]);
     if ((scale == -1.0 && PyErr_Occurred()) || read_numbers(args, kN, kScale, v) < 0) return NULL;
+    if (need_int32(v + 3, 1) < 0 || need_int32(v + 5, 2) < 0 || need_int32(v + 10, 4) < 0 || need_int32(v + ATTEND_HEAD + kCache + 7, 3) < 0)
+        return NULL;
     const ucmx_quant_geometry g = {v[8], v[9], (int32_t)v[10], (int32_t)v[11], (int32_t)v[12], (int32_t)v[13]};
     const ucmx_block_lists l = lists_of(v + ATTEND_HEAD + kCache);
     const int64_t* t = v + kScale;
@@ -340,7 +357,7 @@ static PyObject* mod_quant_write_tokens(PyObject* self, PyObject* const* args, P
         PyErr_SetString(PyExc_TypeError, "quant_write_tokens: wrong number of arguments");
         return NULL;
     }
-    if (read_numbers(args, kN, -1, v) < 0) return NULL;
+    if (read_numbers(args, kN, -1, v) < 0 || need_int32(v + 10, 4) < 0) return NULL;
     const ucmx_quant_geometry g = {v[8], v[9], (int32_t)v[10], (int32_t)v[11], (int32_t)v[12], (int32_t)v[13]};
     int32_t st;
     Py_BEGIN_ALLOW_THREADS;
