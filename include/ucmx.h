@@ -639,7 +639,8 @@ int32_t ucmx_block_attention(const void* q, int64_t q_stride, int32_t n_q_heads,
                              const void* v_cache, const ucmx_kv_geometry* v_geom /* host */,
                              const ucmx_block_lists* lists /* host */, float scale, void* out, float* out_lse, void* workspace,
                              size_t workspace_bytes, ucmx_stream_t stream);
-/* The same over the quantised cache: K and V are what the codes stand for, without another rounding. */
+/* The same over the quantised cache: K and V are what the codes stand for, without another rounding.  A query row is held in 16 bits
+ * whose smallest step is 2^-34 of the row's largest value; bf16 values above 2^-27 of that value are exact. */
 int32_t ucmx_quant_block_attention(const void* q, int64_t q_stride, int32_t n_q_heads, const int32_t* q_offsets,
                                    int32_t n_q_tokens, int32_t max_q_tokens, const void* cache,
                                    const ucmx_quant_geometry* geom /* host */, const ucmx_block_lists* lists /* host */,

@@ -302,8 +302,9 @@ __device__ __forceinline__ uint32_t v_bytes(uint32_t w, int i)
     return sub_bf16x2(mask_or(x, 0x007f007fu, 0x43004300u), mask_or(~x, 0x00800080u, 0x43004300u));
 }
 // K's codes become fp16, whose eleven bits hold two nibble positions: half the shifts, and half or none of the subtractions.
-// (The queries can follow: a column scaled by a power of two fits fp16 to 2^-25 of its largest value.  The weights cannot:
-// their range is not bounded.)  0x6400 is 1024.0, counting in ones.  4 bits: registers i = 0, 2 hold c - 8, registers i = 1, 3
+// (The queries can follow: a column scaled by a power of two to where its largest value is 2^14 or more fits fp16 to 2^-39 of that
+// value, to 2^-35 where a sixteenth of it is held (below).  The weights cannot: their range is not bounded.)
+// 0x6400 is 1024.0, counting in ones.  4 bits: registers i = 0, 2 hold c - 8, registers i = 1, 3
 // hold 1024 + 16 c, whose 1024 + 128 the accumulator starts below (kOddOffset times those queries' sum) and whose 16 is in the
 // queries.  With that offset in all four the sums would lose four bits more.
 __device__ __forceinline__ uint32_t k_nibbles(uint32_t w, int i)
@@ -682,8 +683,10 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                 for (int i = 0; i < D / 8; ++i) most = fmaxf(most, fmaxf(fabsf(bf16lo(raw[i])), fabsf(bf16hi(raw[i]))));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                const uint32_t ex = min(max(__float_as_uint(most) >> 23, 1u), 253u);
-                const float up = __uint_as_float((254u - ex) << 23), down = __uint_as_float(ex << 23);   // powers of two: exact
+                // powers of two (exact) that bring the largest value to [2^14, 2^15): its infinity would be 2^16, and what lies 2^28 below
+                // it is still a normal number
+                const uint32_t ex = min(max(__float_as_uint(most) >> 23, 15u), 253u);
+                const float up = __uint_as_float((268u - ex) << 23), down = __uint_as_float((ex - 14u) << 23);
                 float sum = 0.f, odd = 0.f;                      // of the rounded values; `odd`: of those that meet 1024 + 16 c
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) {
