@@ -616,7 +616,8 @@ int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_geometry* geo
  *   gives each request's query tokens, at most max_q_tokens; NULL: one each.  Rows of out behind q_offsets[n_req] stay as they are.
  *   More than one query token per request needs ctx_lens.
  * n_q_heads a multiple of the cache's heads; head_dim 64, 128 or 256; any block_tokens (bf16 cache).  An infinity in a V row that
- *   is seen makes that dimension infinite or NaN.
+ *   is seen makes that dimension the same infinity (NaN beside the opposite one, and where the row's weight is below 2^-100 of
+ *   the largest).  A query all of whose scores are -infinity counts as one that sees nothing.
  * workspace: ucmx_attention_workspace_bytes(...) bytes (bits: 16 for the bf16 cache), 16-byte aligned, any contents; it depends
  *   on neither the lists nor the batch.  Launches that may overlap need workspaces of their own.  Two kernels per call (one where no list
  *   can be long enough to be split), placed with programmatic stream serialization: both wait for the end of the kernel ahead of

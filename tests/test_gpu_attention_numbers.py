@@ -33,3 +33,37 @@ def test_small_query_values_beside_a_large_one(fmt, first):
     got = ops.quant_block_attention(q.to(DEV), ops.QuantKvCache(data.to(DEV), head_dim=D, bits=fmt), dev([0, n]), block_ids=dev(range(n)), lse=lse)
     R.check(got, out, tol, "out")
     R.check(lse, want, ltol, "lse")
+
+
+@pytest.mark.parametrize("H,G,D,T,counts,nq", [
+    (2, 1, 64, 16, [3, 1], None), (2, 4, 128, 16, [5, 40], None), (1, 8, 128, 32, [4, 2], None), (1, 12, 64, 16, [6], None),
+    (1, 30, 128, 16, [7, 2], None), (1, 6, 256, 16, [3, 900], None), (1, 4, 128, 16, [5, 3], [3, 2]),
+])
+def test_an_infinity_that_is_seen_is_one(H, G, D, T, counts, nq):
+    """A sum of weights above zero times values one of which is infinite is infinite."""
+    s = Setup(81, 16, H, G, D, T, counts, nq).tails()
+    for r, (rows, blocks, ctx) in enumerate(s.lists()):
+        n = len(rows)
+        for at, d, x in ((0, 5, "inf"), (ctx - n, 6, "-inf"), (ctx // 2, 33, "inf"), (ctx // 3, D - 1, "-inf")):
+            at = min(at, ctx - n)
+            s.v16[blocks[at // T][0], at % T, :, d] = float(x)
+    s.vd = s.v16.double()
+    out, _, tol, _ = s.want()
+    assert bool(torch.isinf(out).any(-1).all()) and not bool(torch.isnan(out).any())
+    R.check(s.run(), out, tol)
+
+
+def test_scores_that_are_all_minus_infinity_count_as_unseen():
+    for G, nq in ((1, 1), (4, 1), (8, 2)):
+        s = Setup(82, 16, 2, G, 64, 16, [3, 40, 2], [nq] * 3).tails()
+        s.q[:, :G, 7] = 1.0
+        s.k16[s.ids[s.off[1]:s.off[2]].astype(int), :, 0, 7] = float("-inf")           # the second request's blocks, one head
+        s.kd = s.k16.double()
+        out, want, tol, ltol = s.want()
+        rows = slice(int(s.qoff[1]), int(s.qoff[2]))
+        assert bool(torch.isnan(out[rows, :G]).all())                                  # (the formula's own answer is no number)
+        out[rows, :G], tol[rows, :G], want[rows, :G], ltol[rows, :G] = 0.0, 0.0, float("-inf"), 0.0
+        lse = torch.zeros(s.q.shape[:2], device=DEV)
+        got = s.run(lse=lse)
+        R.check(got, out, tol)
+        R.check(lse, want, ltol)

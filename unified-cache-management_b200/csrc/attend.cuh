@@ -25,9 +25,9 @@
 // until the item ends.  The loads run ahead across items.
 //
 // Rounding.  Scores, maxima, sums and outputs are fp32.  The weights are the one operand that has to become bf16 for
-// the second product; each is split into a bf16 value and the bf16 of what is left (2^-17 relative instead of 2^-9,
-// which would be as large an error as the final rounding of the output).  With at most four columns the two halves
-// share one instruction (columns 4..7 repeat 0..3), otherwise they are two.
+// the second product; each is split into a bf16 value and the bf16 of what is left (2^-16 relative over a bf16 cache, where
+// the first half is the value next below, 2^-17 over codes; 2^-9 without, which would be as large an error as the final rounding
+// of the output).  With at most four columns the two halves share one instruction (columns 4..7 repeat 0..3), otherwise they are two.
 //
 // Measured on a B200 (128 values a head, 32 query heads on 8; device times of a call, both kernels; bytes of the listed K and V):
 //   bf16, 64 requests, 16..52 blocks of 128 tokens: 162 us, 6.3 TB/s, 0.97 of a copy's rate: HBM.  One request of 130 944 tokens:
@@ -239,6 +239,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+// Two weights (not negative) as the bf16 numbers next below them, 0 for 0: what is left of a weight above 0 is above 0, so that both halves
+// of it make an infinity of V the same infinity.
+__device__ __forceinline__ uint32_t pack_below(float lo, float hi)
+{
+    return __byte_perm(max(__float_as_uint(lo), 1u) - 1u, max(__float_as_uint(hi), 1u) - 1u, 0x7632);
 }
 __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b)
 {
@@ -949,7 +955,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
                             }
                         }
                     }
-                    const uint32_t a = pack_bf16(w[0], w[1]), b = pack_bf16(w[2], w[3]);
+                    const uint32_t a = FMT == 16 ? pack_below(w[0], w[1]) : pack_bf16(w[0], w[1]);
+                    const uint32_t b = FMT == 16 ? pack_below(w[2], w[3]) : pack_bf16(w[2], w[3]);
                     const uint32_t al = pack_bf16(w[0] - bf16lo(a), w[1] - bf16hi(a));
                     const uint32_t bl = pack_bf16(w[2] - bf16lo(b), w[3] - bf16hi(b));
                     if (DUP) {
