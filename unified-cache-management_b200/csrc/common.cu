@@ -55,8 +55,14 @@ int32_t* error_word()
 {
     std::lock_guard<std::mutex> lk(g_error_mu);
     if (!g_error_word) {
+        // the first call may be one that a graph captures: an allocation is no part of the graph, but in the capture's own mode it would
+        // end it
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
         void* p = nullptr;
-        if (cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+        const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) {
             cudaGetLastError();
             return nullptr;
         }
