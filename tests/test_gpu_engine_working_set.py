@@ -132,3 +132,27 @@ def test_remap_without_a_deferred_free_list():
                 assert resident.get((r, int(x)), s) == s
                 new[r, int(x)] = s
         resident = new
+
+
+@pytest.mark.parametrize("overlap", [False, True])
+def test_the_delta_step_alone_serves_its_whole_selection(overlap):
+    """Without an attention behind it, too: each selected block has a slot, and what is loaded is what was not resident."""
+    from ucmx.engine import DecodeRetrievalEngine
+    from ucmx.workloads import KvShape, ragged_decode_batch
+    shape = KvShape(n_q_heads=8, n_kv_heads=2, head_dim=128, block_tokens=64, n_layers=2)
+    batch = ragged_decode_batch(seed=44, n_req=6, min_ctx=512, max_ctx=4096, block_tokens=64, ratio=0.3, min_k=3)
+    eng = DecodeRetrievalEngine(shape, batch, DEV, seed=6, delta=True, overlap=overlap)
+    eng.make_queries()
+    off, newest = eng.k_offsets.tolist(), (eng.offsets[1:] - eng.offsets[:-1] - 1).tolist()
+    before = [[set() for _ in range(6)] for _ in range(2)]
+    for step in range(5):
+        eng.step()
+        for l in range(2):
+            table, sel, n = eng.remap_out[l][0].tolist(), eng.sel_ids[l].tolist(), eng.sel_counts[l].tolist()
+            for r in range(6):
+                a, b = off[r], off[r] + n[r]
+                assert sorted(table[a:b]) == list(range(a, b))            # (k is the number of slots)
+                resident = before[l][r] - {newest[r]}
+                assert int(eng.remap_out[l][3][r]) == len(set(sel[a:b]) - resident)
+                before[l][r] = set(sel[a:b])
+        eng.drift_queries(0.6)

@@ -33,14 +33,14 @@ class DecodeRetrievalEngine:
         order: order of the selected ids (best first, or ascending block position).
         delta: keep a resident working set per layer and request and move only the blocks that are new with respect
         to the previous step's selection (what ESA does, ucm/sparse/esa/esa.py:313-338): top-k of block positions in
-        ascending order -> resident-set remap -> block-to-block move of the misses.  Without attend nothing reads the
-        blocks that were moved, and all layers move into the same slots: what such a step shows is its time.
+        ascending order -> resident-set remap -> block-to-block move of the misses, all of them; copies of blocks that filled
+        up since the last step are given up when the step begins.  Without attend nothing reads the blocks that were moved,
+        and all layers move into the same slots: what such a step shows is its time.
         overlap: scoring and selection of layer l+1 run on a second stream while layer l's blocks move (they do not
         depend on each other); the step is then bounded by the block moves alone.
         attend: each layer ends with the attention of its queries over the blocks just selected, written to
         attn_out[layer].  It reads the blocks in the pool, in place of the gather; in the delta step it follows the
-        move and reads the layer's resident working set (one per layer: n_layers x the selected blocks' bytes), whose
-        copies of the blocks that filled up since the last step are given up when the step begins.
+        move and reads the layer's resident working set (one per layer: n_layers x the selected blocks' bytes).
         cache_bits: 4 or 8 keeps a quantised copy of the pool beside it (quant_pool) and attends over that; blocks that
         filled up since the last step are quantised when the step begins."""
         self.shape, self.batch, self.device = shape, batch, device
@@ -105,7 +105,6 @@ class DecodeRetrievalEngine:
             n = batch.total_k
             self.slot_phys = torch.arange(n, **i32)
             self.slot_logical = torch.full((self.L, n), -1, **i32)
-            self.slot_free = torch.ones((self.L, n), dtype=torch.uint8, device=device)
             self.remap_out = [(torch.full((n,), -1, **i32), torch.full((n,), -1, **i32), torch.full((n,), -1, **i32),
                                torch.zeros((batch.n_req,), **i32)) for _ in range(self.L)]
             self.moves = ops.MoveList(n, device)
@@ -149,7 +148,7 @@ class DecodeRetrievalEngine:
         ids, slots, table = self._pool_all
         ops.pool_blocks(self.kv_pool[0], ids, out_slots=slots, out_bf16=table)
         self._quantise(self.new_block_ids)
-        if self.delta and self.attend:             # what a working set holds of these blocks is out of date: not resident any more
+        if self.delta:             # what a working set holds of these blocks is out of date: not resident any more
             self.slot_logical.masked_fill_(self.slot_logical == self._newest, -1)
 
     def _quantise(self, ids: torch.Tensor) -> None:
@@ -162,7 +161,7 @@ class DecodeRetrievalEngine:
         ops.pool_blocks(self.kv_pool[0], self.new_block_ids, out_slots=self.new_block_ids,
                         out_bf16=self.rep_tables[layer])
         self._quantise(self.new_block_ids)
-        if self.delta and self.attend:
+        if self.delta:
             self.slot_logical[layer].masked_fill_(self.slot_logical[layer] == self._newest, -1)
 
     def prefill_pool_all(self, layer: int) -> None:
@@ -170,7 +169,7 @@ class DecodeRetrievalEngine:
         the quantised copy is written anew, and no block is resident in the layer's working set."""
         ops.pool_blocks(self.kv_pool[0], self.block_table, out_slots=self.block_table, out_bf16=self.rep_tables[layer])
         self._quantise(self.block_table)
-        if self.delta and self.attend:
+        if self.delta:
             self.slot_logical[layer].fill_(-1)
 
     def score_layer(self, layer: int, early: bool = False) -> None:
@@ -211,10 +210,9 @@ class DecodeRetrievalEngine:
 
     def remap_layer(self, layer: int) -> None:
         """Which resident slot serves each selected block, and the (pool block -> resident slot) list of the misses."""
-        # a slot per selected block: where an attention reads all of them, the misses take what the last step's selection left
-        # (its attention is over: the moves follow it on this stream)
-        free = None if self.attend else self.slot_free[layer]
-        ops.remap_resident(self.slot_logical[layer], free, self.slot_phys, self.k_offsets,
+        # a request has a slot per block that it selects, so the misses take what the last step's selection left (what read
+        # that is over: the moves follow it on this stream)
+        ops.remap_resident(self.slot_logical[layer], None, self.slot_phys, self.k_offsets,
                            self.sel_ids[layer], self.k_offsets, max_logical=self.max_logical, max_slots=self.out_stride,
                            sel_counts=self.sel_counts[layer], src_map=self.block_table, src_map_offsets=self.offsets,
                            moves=self.moves, out=self.remap_out[layer])
