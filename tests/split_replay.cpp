@@ -46,6 +46,7 @@ int request_of(const Lists& l, const Share& w, int32_t e, int32_t& first, int32_
 extern "C" int64_t replay(const int32_t* offsets, int32_t n_req, int32_t total, int32_t spe, int32_t heads, const int32_t* tiles, int32_t col_tiles,
                           int32_t lead, int32_t blocks, int64_t* out, int64_t room, int64_t* rejected, int32_t* reported)
 {
+    if (too_many_units((int64_t)total * spe + (int64_t)n_req * kLeadMost, heads, col_tiles)) return -2;      // (the host refuses it)
     Lists l{offsets, n_req, total, spe, heads, lead, tiles, col_tiles, {}};
     *reported = 0;
     for (int r = 0; r < n_req; ++r) *reported |= bad_offsets(offsets[r], offsets[r + 1], total);

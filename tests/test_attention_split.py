@@ -10,7 +10,6 @@ import pytest
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LEAD = {False: 16, True: 24}
-LIMIT = 2 ** 31 - 1 - 2 ** 20
 
 
 @pytest.fixture(scope="module")
@@ -30,14 +29,13 @@ def replay(tmp_path_factory):
         n_req = len(off) - 1
         t = None if tiles is None else np.asarray(tiles, np.int32)
         col = 1 if t is None else int(t.max())
-        units = total * spe + n_req * 24
-        assert units <= (2 ** 31 - 1) // 2 and units * heads <= (2 ** 31 - 1) // 2 and units * heads * col <= LIMIT    # what the host lets through
         room = 8 * (n_req + 1) * heads * col + 8 * blocks
         out = np.zeros((room, 10), np.int64)
         rejected, reported = C.c_int64(), C.c_int32()
         p = lambda a, ty: None if a is None else a.ctypes.data_as(C.POINTER(ty))  # noqa: E731
         n = lib.replay(p(off, C.c_int32), n_req, total, spe, heads, p(t, C.c_int32), col, LEAD[tiled or t is not None], blocks,
                        p(out, C.c_int64), C.c_int64(room), C.byref(rejected), C.byref(reported))
+        assert n != -2, "a batch that the host refuses"
         assert n >= 0, "a loop that does not end"
         rows = out[:n]
         block, r, h, ct, lo, hi, first, entries, begins, parts = rows.T

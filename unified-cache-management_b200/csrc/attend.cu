@@ -109,7 +109,7 @@ int32_t attend_common(Params& p, int bits, int32_t head_dim, const void* q, int6
     p.col_tiles = (cols + plan.cols - 1) / plan.cols;
     // the slices of all requests, heads and tiles, and a lead for each of them, are numbered in 32 bits
     const int64_t units = (int64_t)p.total * p.spe + (int64_t)p.n_req * kLeadMost;
-    if (units > INT32_MAX / 2 || units * p.H > INT32_MAX / 2 || units * p.H * p.col_tiles > kUnitLimit)
+    if (too_many_units(units, p.H, p.col_tiles))
         return refuse("attention: more than 2^31 pieces of 16 tokens in the lists of all heads", UCMX_EUNSUPPORTED);
     Maps maps = {};
     if (bits == 16 && p.total > 0) {

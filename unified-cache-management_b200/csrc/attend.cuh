@@ -447,9 +447,6 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
     __syncwarp();
     w.probes = probes;
     share_out(w, __shfl_sync(0xffffffffu, probe, 0), __shfl_sync(0xffffffffu, probe, 31), blockIdx.x, gridDim.x, X::kLead);
-    // the offsets of all requests, shared out among the thread blocks: what no list can have is reported, whether or not it is met below
-    for (int r = blockIdx.x * kThreads + tid; r < p.n_req; r += gridDim.x * kThreads)
-        if (bad_offsets(__ldg(p.offsets + r), __ldg(p.offsets + r + 1), p.total) && p.err) atomicExch(p.err, 3);
     int32_t begin = w.lo;
     Seg* const head = reinterpret_cast<Seg*>(probes + 32);                // the first segment, for the loads and for the arithmetic
     static_assert(sizeof(Seg) <= 48, "a Seg has 48 bytes of shared memory");
@@ -610,6 +607,9 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
 #pragma unroll 1
     for (int s = 0; s < X::kStages; ++s) issue(s);
     __syncwarp();
+    // the offsets of all requests, shared out among the thread blocks: what no list can have is reported, whether or not it is met below
+    for (int r = blockIdx.x * kThreads + tid; r < p.n_req; r += gridDim.x * kThreads)
+        if (bad_offsets(__ldg(p.offsets + r), __ldg(p.offsets + r + 1), p.total) && p.err) atomicExch(p.err, 3);
 
     int stage = 0;
     uint32_t parity = 0;

@@ -37,6 +37,12 @@ UCMX_HOST_DEVICE constexpr int whole_of(int size, int lead) { return size < 64 ?
 // All units of a launch stay below this, and so does what is added to them (the host refuses a batch whose lists, ascending and
 // inside their arrays, could need more).
 constexpr int32_t kUnitLimit = INT32_MAX - (1 << 20);
+// What the sum over the requests (mult = heads) stops at: more than any batch has that is not refused.
+UCMX_HOST_DEVICE int32_t most_units(int32_t heads) { return kUnitLimit / heads; }
+inline bool too_many_units(int64_t units, int64_t heads, int64_t tiles)      // on the host: for lists as long as their arrays
+{
+    return units > INT32_MAX / 2 || units * heads > INT32_MAX / 2 || units * heads * tiles > kUnitLimit - heads;
+}
 
 // How the units are shared out.  Request r begins at (base(r) - base(0)) * mult: base(r) = offsets[r] * spe + r * lead with mult = KV heads x
 // column tiles; or, where requests may need several tiles, base(r) = the sum of (slices + lead) x tiles of the requests before it,
@@ -45,7 +51,6 @@ struct Share {
     const int32_t* scan;               // nullptr: from the offsets
     int32_t mult, tiles;
     int32_t zero;                      // base(0): the lists may begin anywhere in the entry arrays
-    int32_t all;                       // units of the launch
     int32_t lo, hi;                    // this thread block's units
     int32_t size;                      // units of a thread block
     int32_t whole;
@@ -62,37 +67,34 @@ UCMX_HOST_DEVICE int32_t inside(int32_t offset, int32_t total) { return at_least
 // Offsets of one request that the lists cannot have: reported, and nothing outside the arrays or the workspace is touched for them.
 UCMX_HOST_DEVICE bool bad_offsets(int32_t x, int32_t y, int32_t total) { return x < 0 || y < x || y > total; }
 
-// Sum of units that stops at `most` (offsets that go up and down add up to more than any list has).
+// Sum of units that stops at `most` (offsets that go up and down add up to more than there are).
 UCMX_HOST_DEVICE int32_t add_units(int32_t x, int32_t y, int32_t most)
 {
     const uint32_t sum = (uint32_t)x + (uint32_t)y;
     return sum < (uint32_t)most ? (int32_t)sum : most;
 }
-// what the sum over the requests stops at, for mult = heads
-UCMX_HOST_DEVICE int32_t most_units(int32_t heads) { return kUnitLimit / heads; }
-
-// base0, base_end: base(0) and base(n_req).
+// base0, base_end: base(0) and base(n_req).  A sum that reached its end is no batch: none of it is done.
 UCMX_HOST_DEVICE void share_out(Share& w, int32_t base0, int32_t base_end, uint32_t block, uint32_t blocks, int lead)
 {
+    const bool none = base_end < base0 || (w.scan && base_end >= most_units(w.mult));
+    const int32_t all = none ? 0 : (base_end - base0) * w.mult;           // (a captured batch may use less than its capacity)
     w.zero = base0;
-    w.all = at_least(0, base_end - base0) * w.mult;                       // (a captured batch may use less than its capacity)
-    w.size = (int32_t)(((uint32_t)w.all + blocks - 1u) / blocks);         // (the host keeps all + blocks below 2^31)
-    w.lo = at_most(w.all, (int32_t)block * w.size);
-    w.hi = w.lo + at_most(w.size, w.all - w.lo);
+    w.size = (int32_t)(((uint32_t)all + blocks - 1u) / blocks);           // (the host keeps all + blocks below 2^31)
+    w.lo = at_most(all, (int32_t)block * w.size);
+    w.hi = w.lo + at_most(w.size, all - w.lo);
     w.whole = whole_of(w.size, lead);
 }
 
 // The item that holds unit `at`, and the part of it from there on that ends in this thread block.  a, b: base(r), base(r+1) of the
-// request found for it; s.r and s.first are set.  Offsets that do not ascend make items that cannot be (none, or ones that reach beyond the
-// units there are, where no thread block has room for a part): false, with a segment of nothing (n < 0) up to the end of the share.
+// request found for it; s.r and s.first are set.  Offsets that do not ascend make items that cannot be: false, with a segment of nothing
+// (n < 0) up to the end of the share.  They may also make items that begin before the first unit or end behind the last one; their slices lie
+// inside the lists all the same, and parts_of counts the thread blocks that there are.
 UCMX_HOST_DEVICE bool place(Seg& s, const Share& w, int32_t a, int32_t b, int32_t tiles, int32_t heads, int32_t spe, int32_t total, int lead, int32_t at)
 {
     const int32_t item = w.scan ? (b - a) / tiles : b - a;                // units of one (KV head, column tile)
     const int32_t start = (a - w.zero) * w.mult;
     s.n = (item - lead) / spe;
-    // (the last condition: the sums are differences of two bases times mult, so none of them leaves 32 bits)
-    if (item < lead || s.n * spe != item - lead || s.n > total - s.first || start < 0 || at < start || at - start >= item * (heads * tiles) ||
-        start + item * (heads * tiles) > w.all) {
+    if (item < lead || s.n > total - s.first || at < start || at - start >= item * (heads * tiles)) {
         s.begin = s.lo = at;
         s.end = s.hi = at_least(at + 1, w.hi);
         s.from = s.to = 0;
@@ -129,7 +131,7 @@ UCMX_HOST_DEVICE bool passes_over(const Share& w, Seg& s, int32_t& begin, int le
 // first slice.
 UCMX_HOST_DEVICE bool begins_here(const Share& w, const Seg& s, int lead) { return s.end - s.begin <= w.whole || s.begin + lead < w.hi; }
 
-// Thread blocks that hold a part of an item which begins in thread block `block` and ends behind it.
+// Thread blocks that hold a part of an item which begins in thread block `block` and ends behind it; no more than follow.
 UCMX_HOST_DEVICE int32_t parts_of(const Share& w, const Seg& s, int32_t block, int32_t blocks)
 {
     return at_most((s.end - 1) / w.size - block + 1, blocks - block);
