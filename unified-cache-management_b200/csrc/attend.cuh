@@ -12,8 +12,8 @@
 // codes, which have to pass through registers anyway.)
 //
 // Split.  The unit is a slice: up to 16 consecutive tokens of one listed block.  All slices of all (request, KV head,
-// column tile) items are laid end to end, each item behind a lead of 16 or 24 units (what beginning and ending an item costs;
-// without it 190 requests of 1 to 40 blocks took 38 us, with it 17), and cut into equal parts, one per thread block, whatever
+// column tile) items are laid end to end, each item behind a lead of 16 or 24 units (what beginning and ending an item costs:
+// 190 requests of 1 to 40 blocks take 26.6 us with a lead of 1, 14.6 so), and cut into equal parts, one per thread block, whatever
 // the lengths of the requests are.  A short item stays with the thread block that it begins in; a longer one that crosses
 // cuts leaves partial results (running maximum, sum, unnormalised output) in the workspace, which a second small kernel joins
 // in order.  The workspace needs no initial state, and the order of the sums is fixed by the shapes, so results do not change
@@ -31,9 +31,9 @@
 //
 // Measured on a B200 (128 values a head, 32 query heads on 8; device times of a call, both kernels; bytes of the listed K and V):
 //   bf16, 64 requests, 16..52 blocks of 128 tokens: 162 us, 6.3 TB/s, 0.97 of a copy's rate: HBM.  One request of 130 944 tokens:
-//   91 us, 5.9 TB/s.  8 bits, the first batch: 92 us, 5.8 TB/s: HBM, and eight warps per SM.
-//   4 bits, 32 requests of 120..500 blocks of 64 tokens: 139 us, 4.3 TB/s: the integer pipe (codes to bf16: 326 instructions per
-//   slice, 147 of them on a pipe of half rate; 58 % of the issue slots).  Shortest call, 40 slices: 6 us.
+//   92 us, 5.8 TB/s.  8 bits, the first batch: 92 us, 5.7 TB/s: HBM, and eight warps per SM.
+//   4 bits, 32 requests of 120..500 blocks of 64 tokens: 139 us, 4.3 TB/s: turning codes into 16-bit operands (326 instructions per
+//   slice; 62 % of the issue slots, 55 % of the integer pipe's cycles).  Shortest call, 40 slices: 6 us.
 #pragma once
 
 #include <cuda.h>
@@ -489,7 +489,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
             if (X::kTiled || p.ctx) queries_of(p, ps.r, q0, nq);
             if (X::kTiled) {
                 // the tile's query rows on their way into L2: the item begins some steps from here, and reads them before all else
-                // (44 requests with 32 columns: 68 -> 65 us; a tile of 8 has too few of them: the shortest calls lose 0.2 us)
+                // (44 requests with 32 columns: 72 -> 69 us, 100 with 56 columns 137 -> 129; a tile of 8 has too few of them: the
+                // shortest calls lose 0.2 us)
                 static_assert(X::kCols * (D / 64) <= kThreads, "a line per thread");
                 const int line = warp * 32 + lane, cc = ps.ct * X::kCols + line / (D / 64);
                 if (line < X::kCols * (D / 64) && cc < nq * p.G) {
@@ -1182,8 +1183,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
 // Joins the partial results of the item that begins in thread block blockIdx.x and ends in a later one, eight columns per
 // blockIdx.y.  Part 0 is that block's trailing result, the others are leading ones.  Latency is all there is to it, and as many
 // thread blocks as can be at once: a few parts are joined column by column, one warp each; many of them by all warps together, two
-// columns at a time.  (All warps over every item, eight columns in registers: 44 requests with 32 columns spent 21 us here, 6 so;
-// 6 requests of 6 650..29 600 tokens, 256 values a head, 25 parts: 12 us.)
+// columns at a time.  (All warps over every item, eight columns in registers: 44 requests with 32 columns spent 21 us here, 5.7 so;
+// 6 requests of 6 650..29 600 tokens, 256 values a head, 25 parts: 12 us; one request of 130 944 tokens, 37 parts a head: 11 us.)
 template <int D, int COLS>
 __global__ void __launch_bounds__(256, 4) attend_join_kernel(const Params p, const int n_blocks)
 {
@@ -1339,10 +1340,10 @@ __global__ void __launch_bounds__(256, 4) attend_join_kernel(const Params p, con
 // ---------------------------------------------------------------------------------------------------- host side
 
 // Columns of a tile for `cols` query rows of a KV head.  A tile reads K and V once and pays for its matrix instructions and
-// weights: a tile of 32 takes about 1.5 times one of 16 (24 requests of 6400 tokens, 128 values a head, 8 heads: 32 columns 138 us
-// in one tile, 202 us in two; 40 columns 241 us in two, 230 us in three).  Codes are decoded once per tile, but beside 128
-// accumulators there are no registers left for it: 16 is their widest (8 requests of 8192 tokens, 32 columns: 72 us against 94 us
-// with 32), as it is with 256 values a head.
+// weights: a tile of 32 takes about 1.3 times one of 16 (24 requests of 6400 tokens, 128 values a head, 8 heads: 32 columns 129 us
+// in one tile, 202 us in two; 40 columns 235 us in two, 223 us in three).  Codes are decoded once per tile, but beside 128
+// accumulators there are no registers left for it: 16 is their widest (8 requests of 8192 tokens, 32 columns, 4 bits: 67 us against
+// 78 us with 32), as it is with 256 values a head.
 inline int tile_cols(int cols, int head_dim, int format)
 {
     if (cols <= 4) return 4;

@@ -14,9 +14,9 @@
 // exact in fp32: where it is half a step or more (ties, and quotients the reciprocal put on the wrong side) the code is settled by
 // it and by what the difference x - zero was rounded by.  A division per value, and fp64 for the ties, were the bound of this kernel.
 //
-// Measured on a B200 (8 heads of 128 values): 300 blocks of 128 tokens to 8 bits in 67 us (3.6 TB/s of both sides' bytes; floor
-// 36 us), back in 41 us (5.8 TB/s); 8144 tokens to 4 bits in 19 us, back in 11 us.  Writing is bound by instructions (74 per row
-// and lane, 60 % of the issue slots), reading by HBM.
+// Measured on a B200 (8 heads of 128 values): 300 blocks of 128 tokens to 8 bits in 66 us (3.6 TB/s of both sides' bytes; floor
+// 36 us), back in 42 us (5.7 TB/s); 8144 tokens to 4 bits in 20 us, back in 12 us.  Writing is bound by instructions (74 warp
+// instructions a row, 69 % of the issue slots; 4 bits 61 %); reading comes within a sixth of the copy's rate with 81 % of them.
 #include "common.cuh"
 
 namespace ucmx {

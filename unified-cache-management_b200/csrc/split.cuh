@@ -24,14 +24,14 @@ struct Seg {
 };
 
 // An item's fixed cost in slices: queries in, four warps' results joined, result out.  Tiles of 16 and 32 columns have more to join
-// (24 requests of 8..40 columns: 43 us with 16, 38 with 24, 39 with 32; one column tile of 8, 4 bits, 3 requests: 13 us with 16, 14 with 24).
+// (24 requests of 8..40 columns: 41.8 us with 16, 37.4 with 24, 38.4 with 32; a tile of 4, 4 bits, 3 requests: 11.4 us with 16, 12.5 with 24).
 constexpr int lead_of(bool tiled) { return tiled ? 24 : 16; }
 constexpr int kLeadMost = lead_of(true);
 constexpr int kMaxScan = 1023;         // requests whose column tiles are counted exactly
 // Items up to this many units, for shares of `size` units, are not split.  Where the shares are small a thread block has an item or two
-// whatever is done, and whole ones need no joining, up to 32 slices (119 requests of 6 to 18 slices: 10 us, 14 where
-// the longer of them were split; beyond 32 slices the warps' own share of an item grows: 3 requests over 4 bits 13 -> 16 us).  Where the shares are larger a whole item makes one that
-// much longer than the others (the 24 requests above, with the joining kernel of then: 41 us, 46 with 56 units).
+// whatever is done, and whole ones need no joining, up to 32 slices (119 requests of 6 to 18 slices: 10.2 us, 11.7 where the longer of
+// them are split; beyond 32 slices the warps' own share of an item grows: 3 requests over 4 bits 17.7 us with 64, 11.4 so).  Where the
+// shares are larger a whole item makes one that much longer than the others (the 24 requests above: 42.8 us with 56 units, 37.4 so).
 UCMX_HOST_DEVICE constexpr int whole_of(int size, int lead) { return size < 64 ? 32 + lead : size / 8 > 32 ? size / 8 : 32; }
 
 // All units of a launch stay below this, and so does what is added to them (the host refuses a batch whose lists, ascending and
