@@ -156,3 +156,21 @@ def test_the_delta_step_alone_serves_its_whole_selection(overlap):
                 assert int(eng.remap_out[l][3][r]) == len(set(sel[a:b]) - resident)
                 before[l][r] = set(sel[a:b])
         eng.drift_queries(0.6)
+
+
+@pytest.mark.parametrize("overlap", [False, True])
+def test_delta_steps_with_host_buffers_attend_to_their_selection(overlap):
+    """The end-to-end step, launched and from its graph: queries and a refilled block new each time."""
+    eng = make(overlap=overlap)
+    eng.make_queries()
+    eng.alloc_host()
+    new = eng.new_block_ids.long()
+    for step in range(5):
+        if step == 2:
+            eng.capture_host()
+        eng.kv_pool[:, new] = torch.randn(eng.kv_pool[:, new].shape, device=DEV, generator=eng.gen).to(torch.bfloat16)
+        noise = torch.randn(eng.q_host.shape, generator=torch.Generator().manual_seed(step))
+        eng.q_host.copy_((0.7 * eng.q_host.float() + 0.7 * noise).to(torch.bfloat16))
+        torch.cuda.synchronize()
+        eng.step_host()
+        check(eng)
