@@ -614,6 +614,7 @@ int32_t ucmx_quant_read_blocks(const void* cache, const ucmx_quant_geometry* geo
  * An id beyond its cache or table is dropped and reported (ucmx_device_error code 3).
  * q is bf16 [n_q_tokens, n_q_heads, head_dim], q_stride elements between tokens (a multiple of 8).  q_offsets (n_req+1 entries)
  *   gives each request's query tokens, at most max_q_tokens; NULL: one each.  Rows of out behind q_offsets[n_req] stay as they are.
+ *   Offsets that do not ascend, lie outside the queries or give a request more tokens are reported (code 3), its result is not defined.
  *   More than one query token per request needs ctx_lens.
  * n_q_heads a multiple of the cache's heads; head_dim 64, 128 or 256; any block_tokens (bf16 cache).  An infinity in a V row that
  *   is seen makes that dimension the same infinity (NaN beside the opposite one, and where the row's weight is below 2^-100 of

@@ -42,3 +42,20 @@ def test_every_call_with_offsets_that_lists_cannot_have_says_so(fmt, nq):
     torch.cuda.synchronize()
     assert _native.device_error() == 0
     s.check()
+
+
+@pytest.mark.parametrize("fmt,G", [(16, 16), (16, 1), (4, 8)])
+def test_query_offsets_that_batches_cannot_have_are_reported_wherever_they_stand(fmt, G):
+    """A request whose query tokens go backwards, are more than the call allows or lie outside the queries: code 3, whichever request it is."""
+    from ucmx import _native
+    n = 40
+    s = Setup(92, fmt, 2, G, 64, 16, [3] * n, [3] * n).tails()
+    good = s.qoff.tolist()
+    _native.device_error()
+    for at, value in ((1, -1), (9, 0), (20, 80), (33, 10), (39, 113), (40, 121), (40, 2 ** 31 - 1), (17, -2 ** 31), (40, 100), (40, -5), (0, -3)):
+        off = list(good)
+        off[at] = value
+        s.run(q_offsets=torch.tensor(off, dtype=torch.int32, device=DEV))
+        torch.cuda.synchronize()
+        assert _native.device_error() == 3, (at, value)
+    s.check()

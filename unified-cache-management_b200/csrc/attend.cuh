@@ -127,6 +127,12 @@ __device__ __forceinline__ int request_of(const Params& p, const Share& w, int32
     }
 }
 
+// Query rows [q0, end) that no request of this call can have.
+__device__ __forceinline__ bool bad_queries(const Params& p, int32_t q0, int32_t end)
+{
+    return q0 < 0 || end < q0 || end > p.n_q_tokens || end - q0 > p.max_q;
+}
+
 // Query rows of request r: first row and how many (clamped to the query tensor and to max_q).
 __device__ __forceinline__ void queries_of(const Params& p, int r, int& q0, int& nq)
 {
@@ -135,11 +141,12 @@ __device__ __forceinline__ void queries_of(const Params& p, int r, int& q0, int&
         nq = r < p.n_q_tokens ? 1 : 0;
         return;
     }
+    const int32_t end = __ldg(p.q_offsets + r + 1);
     q0 = __ldg(p.q_offsets + r);
-    nq = __ldg(p.q_offsets + r + 1) - q0;
-    if (q0 < 0 || nq < 0 || nq > p.max_q || q0 + (int64_t)nq > p.n_q_tokens) {
+    nq = (int)((uint32_t)end - (uint32_t)q0);
+    if (bad_queries(p, q0, end)) {
         if (p.err && threadIdx.x == 0) atomicExch(p.err, 3);
-        nq = q0 < 0 || q0 >= p.n_q_tokens ? 0 : max(0, min(min(nq, p.max_q), p.n_q_tokens - q0));
+        nq = q0 < 0 || q0 >= p.n_q_tokens || end <= q0 ? 0 : min(min(nq, p.max_q), p.n_q_tokens - q0);
     }
 }
 
@@ -608,9 +615,12 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
 #pragma unroll 1
     for (int s = 0; s < X::kStages; ++s) issue(s);
     __syncwarp();
-    // the offsets of all requests, shared out among the thread blocks: what no list can have is reported, whether or not it is met below
+    // the offsets of all requests, shared out among the thread blocks: what no list and no batch can have is reported, whether or not it is
+    // met below
     for (int r = blockIdx.x * kThreads + tid; r < p.n_req; r += gridDim.x * kThreads)
-        if (bad_offsets(__ldg(p.offsets + r), __ldg(p.offsets + r + 1), p.total) && p.err) atomicExch(p.err, 3);
+        if ((bad_offsets(__ldg(p.offsets + r), __ldg(p.offsets + r + 1), p.total) ||
+             (p.q_offsets && bad_queries(p, __ldg(p.q_offsets + r), __ldg(p.q_offsets + r + 1)))) && p.err)
+            atomicExch(p.err, 3);
 
     int stage = 0;
     uint32_t parity = 0;
