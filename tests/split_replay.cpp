@@ -100,3 +100,5 @@ extern "C" int64_t replay(const int32_t* offsets, int32_t n_req, int32_t total, 
     }
     return n;
 }
+
+extern "C" int32_t row_holds(int32_t t0, int32_t t1, int32_t size, int32_t at) { return in_row(t0, t1, size, at); }

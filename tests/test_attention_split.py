@@ -46,6 +46,7 @@ def replay(tmp_path_factory):
         assert bool(((parts >= 0) & (block + parts <= blocks)).all()), "more parts than thread blocks"
         return rows, rejected.value, bool(reported.value)
 
+    run.lib = lib
     return run
 
 
@@ -144,3 +145,14 @@ def test_any_offsets_at_all(replay, seed):
         _, _, reported = replay(off, total, spe, heads, int(rng.choice([1, 22, 592])), tiles)
         off = off.astype(np.int64)
         assert reported == bool((off < 0).any() or (off > total).any() or (np.diff(off) < 0).any())
+
+
+def test_places_in_a_row_of_a_block_table(replay):
+    """A place is looked up where it lies inside its row and inside the table, whatever the row's offsets are: no difference of them wraps."""
+    ends = [-2 ** 31, -2 ** 31 + 1, -7, -1, 0, 1, 5, 6, 90, 100, 101, 2 ** 30, 2 ** 31 - 2, 2 ** 31 - 1]
+    for t0 in ends:
+        for t1 in ends:
+            for size in (0, 1, 100, 2 ** 31 - 1):
+                for at in (0, 1, 4, 94, 99, 100, 2 ** 31 - 1):
+                    want = t0 >= 0 and t0 + at < min(t1, size)
+                    assert replay.lib.row_holds(t0, t1, size, at) == want, (t0, t1, size, at)

@@ -59,3 +59,23 @@ def test_query_offsets_that_batches_cannot_have_are_reported_wherever_they_stand
         torch.cuda.synchronize()
         assert _native.device_error() == 3, (at, value)
     s.check()
+
+
+def test_rows_of_a_block_table_that_begin_or_end_anywhere():
+    """Table offsets beyond the table, backwards and at the ends of their type: the entries are dropped and reported."""
+    import numpy as np
+    from ucmx import _native
+    for fmt in (16, 4):
+        s = Setup(93, fmt, 2, 4, 128, 16, [6, 5])
+        table = s.ids.copy()
+        s.positions = np.asarray([5, 0, 2, 4, 1, 3, 0, 4, 2, 1, 3], np.int32)
+        for off, held in (([0, 6, 11], (6, 5)), ([0, 5, -2 ** 31], (5, 0)), ([-2 ** 31, 6, 11], (0, 5)), ([2 ** 31 - 1, 6, 2 ** 31 - 1], (0, 5)),
+                          ([3, 2, 4], (0, 2)), ([-1, 6, 9], (0, 3))):
+            row = [(off[0], held[0]), (off[1], held[1])]
+            s.ids = np.asarray([table[row[i // 6][0] + p] if p < row[i // 6][1] else -1 for i, p in enumerate(s.positions)], np.int32)
+            want = s.want()
+            _native.device_error()
+            got = s.run(block_ids=None, block_table=torch.from_numpy(table).to(DEV), table_offsets=torch.tensor(off, dtype=torch.int32, device=DEV))
+            torch.cuda.synchronize()
+            assert _native.device_error() == (0 if held == (6, 5) else 3), off
+            R.check(got, want[0], want[2], str(off))

@@ -514,8 +514,8 @@ __global__ void __launch_bounds__(kThreads, Traits<FMT, D, NT, DUP>::kOcc) atten
         my_flags = 0;
         if (!mine || e >= p_entries || pos_block < 0) return;
         if (!p.block_ids) {
-            const int32_t t0 = __ldg(p.table_offsets + ps.r), t1 = min(__ldg(p.table_offsets + ps.r + 1), p.table_size);
-            if (t0 < 0 || pos_block >= t1 - t0) {
+            const int32_t t0 = __ldg(p.table_offsets + ps.r);
+            if (!in_row(t0, __ldg(p.table_offsets + ps.r + 1), p.table_size, pos_block)) {
                 if (p.err) atomicExch(p.err, 3);
                 return;
             }

@@ -67,6 +67,12 @@ UCMX_HOST_DEVICE int32_t inside(int32_t offset, int32_t total) { return at_least
 // Offsets of one request that the lists cannot have: reported, and nothing outside the arrays or the workspace is touched for them.
 UCMX_HOST_DEVICE bool bad_offsets(int32_t x, int32_t y, int32_t total) { return x < 0 || y < x || y > total; }
 
+// Does place `at` (not negative) lie in the row [t0, t1) of a table of `size` entries?  t0 and t1 may be anything.
+UCMX_HOST_DEVICE bool in_row(int32_t t0, int32_t t1, int32_t size, int32_t at)
+{
+    return t0 >= 0 && (int64_t)t0 + at < at_most(t1, size);
+}
+
 // Sum of units that stops at `most` (offsets that go up and down add up to more than there are).
 UCMX_HOST_DEVICE int32_t add_units(int32_t x, int32_t y, int32_t most)
 {
